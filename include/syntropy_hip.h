@@ -30,6 +30,7 @@ extern "C" {
 #define SYN_E_WORKSPACE 3    /* the workspace is smaller than the call needs */
 #define SYN_E_DEVICE 4       /* the HIP runtime refused the launch */
 
+#define SYN_F32 0
 #define SYN_F16 1
 #define SYN_BF16 30
 #define SYN_Q4_0 2
@@ -185,6 +186,74 @@ int syn_logits_workspace_bytes(uint32_t layout, int32_t wtype, uint32_t rows, ui
 int syn_logits(uint32_t layout, int32_t wtype, const void* head, uint64_t head_bytes, uint32_t vocab,
                uint32_t hidden, const float* g, float eps, const float* x, uint32_t rows, float* y, void* ws,
                uint64_t ws_bytes, void* stream);
+
+/* ---- Products over int8 weights with a scale a channel ----------------------------------------
+ * W is int8 codes [rows][k_in], rows w_stride bytes apart (a multiple of 16, at least k_in; the first
+ * on 16 bytes), with an F32 scale a row (channel) and, if `bias` is not NULL, an F32 bias a row.  The
+ * activations x [rows, k_in] (F32, F16 or BF16, rows x_stride values apart, each value at its natural
+ * alignment) are quantized inside the call, a scale a token t:
+ *   a = max |x_t|, s = a / 127, i = 1 / s (0 where s is 0 or 1 / s infinite), q = rint(x i),
+ * each one IEEE F32 operation, rint to the nearest even; a row with a NaN or an infinity has the scale
+ * NaN and codes 0.  S = sum of q_tk w_ok, exact in I32 (k_in <= 131072), and
+ *   y_to = (S s_t) s_o (+ bias_o),
+ * the sum converted and each product and sum rounded to F32, then rounded to y's type.  The value does
+ * not depend on the row count, the strides or the other rows.  w_bytes, the view's length, has to reach
+ * the last row's last code; up to 15 bytes behind a row's codes, in its last 16-byte piece, may be read
+ * whatever they hold.  y may not overlap an operand.  No counterpart in the reference.
+ * syn_i8_quantize: rows of x to codes (rows code_stride bytes apart, a multiple of 16, at least k; zeros
+ *   behind a row's last code up to a multiple of 128 or the stride, whichever is less) and scales [rows]:
+ *   a token's rows, or a weight matrix's, whose rows are its channels.
+ * syn_i8_gemv: the product, W [n_out, k_in] to y [rows, n_out] (F32, F16 or BF16, rows y_stride values
+ *   apart).
+ * syn_i8_gate_up_act: W [2 n_out, k_in] holds gate rows, then up rows: y = silu(g) u of the two F32
+ *   values, silu with the reference's software exp (crates/kernels/src/reference/math.rs:82-84), the
+ *   product rounded once more to y's type.
+ * syn_i8_act_quantize, then syn_i8_gemv_quantized: the product's two halves over a workspace of
+ *   syn_i8_gemv_workspace_bytes, for several matrices on the same rows (one whose products share it one
+ *   after another; of the largest workspace of them, else K may be split less, to the same values).
+ * syn_i8_logits: RmsNorm of F32 rows as syn_rms_norm (k_in <= 16384), then the head as syn_i8_gemv; the
+ *   workspace holds the normalised rows first.
+ * Workspaces are 256-byte aligned; gated is 1 for syn_i8_gate_up_act, else 0. */
+#define SYN_I8_MAX_K 131072
+int syn_i8_quantize(int32_t xtype, const void* x, uint64_t x_stride, uint32_t rows, uint32_t k, int8_t* codes,
+                    uint64_t code_stride, float* scales, void* stream);
+int syn_i8_gemv_workspace_bytes(uint32_t n_out, uint32_t k_in, uint32_t rows, int32_t gated, uint64_t* bytes);
+int syn_i8_gemv(const int8_t* w, uint64_t w_bytes, uint64_t w_stride, const float* w_scales, const float* bias,
+                uint32_t n_out, uint32_t k_in, int32_t xtype, const void* x, uint64_t x_stride, uint32_t rows,
+                int32_t ytype, void* y, uint64_t y_stride, void* ws, uint64_t ws_bytes, void* stream);
+int syn_i8_gate_up_act(const int8_t* w, uint64_t w_bytes, uint64_t w_stride, const float* w_scales, const float* bias,
+                       uint32_t n_out, uint32_t k_in, int32_t xtype, const void* x, uint64_t x_stride, uint32_t rows,
+                       int32_t ytype, void* y, uint64_t y_stride, void* ws, uint64_t ws_bytes, void* stream);
+int syn_i8_act_quantize(int32_t xtype, const void* x, uint64_t x_stride, uint32_t rows, uint32_t k_in, void* ws,
+                        uint64_t ws_bytes, void* stream);
+int syn_i8_gemv_quantized(const int8_t* w, uint64_t w_bytes, uint64_t w_stride, const float* w_scales,
+                          const float* bias, uint32_t n_out, uint32_t k_in, uint32_t rows, int32_t ytype, void* y,
+                          uint64_t y_stride, void* ws, uint64_t ws_bytes, void* stream);
+int syn_i8_logits_workspace_bytes(uint32_t vocab, uint32_t hidden, uint32_t rows, uint64_t* bytes);
+int syn_i8_logits(const int8_t* head, uint64_t head_bytes, uint64_t head_stride, const float* head_scales,
+                  uint32_t vocab, uint32_t hidden, const float* g, float eps, const float* x, uint32_t rows, float* y,
+                  void* ws, uint64_t ws_bytes, void* stream);
+
+/* ---- Log probabilities of given tokens -----------------------------------------------------------
+ * For each row of logits x [rows, vocab] (F32, F16 or BF16, rows x_stride values apart; -infinity hides
+ * a token), with z = x scale (scale: the inverse of a sampling temperature, finite and above 0):
+ *   logprob [rows] F32: log softmax(z) at tokens[row];
+ *   rank [rows] I32: how many of the row's logits are greater than the token's (0: none is);
+ *   entropy [rows] F32: of softmax(z), in nats;
+ *   top_ids I32, top_logprobs F32 [rows, top]: the `top` (0 to 64, at most vocab) greatest logits' indices,
+ *     greatest first, the lower index first among equals, and their log probabilities.
+ * tokens are I32 or, with token_bytes 8, I64.  A negative one asks for none: logprob 0, rank -1; one of
+ * vocab or more gives NaN and -1.  Where every logit of a row is -infinity, its log probabilities are
+ * -infinity and its entropy 0; a NaN or +infinity in it makes its log probabilities and its entropy NaN.
+ * Among the greatest a NaN stands above +infinity; compared for the rank it is neither greater nor less.
+ * Sums are held in F32 (rank: exact).  A row's results do not depend on the other rows.
+ * ws: 256-byte aligned, syn_token_logprobs_workspace_bytes.  No counterpart in the reference. */
+#define SYN_LOGPROBS_MAX_TOP 64
+int syn_token_logprobs_workspace_bytes(int32_t xtype, uint32_t rows, uint32_t vocab, uint32_t top, uint64_t* bytes);
+int syn_token_logprobs(int32_t xtype, const void* x, uint64_t x_stride, uint32_t rows, uint32_t vocab,
+                       const void* tokens, uint32_t token_bytes, float scale, uint32_t top, float* logprob,
+                       int32_t* rank, float* entropy, int32_t* top_ids, float* top_logprobs, void* ws,
+                       uint64_t ws_bytes, void* stream);
 
 /* ---- Prefill GEMM ---------------------------------------------------------------------------
  * Q4_K weights times many activation rows on the matrix cores, each output bit-identical to

@@ -68,6 +68,16 @@ def lib():
         "syn_rms_norm": [vp, vp, u32, u32, C.c_float, vp, vp],
         "syn_logits_workspace_bytes": [u32, i32, u32, u32, u32, C.POINTER(C.c_uint64)],
         "syn_logits": [u32, i32, vp, u64, u32, u32, vp, C.c_float, vp, u32, vp, vp, u64, vp],
+        "syn_i8_quantize": [i32, vp, u64, u32, u32, vp, u64, vp, vp],
+        "syn_i8_gemv_workspace_bytes": [u32, u32, u32, i32, C.POINTER(C.c_uint64)],
+        "syn_i8_gemv": [vp, u64, u64, vp, vp, u32, u32, i32, vp, u64, u32, i32, vp, u64, vp, u64, vp],
+        "syn_i8_gate_up_act": [vp, u64, u64, vp, vp, u32, u32, i32, vp, u64, u32, i32, vp, u64, vp, u64, vp],
+        "syn_i8_act_quantize": [i32, vp, u64, u32, u32, vp, u64, vp],
+        "syn_i8_gemv_quantized": [vp, u64, u64, vp, vp, u32, u32, u32, i32, vp, u64, vp, u64, vp],
+        "syn_i8_logits_workspace_bytes": [u32, u32, u32, C.POINTER(C.c_uint64)],
+        "syn_i8_logits": [vp, u64, u64, vp, u32, u32, vp, C.c_float, vp, u32, vp, vp, u64, vp],
+        "syn_token_logprobs_workspace_bytes": [i32, u32, u32, u32, C.POINTER(C.c_uint64)],
+        "syn_token_logprobs": [i32, vp, u64, u32, u32, vp, u32, C.c_float, u32, vp, vp, vp, vp, vp, vp, u64, vp],
         "syn_moe_route": [vp, vp, u32, u32, u32, u32, i32, vp, vp, vp, vp],
         "syn_moe_pack": [vp, u32, u32, u32, vp, vp, vp, vp],
         "syn_moe_grouped_workspace_bytes": [i32, u32, u32, u32, u32, u32, C.POINTER(C.c_uint64)],

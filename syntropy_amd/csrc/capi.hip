@@ -9,6 +9,7 @@
 
 #include "../../include/syntropy_hip.h"
 #include "capi_rows.hpp"
+#include "int8.hpp"
 #include "kernels.hpp"
 
 #define SYN_EXPORT extern "C" __attribute__((visibility("default")))
@@ -1017,6 +1018,239 @@ SYN_EXPORT int syn_dequantize(int32_t wtype, const void* src, uint64_t src_bytes
     if (!src || !out) return fail(SYN_E_INVALID, "%s: null operand", W);
     syn::launch_dequantize(wtype, (const uint8_t*)src, src_bytes / bb * syn::block_elems(wtype), out,
                            (hipStream_t)stream);
+    return check_launch(W);
+}
+
+// ---- int8 products with a scale a token and a channel, log probabilities ------------------------
+
+namespace {
+
+int elem_bytes(int32_t ty) { return ty == SYN_F32 ? 4 : 2; }
+
+int check_values(const char* W, const char* what, int32_t ty, const void* p, uint64_t stride, uint64_t rows, uint64_t n) {
+    if (ty != SYN_F32 && !float_type(ty)) return fail(SYN_E_UNSUPPORTED, "%s: %s of type %d is not F32, F16 or BF16", W, what, ty);
+    if (!p) return fail(SYN_E_INVALID, "%s: null %s", W, what);
+    if (!aligned(p, elem_bytes(ty))) return fail(SYN_E_INVALID, "%s: %s is not aligned to its values", W, what);
+    if (rows > 1 && stride < n)
+        return fail(SYN_E_INVALID, "%s: %s has rows of %llu values %llu apart", W, what, (unsigned long long)n, (unsigned long long)stride);
+    if (stride > (1ull << 40)) return fail(SYN_E_INVALID, "%s: the stride of %s is too large", W, what);
+    return SYN_OK;
+}
+
+int check_i8_shape(const char* W, uint64_t w_rows, uint32_t k, uint32_t rows) {
+    if (k == 0 || k > SYN_I8_MAX_K) return fail(SYN_E_UNSUPPORTED, "%s: rows of %u values (1 to %d)", W, k, SYN_I8_MAX_K);
+    if (w_rows > 0x7FFFFF00ull || rows > 0x7FFFFF00u) return fail(SYN_E_INVALID, "%s: too many rows", W);
+    return SYN_OK;
+}
+
+uint64_t i8_ws_bytes(uint64_t w_rows, uint32_t k, uint32_t rows, int gated) {
+    if (rows == 0 || w_rows == 0) return 0;
+    uint64_t b = syn::i8_act_layout(rows, k).partial;
+    const uint64_t splits = (uint64_t)syn::i8_splits((int)w_rows, (int)k, (int)rows, gated);
+    if (splits > 1) b += 4 * splits * rows * w_rows;
+    return syn::align_up(b, 256);
+}
+
+int check_ws(const char* W, const void* ws, uint64_t have, uint64_t need) {
+    if (!ws || !aligned(ws, 256)) return fail(SYN_E_INVALID, "%s: the workspace must be 256-byte aligned", W);
+    if (have < need)
+        return fail(SYN_E_WORKSPACE, "%s: the workspace holds %llu bytes, the call needs %llu", W, (unsigned long long)have,
+                    (unsigned long long)need);
+    return SYN_OK;
+}
+
+// The product over w_rows = n_out (1 + gated) rows of W; with x null over rows quantized into ws before.
+int i8_product(const char* W, int gated, const int8_t* w, uint64_t w_bytes, uint64_t w_stride, const float* w_scales,
+               const float* bias, uint32_t n_out, uint32_t k_in, int32_t xtype, const void* x, uint64_t x_stride,
+               bool quantized, uint32_t rows, int32_t ytype, void* y, uint64_t y_stride, void* ws, uint64_t ws_bytes,
+               void* stream) {
+    const uint64_t w_rows = (uint64_t)n_out * (gated ? 2 : 1);
+    if (int rc = check_i8_shape(W, w_rows, k_in, rows)) return rc;
+    if (rows == 0 || n_out == 0) return SYN_OK;
+    if (!w || !w_scales) return fail(SYN_E_INVALID, "%s: null weights or scales", W);
+    if (!aligned(w, 16) || w_stride % 16)
+        return fail(SYN_E_INVALID, "%s: the weight rows must be on 16 bytes (stride %llu)", W, (unsigned long long)w_stride);
+    if (w_stride < k_in || w_stride > (1ull << 30))
+        return fail(SYN_E_INVALID, "%s: weight rows of %u bytes %llu apart", W, k_in, (unsigned long long)w_stride);
+    const uint64_t need_w = (w_rows - 1) * w_stride + k_in;
+    if (w_bytes < need_w)
+        return fail(SYN_E_INVALID, "%s: the weight view holds %llu bytes, the matrix %llu", W, (unsigned long long)w_bytes,
+                    (unsigned long long)need_w);
+    if (!aligned(w_scales, 4) || (bias && !aligned(bias, 4)))
+        return fail(SYN_E_INVALID, "%s: scales and bias must be 4-byte aligned", W);
+    if (!quantized)
+        if (int rc = check_values(W, "x", xtype, x, x_stride, rows, k_in)) return rc;
+    if (int rc = check_values(W, "y", ytype, y, y_stride, rows, n_out)) return rc;
+    const syn::I8Act l = syn::i8_act_layout(rows, k_in);
+    if (int rc = check_ws(W, ws, ws_bytes, quantized ? l.partial : i8_ws_bytes(w_rows, k_in, rows, gated))) return rc;
+    uint8_t* base = (uint8_t*)ws;
+    syn::I8Args a{};
+    a.w = w;
+    a.ldw = w_stride;
+    a.ws = w_scales;
+    a.bias = bias;
+    a.n_out = (int)n_out;
+    a.k = (int)k_in;
+    a.xq = (const int8_t*)base;
+    a.xs = (const float*)(base + l.scales);
+    a.T = (int)rows;
+    a.y = y;
+    a.ldy = y_stride;
+    a.ytype = ytype;
+    a.splits = syn::i8_splits((int)w_rows, (int)k_in, (int)rows, gated);
+    if (a.splits > 1) {  // (rows quantized before: as many parts as their workspace has room for)
+        const uint64_t room = (ws_bytes - l.partial) / (4ull * rows * w_rows);
+        if (room < (uint64_t)a.splits) a.splits = room > 1 ? (int)room : 1;
+    }
+    a.partial = a.splits > 1 ? (int*)(base + l.partial) : nullptr;
+    a.gated = gated;
+    if (!quantized) {
+        if (syn::i8_fused((int)w_rows, (int)k_in, (int)rows, gated)) {
+            a.x = x;
+            a.ldx = x_stride;
+            a.xtype = xtype;
+        } else {
+            syn::launch_i8_quantize(xtype, x, x_stride, (int)rows, (int)k_in, (int8_t*)base, syn::i8_padded(k_in),
+                                    (float*)(base + l.scales), (hipStream_t)stream);
+            if (int rc = check_launch(W)) return rc;
+        }
+    }
+    syn::launch_i8_gemv(a, (hipStream_t)stream);
+    return check_launch(W);
+}
+
+}  // namespace
+
+SYN_EXPORT int syn_i8_quantize(int32_t xtype, const void* x, uint64_t x_stride, uint32_t rows, uint32_t k, int8_t* codes,
+                               uint64_t code_stride, float* scales, void* stream) {
+    const char* W = "syn_i8_quantize";
+    if (int rc = check_i8_shape(W, 0, k, rows)) return rc;
+    if (rows == 0) return SYN_OK;
+    if (int rc = check_values(W, "x", xtype, x, x_stride, rows, k)) return rc;
+    if (!codes || !scales || !aligned(codes, 16) || !aligned(scales, 4))
+        return fail(SYN_E_INVALID, "%s: codes must be 16-byte and scales 4-byte aligned", W);
+    if (code_stride % 16 || code_stride < k || code_stride > (1ull << 30))
+        return fail(SYN_E_INVALID, "%s: code rows of %u bytes %llu apart (a multiple of 16)", W, k,
+                    (unsigned long long)code_stride);
+    syn::launch_i8_quantize(xtype, x, x_stride, (int)rows, (int)k, codes, code_stride, scales, (hipStream_t)stream);
+    return check_launch(W);
+}
+
+SYN_EXPORT int syn_i8_gemv_workspace_bytes(uint32_t n_out, uint32_t k_in, uint32_t rows, int32_t gated, uint64_t* bytes) {
+    const char* W = "syn_i8_gemv_workspace_bytes";
+    if (!bytes) return fail(SYN_E_INVALID, "%s: null output", W);
+    const uint64_t w_rows = (uint64_t)n_out * (gated ? 2 : 1);
+    if (int rc = check_i8_shape(W, w_rows, k_in, rows)) return rc;
+    *bytes = i8_ws_bytes(w_rows, k_in, rows, gated ? 1 : 0);
+    return SYN_OK;
+}
+
+SYN_EXPORT int syn_i8_gemv(const int8_t* w, uint64_t w_bytes, uint64_t w_stride, const float* w_scales, const float* bias,
+                           uint32_t n_out, uint32_t k_in, int32_t xtype, const void* x, uint64_t x_stride, uint32_t rows,
+                           int32_t ytype, void* y, uint64_t y_stride, void* ws, uint64_t ws_bytes, void* stream) {
+    return i8_product("syn_i8_gemv", 0, w, w_bytes, w_stride, w_scales, bias, n_out, k_in, xtype, x, x_stride, false, rows,
+                      ytype, y, y_stride, ws, ws_bytes, stream);
+}
+
+SYN_EXPORT int syn_i8_gate_up_act(const int8_t* w, uint64_t w_bytes, uint64_t w_stride, const float* w_scales,
+                                  const float* bias, uint32_t n_out, uint32_t k_in, int32_t xtype, const void* x,
+                                  uint64_t x_stride, uint32_t rows, int32_t ytype, void* y, uint64_t y_stride, void* ws,
+                                  uint64_t ws_bytes, void* stream) {
+    return i8_product("syn_i8_gate_up_act", 1, w, w_bytes, w_stride, w_scales, bias, n_out, k_in, xtype, x, x_stride, false,
+                      rows, ytype, y, y_stride, ws, ws_bytes, stream);
+}
+
+SYN_EXPORT int syn_i8_act_quantize(int32_t xtype, const void* x, uint64_t x_stride, uint32_t rows, uint32_t k_in, void* ws,
+                                   uint64_t ws_bytes, void* stream) {
+    const char* W = "syn_i8_act_quantize";
+    if (int rc = check_i8_shape(W, 0, k_in, rows)) return rc;
+    if (rows == 0) return SYN_OK;
+    if (int rc = check_values(W, "x", xtype, x, x_stride, rows, k_in)) return rc;
+    const syn::I8Act l = syn::i8_act_layout(rows, k_in);
+    if (int rc = check_ws(W, ws, ws_bytes, l.partial)) return rc;
+    syn::launch_i8_quantize(xtype, x, x_stride, (int)rows, (int)k_in, (int8_t*)ws, syn::i8_padded(k_in),
+                            (float*)((uint8_t*)ws + l.scales), (hipStream_t)stream);
+    return check_launch(W);
+}
+
+SYN_EXPORT int syn_i8_gemv_quantized(const int8_t* w, uint64_t w_bytes, uint64_t w_stride, const float* w_scales,
+                                     const float* bias, uint32_t n_out, uint32_t k_in, uint32_t rows, int32_t ytype,
+                                     void* y, uint64_t y_stride, void* ws, uint64_t ws_bytes, void* stream) {
+    return i8_product("syn_i8_gemv_quantized", 0, w, w_bytes, w_stride, w_scales, bias, n_out, k_in, 0, nullptr, 0, true,
+                      rows, ytype, y, y_stride, ws, ws_bytes, stream);
+}
+
+SYN_EXPORT int syn_i8_logits_workspace_bytes(uint32_t vocab, uint32_t hidden, uint32_t rows, uint64_t* bytes) {
+    if (int rc = syn_i8_gemv_workspace_bytes(vocab, hidden, rows, 0, bytes)) return rc;
+    *bytes += syn::align_up(4ull * rows * hidden, 256);
+    return SYN_OK;
+}
+
+SYN_EXPORT int syn_i8_logits(const int8_t* head, uint64_t head_bytes, uint64_t head_stride, const float* head_scales,
+                             uint32_t vocab, uint32_t hidden, const float* g, float eps, const float* x, uint32_t rows,
+                             float* y, void* ws, uint64_t ws_bytes, void* stream) {
+    const char* W = "syn_i8_logits";
+    uint64_t need = 0;
+    if (int rc = syn_i8_logits_workspace_bytes(vocab, hidden, rows, &need)) return rc;
+    if (hidden > (uint32_t)syn::NORM_MAX_COLS)
+        return fail(SYN_E_UNSUPPORTED, "%s: hidden %u (at most %d)", W, hidden, syn::NORM_MAX_COLS);
+    if (rows == 0 || vocab == 0) return SYN_OK;
+    if (!x || !g || !aligned(x, 4) || !aligned(g, 4)) return fail(SYN_E_INVALID, "%s: x and g must be 4-byte aligned", W);
+    if (int rc = check_ws(W, ws, ws_bytes, need)) return rc;
+    const uint64_t hb = syn::align_up(4ull * rows * hidden, 256);
+    // the head's own checks before the norm is enqueued: a refused call enqueues nothing
+    if (!head || !head_scales || !y || !aligned(head, 16) || head_stride % 16 || head_stride < hidden ||
+        head_stride > (1ull << 30) || head_bytes < (uint64_t)(vocab - 1) * head_stride + hidden || !aligned(y, 4) ||
+        !aligned(head_scales, 4))
+        return fail(SYN_E_INVALID, "%s: the head's view, stride, scales or y", W);
+    syn::launch_rms_norm(x, g, (int)rows, (int)hidden, eps, (float*)ws, (hipStream_t)stream);
+    if (int rc = check_launch(W)) return rc;
+    return i8_product(W, 0, head, head_bytes, head_stride, head_scales, nullptr, vocab, hidden, SYN_F32, ws, hidden, false,
+                      rows, SYN_F32, y, vocab, (uint8_t*)ws + hb, ws_bytes - hb, stream);
+}
+
+namespace {
+int check_logprobs(const char* W, int32_t xtype, uint32_t rows, uint32_t vocab, uint32_t top) {
+    if (xtype != SYN_F32 && !float_type(xtype)) return fail(SYN_E_UNSUPPORTED, "%s: logits of type %d are not F32, F16 or BF16", W, xtype);
+    if (vocab == 0 || vocab > 0x7FFFFF00u || rows > 0x7FFFFF00u) return fail(SYN_E_INVALID, "%s: %u rows of %u logits", W, rows, vocab);
+    if (top > SYN_LOGPROBS_MAX_TOP || top > vocab)
+        return fail(SYN_E_UNSUPPORTED, "%s: the %u greatest of %u logits (at most %d)", W, top, vocab, SYN_LOGPROBS_MAX_TOP);
+    return SYN_OK;
+}
+static_assert(SYN_LOGPROBS_MAX_TOP == syn::LOGPROB_MAX_TOP, "the header's limit");
+static_assert(SYN_I8_MAX_K == syn::I8_MAX_K, "the header's limit");
+}  // namespace
+
+SYN_EXPORT int syn_token_logprobs_workspace_bytes(int32_t xtype, uint32_t rows, uint32_t vocab, uint32_t top,
+                                                  uint64_t* bytes) {
+    const char* W = "syn_token_logprobs_workspace_bytes";
+    if (!bytes) return fail(SYN_E_INVALID, "%s: null output", W);
+    if (int rc = check_logprobs(W, xtype, rows, vocab, top)) return rc;
+    *bytes = syn::logprob_ws_bytes((int)rows, (int)vocab, (int)top);
+    return SYN_OK;
+}
+
+SYN_EXPORT int syn_token_logprobs(int32_t xtype, const void* x, uint64_t x_stride, uint32_t rows, uint32_t vocab,
+                                  const void* tokens, uint32_t token_bytes, float scale, uint32_t top, float* logprob,
+                                  int32_t* rank, float* entropy, int32_t* top_ids, float* top_logprobs, void* ws,
+                                  uint64_t ws_bytes, void* stream) {
+    const char* W = "syn_token_logprobs";
+    if (int rc = check_logprobs(W, xtype, rows, vocab, top)) return rc;
+    if (token_bytes != 4 && token_bytes != 8) return fail(SYN_E_UNSUPPORTED, "%s: tokens of %u bytes (4 or 8)", W, token_bytes);
+    if (!(scale > 0.0f && scale < __builtin_inff())) return fail(SYN_E_INVALID, "%s: the scale %g is not finite and above 0", W, scale);
+    if (rows == 0) return SYN_OK;
+    if (int rc = check_values(W, "x", xtype, x, x_stride, rows, vocab)) return rc;
+    if (!tokens || !logprob || !rank || !entropy || (top && (!top_ids || !top_logprobs)))
+        return fail(SYN_E_INVALID, "%s: null operand", W);
+    if (!aligned(tokens, token_bytes) || !aligned(logprob, 4) || !aligned(rank, 4) || !aligned(entropy, 4) ||
+        !aligned(top_ids, 4) || !aligned(top_logprobs, 4))
+        return fail(SYN_E_INVALID, "%s: operands must be aligned to their values", W);
+    const uint64_t need = syn::logprob_ws_bytes((int)rows, (int)vocab, (int)top);
+    if (need)
+        if (int rc = check_ws(W, ws, ws_bytes, need)) return rc;
+    const syn::LogprobArgs a{x, x_stride, xtype, (int)rows, (int)vocab, tokens, token_bytes == 8, scale, (int)top,
+                             logprob, rank, entropy, top_ids, top_logprobs, (uint8_t*)ws};
+    syn::launch_logprobs(a, (hipStream_t)stream);
     return check_launch(W);
 }
 

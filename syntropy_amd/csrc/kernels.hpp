@@ -193,4 +193,24 @@ void launch_tile64_repack(const uint8_t* src, uint8_t* dst, uint64_t bytes, int 
 void launch_quantize(int ty, const float* x, uint64_t n, uint8_t* out, hipStream_t stream);
 void launch_dequantize(int ty, const uint8_t* src, uint64_t n, float* out, hipStream_t stream);
 
+// logprobs.hip: log probabilities of given tokens, entropy and the most probable tokens of rows of logits
+constexpr int LOGPROB_MAX_TOP = 64;
+struct LogprobArgs {
+    const void* x;  // [rows][vocab] of xtype, rows ldx values apart
+    uint64_t ldx;
+    int xtype, rows, vocab;
+    const void* tokens;  // [rows] I32, or I64 where wide
+    int wide;
+    float scale;
+    int top;
+    float* logprob;
+    int32_t* rank;
+    float* entropy;
+    int32_t* top_ids;     // [rows][top]
+    float* top_logprobs;  // [rows][top]
+    uint8_t* ws;
+};
+uint64_t logprob_ws_bytes(int rows, int vocab, int top);
+void launch_logprobs(const LogprobArgs& a, hipStream_t stream);
+
 }  // namespace syn

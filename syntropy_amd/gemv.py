@@ -9,6 +9,7 @@ import ctypes as C
 import functools
 from dataclasses import dataclass
 from enum import IntEnum
+from typing import NamedTuple
 
 import torch
 
@@ -236,6 +237,104 @@ def logits(head: Weights, g: torch.Tensor, eps: float, x: torch.Tensor, rows: in
     return y
 
 
+_VALUE_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
+
+
+def _value_type(t: torch.Tensor, what: str) -> int:
+    ty = _VALUE_TYPES.get(t.dtype)
+    if ty is None:
+        raise GemvError("Activations", f"`{what}` is of {t.dtype}, not float32, float16 or bfloat16")
+    return ty
+
+
+def _ptr_rows(t: torch.Tensor, rows: int, n: int, what: str, device=None) -> int:
+    """The row stride, in values, of a device tensor of at least `rows` rows of n values side by side: one
+    of two dimensions with any row stride, or a contiguous one of enough values."""
+    if not t.is_cuda or (device is not None and t.device != device):
+        raise GemvError("Len", f"`{what}` must be on the operands' device")
+    if rows < 0:
+        raise GemvError("Len", f"{rows} rows")
+    if t.dim() == 2 and t.shape[1] == n and t.shape[0] >= rows and (t.stride(1) == 1 or n == 1):
+        if rows <= 1 or t.stride(0) >= n:
+            return max(t.stride(0), n)
+    if not t.is_contiguous() or t.numel() < rows * n:
+        raise GemvError("Len", f"`{what}` holds {t.numel()} values, the op needs {rows} rows of {n} side by side")
+    return n
+
+
+class _on:
+    """The stream a call runs on: `stream` (a torch stream or a handle), or the current one of t's device,
+    with that device current, and what torch allocates meanwhile belonging to that stream."""
+
+    __slots__ = ("device", "stream", "held")
+
+    def __init__(self, t: torch.Tensor, stream):
+        self.device, self.stream, self.held = t.device.index, stream, None
+
+    def __enter__(self) -> int:
+        if self.stream is None and self.device == torch.cuda.current_device():
+            return torch._C._cuda_getCurrentRawStream(self.device)
+        if self.stream is None:
+            self.held = torch.cuda.device(self.device)
+            self.held.__enter__()
+            return torch._C._cuda_getCurrentRawStream(self.device)
+        s = self.stream
+        if not hasattr(s, "cuda_stream"):
+            s = torch.cuda.ExternalStream(int(s), device=self.device)
+        if s.device.index != self.device:
+            raise GemvError("Len", f"the stream is of {s.device}, the operands of cuda:{self.device}")
+        self.held = torch.cuda.stream(s)
+        self.held.__enter__()
+        return s.cuda_stream
+
+    def __exit__(self, *e):
+        if self.held is not None:
+            self.held.__exit__(*e)
+
+
+class TokenLogprobs(NamedTuple):
+    """What token_logprobs gives, a row each: the token's log probability F32 and rank I32, the entropy F32,
+    the greatest logits' indices I32 [rows, top] and their log probabilities F32 [rows, top]."""
+
+    logprob: torch.Tensor
+    rank: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, scale: float = 1.0,
+                   stream=None) -> TokenLogprobs:
+    """Of each row of logits [rows, vocab] (F32, F16 or BF16; strided rows; -infinity hides a token), with z =
+    logits * scale (the inverse of a sampling temperature): log softmax(z) at tokens[row] (int32 or int64), the
+    number of logits greater than that token's, the entropy of softmax(z) in nats, and the `top` (0 to 64)
+    greatest logits' indices, the lower one first among equals, with their log probabilities.
+
+    A negative token asks for none (logprob 0, rank -1); one of vocab or more gives NaN and -1.  A row whose
+    every logit is -infinity has log probabilities of -infinity and the entropy 0; one with a NaN or +infinity
+    has NaN for both."""
+    if logits.dim() != 2 or tokens.dim() != 1 or tokens.shape[0] != logits.shape[0]:
+        raise GemvError("Len", "logits must be rows of values, with a token each")
+    rows, vocab = logits.shape
+    if not 0 <= top <= min(vocab, 64):
+        raise GemvError("Len", f"the {top} greatest of {vocab} logits (0 to 64)")
+    if tokens.dtype not in (torch.int32, torch.int64) or not tokens.is_contiguous() or tokens.device != logits.device:
+        raise GemvError("Len", "tokens must be contiguous int32 or int64 values beside the logits")
+    ty, stride = _value_type(logits, "logits"), _ptr_rows(logits, rows, vocab, "logits")
+    with _on(logits, stream) as s:
+        dev = logits.device
+        values = torch.empty(2, rows, dtype=torch.float32, device=dev)
+        ranks = torch.empty(rows, dtype=torch.int32, device=dev)
+        ids = torch.empty(rows, top, dtype=torch.int32, device=dev)
+        lps = torch.empty(rows, top, dtype=torch.float32, device=dev)
+        need = _need("syn_token_logprobs_workspace_bytes", ty, rows, vocab, top)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        call("syn_token_logprobs", ty, logits.data_ptr(), stride, rows, vocab, tokens.data_ptr(), tokens.element_size(),
+             scale, top, values.data_ptr(), ranks.data_ptr(), values.data_ptr() + 4 * rows, ids.data_ptr(), lps.data_ptr(),
+             ws.data_ptr() if need else None, need, s)
+    return TokenLogprobs(values[0], ranks, values[1], ids, lps)
+
+
 class GemvBatch:
     """Up to 8 independent single-row Q4_K Gemv ops launched together (one batched Q8_K
     quantization, one grouped GEMV): each y[i] equals gemv(ws[i], x[i], 1) bit for bit.  The
@@ -337,4 +436,4 @@ def dequantize(ty: WeightType, src: torch.Tensor, stream=None) -> torch.Tensor:
 __all__ = ["WeightType", "Weights", "GemvError", "SynError", "GemvBatch", "workspace_bytes", "quantize_into",
            "repack", "LAYOUT_SOURCE", "LAYOUT_X8", "LAYOUT_SPLIT",
            "gemv_quantized", "gemv", "quantize", "dequantize", "new_workspace", "gemm_workspace",
-           "gemm_quantize_into", "gemm_quantized", "gate_up_act", "lib"]
+           "gemm_quantize_into", "gemm_quantized", "gate_up_act", "token_logprobs", "TokenLogprobs", "lib"]

@@ -1,0 +1,173 @@
+"""Products over int8 weights with a scale a channel (output row) on the MI355X: activations of F32, F16 or
+BF16 are quantized inside the call to int8 with a scale a token, the sums are exact in I32.  Beside
+`gemv` (scales a block of 32 or 256 weights, bit-identical to the reference's provider) these take one
+scale a row, which leaves the matrix cores nothing but integers; the reference has no such type.
+
+    w = int8.quantize_weights(matrix)            # or int8.Weights(codes, scales) of a checkpoint
+    y = int8.gemv(w, x, rows)                    # x [rows, k_in] -> [rows, n_out] of x's type
+    h = int8.gate_up_act(gate_up, x, rows)       # silu(gate x) * (up x) of a stacked matrix
+
+Every call runs the HIP kernels through the C ABI; there is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass
+
+import torch
+
+from ._lib import SynError, call
+from .gemv import GemvError, _need, _on, _ptr_rows, _value_type
+
+MAX_K = 131072
+
+
+@dataclass
+class Weights:
+    """`codes` int8 [n_out, k_in] with F32 `scales` [n_out] and an optional F32 `bias` [n_out], device
+    tensors: the row o stands for codes[o] * scales[o].  Rows lie side by side and start on 16 bytes: a
+    codes tensor whose rows do not (k_in no multiple of 16, say) is copied once, here, into rows of whole
+    128-byte lines; any other is kept as it is."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    bias: torch.Tensor | None = None
+
+    def __post_init__(self):
+        c, s, b = self.codes, self.scales, self.bias
+        if not (c.is_cuda and c.dtype == torch.int8 and c.dim() == 2):
+            raise GemvError("Len", "codes must be an int8 device tensor of rows")
+        self.n_out, self.k_in = c.shape
+        if not 1 <= self.k_in <= MAX_K:
+            raise GemvError("RowLength", f"rows of {self.k_in} codes (1 to {MAX_K})")
+        for what, t in (("scales", s), ("bias", b)):
+            if t is None and what == "bias":
+                continue
+            if not (t.device == c.device and t.dtype == torch.float32 and t.is_contiguous()) or t.shape != (self.n_out,):
+                raise GemvError("Len", f"{what} must be a contiguous F32 tensor of {self.n_out} values beside the codes")
+        if c.stride(1) != 1 or c.stride(0) < self.k_in or c.stride(0) % 16 or c.data_ptr() % 16:
+            rows = torch.zeros(self.n_out, -(-self.k_in // 128) * 128, dtype=torch.int8, device=c.device)[:, :self.k_in]
+            self.codes = c = rows.copy_(c)
+        self.stride = c.stride(0)
+        self.view_bytes = max(0, (self.n_out - 1) * self.stride + self.k_in)
+        self.bias_ptr = 0 if b is None else b.data_ptr()
+
+
+def quantize_rows(x: torch.Tensor, stream=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Each row of x [rows, k] (F32, F16 or BF16): int8 codes [rows, k] (in rows of whole 128-byte lines)
+    and F32 scales [rows], code = rint(x / scale) with scale = max |x| / 127.  A row with a NaN or an
+    infinity has the scale NaN and codes 0."""
+    if x.dim() != 2:
+        raise GemvError("Len", "x must be rows of values")
+    rows, k = x.shape
+    ty, stride = _value_type(x, "x"), _ptr_rows(x, rows, k, "x")
+    with _on(x, stream) as s:
+        codes = torch.empty(rows, -(-k // 128) * 128, dtype=torch.int8, device=x.device)
+        scales = torch.empty(rows, dtype=torch.float32, device=x.device)
+        call("syn_i8_quantize", ty, x.data_ptr(), stride, rows, k, codes.data_ptr(), codes.shape[1], scales.data_ptr(), s)
+    return codes[:, :k], scales
+
+
+def quantize_weights(w: torch.Tensor, bias: torch.Tensor | None = None, stream=None) -> Weights:
+    """A matrix [n_out, k_in] of F32, F16 or BF16 with a scale a channel (quantize_rows of its rows)."""
+    codes, scales = quantize_rows(w, stream)
+    return Weights(codes, scales, bias)
+
+
+def workspace_bytes(n_out: int, k_in: int, rows: int, gated: bool = False) -> int:
+    """Scratch bytes of a call: the quantized rows, and partial sums where K is split."""
+    return _need("syn_i8_gemv_workspace_bytes", n_out, k_in, rows, 1 if gated else 0)
+
+
+def _out(y, x, rows, n, dtype):
+    if y is None:
+        return torch.empty(rows, n, dtype=dtype or x.dtype, device=x.device)
+    if dtype is not None and dtype != y.dtype:
+        raise GemvError("Len", f"`y` is of {y.dtype}, not {dtype}")
+    return y
+
+
+def _product(name, gated, w, n, x, rows, y, ws, dtype, stream):
+    if x.device != w.codes.device:
+        raise GemvError("Len", f"x is on {x.device}, the weights on {w.codes.device}")
+    ty, xs = _value_type(x, "x"), _ptr_rows(x, rows, w.k_in, "x")
+    with _on(x, stream) as s:
+        y = _out(y, x, rows, n, dtype)
+        yty, ys = _value_type(y, "y"), _ptr_rows(y, rows, n, "y", x.device)
+        if ws is None:
+            ws = torch.empty(max(workspace_bytes(n, w.k_in, rows, gated), 256), dtype=torch.uint8, device=x.device)
+        call(name, w.codes.data_ptr(), w.view_bytes, w.stride, w.scales.data_ptr(), w.bias_ptr, n, w.k_in, ty, x.data_ptr(),
+             xs, rows, yty, y.data_ptr(), ys, ws.data_ptr(), ws.numel(), s)
+    return y
+
+
+def gemv(w: Weights, x: torch.Tensor, rows: int, y: torch.Tensor | None = None, ws: torch.Tensor | None = None,
+         dtype: torch.dtype | None = None, stream=None) -> torch.Tensor:
+    """y [rows, n_out] = x W^T (+ bias) for the first `rows` rows of x [., k_in], of x's type, y's or
+    `dtype` (F32, F16, BF16).  x and y may have strided rows."""
+    return _product("syn_i8_gemv", False, w, w.n_out, x, rows, y, ws, dtype, stream)
+
+
+def gate_up_act(w: Weights, x: torch.Tensor, rows: int, y: torch.Tensor | None = None, ws: torch.Tensor | None = None,
+                dtype: torch.dtype | None = None, stream=None) -> torch.Tensor:
+    """GateUpAct{Silu} over a stacked matrix (gate rows, then up rows: w.n_out = 2 n): y [rows, n] =
+    silu(gate x) * (up x), both products the F32 values of gemv."""
+    if w.n_out % 2:
+        raise GemvError("Len", f"a stacked gate/up matrix has an even row count, not {w.n_out}")
+    return _product("syn_i8_gate_up_act", True, w, w.n_out // 2, x, rows, y, ws, dtype, stream)
+
+
+class Rows:
+    """Rows of x quantized once (quantize_into) for several matrices of the same k_in (gemv_quantized): a
+    workspace for their codes and for the products of `n_outs` outputs each."""
+
+    def __init__(self, rows: int, k_in: int, *n_outs: int, device="cuda"):
+        self.rows, self.k_in = rows, k_in
+        need = max(workspace_bytes(n, k_in, rows) for n in n_outs or (1,))
+        self.ws = torch.empty(max(need, 256), dtype=torch.uint8, device=device)
+
+
+def quantize_into(x: torch.Tensor, r: Rows, stream=None) -> None:
+    """The first r.rows rows of x into r."""
+    ty, xs = _value_type(x, "x"), _ptr_rows(x, r.rows, r.k_in, "x", r.ws.device)
+    with _on(x, stream) as s:
+        call("syn_i8_act_quantize", ty, x.data_ptr(), xs, r.rows, r.k_in, r.ws.data_ptr(), r.ws.numel(), s)
+
+
+def gemv_quantized(w: Weights, r: Rows, y: torch.Tensor, stream=None) -> torch.Tensor:
+    """gemv over rows quantized before: the same values."""
+    if w.k_in != r.k_in:
+        raise GemvError("Len", f"the rows hold {r.k_in} codes, the weights {w.k_in}")
+    if w.codes.device != r.ws.device:
+        raise GemvError("Len", f"the rows are on {r.ws.device}, the weights on {w.codes.device}")
+    yty, ys = _value_type(y, "y"), _ptr_rows(y, r.rows, w.n_out, "y", r.ws.device)
+    with _on(y, stream) as s:
+        call("syn_i8_gemv_quantized", w.codes.data_ptr(), w.view_bytes, w.stride, w.scales.data_ptr(), w.bias_ptr, w.n_out,
+             w.k_in, r.rows, yty, y.data_ptr(), ys, r.ws.data_ptr(), r.ws.numel(), s)
+    return y
+
+
+def logits(head: Weights, g: torch.Tensor, eps: float, x: torch.Tensor, rows: int, y: torch.Tensor | None = None,
+           stream=None) -> torch.Tensor:
+    """Logits over an int8 head: each F32 row of x [., hidden] normalised by (g, eps) as gemv.rms_norm, then
+    y F32 [rows, vocab] = head x as gemv."""
+    if not (x.is_cuda and x.dtype == torch.float32 and x.is_contiguous() and x.numel() >= rows * head.k_in):
+        raise GemvError("Len", f"x must be a contiguous F32 device tensor of {rows * head.k_in} values")
+    if head.codes.device != x.device or g.device != x.device or g.dtype != torch.float32 or g.numel() != head.k_in:
+        raise GemvError("Len", f"g must hold {head.k_in} F32 values beside x and the head")
+    if head.bias is not None:
+        raise GemvError("Activations", "a head has no bias")
+    with _on(x, stream) as s:
+        if y is None:
+            y = torch.empty(rows, head.n_out, dtype=torch.float32, device=x.device)
+        elif not (y.device == x.device and y.dtype == torch.float32 and y.is_contiguous() and y.numel() >= rows * head.n_out):
+            raise GemvError("Len", f"y must be a contiguous F32 device tensor of {rows * head.n_out} values")
+        need = _need("syn_i8_logits_workspace_bytes", head.n_out, head.k_in, rows)
+        ws = torch.empty(max(need, 256), dtype=torch.uint8, device=x.device)
+        call("syn_i8_logits", head.codes.data_ptr(), head.view_bytes, head.stride, head.scales.data_ptr(), head.n_out,
+             head.k_in, g.data_ptr(), C.c_float(eps), x.data_ptr(), rows, y.data_ptr(), ws.data_ptr(), ws.numel(), s)
+    return y
+
+
+__all__ = ["Weights", "Rows", "SynError", "GemvError", "quantize_rows", "quantize_weights", "workspace_bytes", "gemv",
+           "gate_up_act", "quantize_into", "gemv_quantized", "logits"]
