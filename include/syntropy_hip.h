@@ -213,8 +213,9 @@ int syn_logits(uint32_t layout, int32_t wtype, const void* head, uint64_t head_b
  *   after another; of the largest workspace of them, else K may be split less, to the same values).
  * syn_i8_logits: RmsNorm of F32 rows as syn_rms_norm (k_in <= 16384), then the head as syn_i8_gemv; the
  *   workspace holds the normalised rows first.
- * Workspaces are 256-byte aligned; gated is 1 for syn_i8_gate_up_act, else 0. */
+ * At most SYN_I8_MAX_ROWS activation rows and 2^24 - 1 weight rows.  Workspaces are 256-byte aligned; gated is 1 for syn_i8_gate_up_act, else 0. */
 #define SYN_I8_MAX_K 131072
+#define SYN_I8_MAX_ROWS 2097120
 int syn_i8_quantize(int32_t xtype, const void* x, uint64_t x_stride, uint32_t rows, uint32_t k, int8_t* codes,
                     uint64_t code_stride, float* scales, void* stream);
 int syn_i8_gemv_workspace_bytes(uint32_t n_out, uint32_t k_in, uint32_t rows, int32_t gated, uint64_t* bytes);

@@ -1039,7 +1039,10 @@ int check_values(const char* W, const char* what, int32_t ty, const void* p, uin
 
 int check_i8_shape(const char* W, uint64_t w_rows, uint32_t k, uint32_t rows) {
     if (k == 0 || k > SYN_I8_MAX_K) return fail(SYN_E_UNSUPPORTED, "%s: rows of %u values (1 to %d)", W, k, SYN_I8_MAX_K);
-    if (w_rows > 0x7FFFFF00ull || rows > 0x7FFFFF00u) return fail(SYN_E_INVALID, "%s: too many rows", W);
+    // what a launch's grid holds
+    if (w_rows >= 1ull << 24 || rows > SYN_I8_MAX_ROWS)
+        return fail(SYN_E_UNSUPPORTED, "%s: %llu weight rows (below 2^24), %u rows (at most %d)", W, (unsigned long long)w_rows,
+                    rows, SYN_I8_MAX_ROWS);
     return SYN_OK;
 }
 
@@ -1124,7 +1127,7 @@ int i8_product(const char* W, int gated, const int8_t* w, uint64_t w_bytes, uint
 SYN_EXPORT int syn_i8_quantize(int32_t xtype, const void* x, uint64_t x_stride, uint32_t rows, uint32_t k, int8_t* codes,
                                uint64_t code_stride, float* scales, void* stream) {
     const char* W = "syn_i8_quantize";
-    if (int rc = check_i8_shape(W, 0, k, rows)) return rc;
+    if (int rc = check_i8_shape(W, rows, k, 0)) return rc;
     if (rows == 0) return SYN_OK;
     if (int rc = check_values(W, "x", xtype, x, x_stride, rows, k)) return rc;
     if (!codes || !scales || !aligned(codes, 16) || !aligned(scales, 4))

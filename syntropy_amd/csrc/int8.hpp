@@ -2,6 +2,8 @@
 // a scale a token: shared geometry and device helpers.
 #pragma once
 
+#include <type_traits>
+
 #include "common.hpp"
 
 namespace syn {
@@ -23,7 +25,7 @@ struct I8Act {
 SYN_HD inline I8Act i8_act_layout(uint64_t rows, uint64_t k) {
     I8Act a;
     a.scales = align_up(rows * i8_padded(k), 256);
-    a.partial = align_up(a.scales + 4 * rows, 256);
+    a.partial = a.scales + 4 * align_up(rows, 256);  // (a tile reads the scales of its last rows' places too)
     return a;
 }
 
@@ -47,10 +49,33 @@ struct I8Args {
     int gated;             // w is [gate; up]: y = silu(gate) * up
 };
 
-SYN_DEV float i8_load(const void* x, int ty, uint64_t i) {
-    if (ty == T_F32) return ((const float*)x)[i];
-    const uint32_t h = ((const uint16_t*)x)[i];
-    return ty == T_F16 ? f16_to_f32(h) : u2f(h << 16);
+// Eight values from i on of a row of k (zeros past its end), at any alignment.
+template <int TY>
+SYN_DEV void i8_load8(const uint8_t* xr, int i, int k, float (&v)[8]) {
+    if (i + 8 <= k) {
+        if constexpr (TY == T_F32) {
+            __builtin_memcpy(v, xr + 4 * (int64_t)i, 32);
+        } else {
+            uint32_t h[4];
+            __builtin_memcpy(h, xr + 2 * (int64_t)i, 16);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t b = h[j / 2] >> (16 * (j & 1)) & 0xFFFFu;
+                v[j] = TY == T_F16 ? f16_to_f32(b) : u2f(b << 16);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j] = 0.0f;
+            if (i + j < k) {
+                if constexpr (TY == T_F32)
+                    v[j] = ((const float*)xr)[i + j];
+                else
+                    v[j] = TY == T_F16 ? f16_to_f32(((const uint16_t*)xr)[i + j]) : u2f((uint32_t)((const uint16_t*)xr)[i + j] << 16);
+            }
+        }
+    }
 }
 // BF16 by round to nearest even, a NaN kept one.
 SYN_DEV uint32_t bf16_bits(float v) {
@@ -78,10 +103,21 @@ SYN_DEV I8Scale i8_scale(uint32_t amax_bits) {
     const float inv = s != 0.0f ? recip_rn(s) : 0.0f;
     return {s, finite_f(inv) ? inv : 0.0f};
 }
-// (a row with a NaN or an infinity: v inv may be a NaN, whose conversion is 0; an infinity's is not, so
-// the factor's sign says nothing and the code is zeroed by the caller through `inv` = 0)
-SYN_DEV int i8_code(float v, float inv) {
-    return inv == 0.0f ? 0 : (int)__builtin_rintf(v * inv);
+// The largest magnitude's bits of eight values and m.
+SYN_DEV uint32_t i8_max8(const float (&v)[8], uint32_t m) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t b = f2u(v[j]) & 0x7FFFFFFFu;
+        m = m > b ? m : b;
+    }
+    return m;
+}
+// Their codes.  (Where inv is 0 the codes are 0, whatever the value: an infinity times 0 is a NaN.)
+SYN_DEV uint2 i8_codes8(const float (&v)[8], float inv) {
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j / 4] |= ((uint32_t)(int)__builtin_rintf(v[j] * inv) & 0xFFu) << (8 * (j & 3));
+    return inv == 0.0f ? uint2{0, 0} : uint2{w[0], w[1]};
 }
 
 // An output from its exact sum: RN(RN(RN(S) sx) sw), the bias added.  |S| may pass 2^24, so the first
@@ -90,8 +126,20 @@ SYN_DEV float i8_value(int sum, float sx, float sw) { return ((float)sum * sx) *
 
 void launch_i8_quantize(int xtype, const void* x, uint64_t ldx, int rows, int k, int8_t* codes, uint64_t ldc,
                         float* scales, hipStream_t stream);
+// int8_few.hip: up to 32 tokens, weights straight to registers
+bool i8_few_fits(int T);
+bool i8_few_fused(int rows_w, int k, int T, int gated);  // the kernel quantizes the rows itself
+void launch_i8_few(const I8Args& a, hipStream_t stream);
+// int8_gemm.hip: tiles through LDS, K in one part or several
+struct I8Pick {
+    int tile, splits;
+};
+I8Pick i8_gemm_pick(int rows_w, int k, int T, int gated);
+bool i8_gemm_reaches(int tile, const I8Args& a);
+void launch_i8_gemm(int tile, const I8Args& a, hipStream_t stream);
+// int8.hip
 int i8_splits(int rows_w, int k, int T, int gated);
-void launch_i8_gemv(const I8Args& a, hipStream_t stream);
 bool i8_fused(int rows_w, int k, int T, int gated);
+void launch_i8_gemv(const I8Args& a, hipStream_t stream);
 
 }  // namespace syn

@@ -38,7 +38,7 @@ BAD = [
     (dict(ytype=12), UNSUPPORTED), (dict(x=0), INVALID), (dict(x=A + 2), INVALID), (dict(x=A + 1, xtype=F16), INVALID),
     (dict(xs=255), INVALID), (dict(xs=1 << 41), INVALID), (dict(y=0), INVALID), (dict(y=A + 1, ytype=BF16), INVALID),
     (dict(ys=7), INVALID), (dict(ws=0), INVALID), (dict(ws=A + 128), INVALID), (dict(ws_bytes=100), WORKSPACE),
-    (dict(rows=0x80000000), INVALID), (dict(n=0x7FFFFFFF), INVALID),
+    (dict(rows=2097121), UNSUPPORTED), (dict(n=1 << 24), UNSUPPORTED),
 ]
 
 
@@ -66,7 +66,7 @@ def test_workspace_queries():
     assert rc("syn_i8_gemv_workspace_bytes", 4096, 2011, 5, 0, C.byref(out)) == 0 and out.value >= 5 * 2048 + 20
     assert rc("syn_i8_gemv_workspace_bytes", 4096, 0, 5, 0, C.byref(out)) == UNSUPPORTED
     assert rc("syn_i8_gemv_workspace_bytes", 4096, 2011, 5, 0, None) == INVALID
-    assert rc("syn_i8_gemv_workspace_bytes", 0x60000000, 64, 5, 1, C.byref(out)) == INVALID
+    assert rc("syn_i8_gemv_workspace_bytes", 1 << 23, 64, 5, 1, C.byref(out)) == UNSUPPORTED
     assert rc("syn_token_logprobs_workspace_bytes", F32, 4, 50, 65, C.byref(out)) == UNSUPPORTED
     assert rc("syn_token_logprobs_workspace_bytes", F32, 4, 0, 0, C.byref(out)) == INVALID
     assert rc("syn_token_logprobs_workspace_bytes", 2, 4, 50, 0, C.byref(out)) == UNSUPPORTED
