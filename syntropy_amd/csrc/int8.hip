@@ -100,7 +100,7 @@ __global__ __launch_bounds__(256) void k_i8_fold(I8Args g) {
     if (g.gated) {
         float u = i8_value(s1, sx, g.ws[g.n_out + n]);
         if (g.bias) u = u + g.bias[g.n_out + n];
-        v = ref_silu(v) * u;
+        v = i8_silu(v) * u;
     }
     i8_store(g.y, g.ytype, (uint64_t)t * g.ldy + n, v);
 }

@@ -82,6 +82,13 @@ SYN_DEV uint32_t bf16_bits(float v) {
     const uint32_t u = f2u(v);
     return v != v ? 0x7FC0u : (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
 }
+template <int TY>
+SYN_DEV uint32_t i8_half2(float a, float b) {
+    if constexpr (TY == T_F16)
+        return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16;
+    else
+        return bf16_bits(a) | bf16_bits(b) << 16;
+}
 SYN_DEV void i8_store(void* y, int ty, uint64_t i, float v) {
     if (ty == T_F32)
         ((float*)y)[i] = v;
@@ -123,6 +130,30 @@ SYN_DEV uint2 i8_codes8(const float (&v)[8], float inv) {
 // An output from its exact sum: RN(RN(RN(S) sx) sw), the bias added.  |S| may pass 2^24, so the first
 // rounding is the conversion's.
 SYN_DEV float i8_value(int sum, float sx, float sw) { return ((float)sum * sx) * sw; }
+
+// silu(g) = g / (1 + exp(-g)): the exponential as 2^t of the rounded product t = -g log2(e) and a factor for
+// what the rounding left, within a step; the reciprocal within a step.  Below -88, where the exponential
+// nears F32's end, the quotient is 0 (for a value below 2^-120); an infinite or NaN g is met in the product.
+SYN_DEV float i8_silu(float g) {
+    const float gc = __builtin_amdgcn_fmed3f(g, -88.0f, 100.0f);
+    const float t = gc * -1.44269504088896340736f;
+    const float r = __builtin_fmaf(gc, -1.44269504088896340736f, -t);
+    const float e0 = __builtin_amdgcn_exp2f(t);
+    const float e = __builtin_fmaf(e0, r * 0.69314718055994530942f, e0);
+    return g * __builtin_amdgcn_rcpf(g < -88.0f ? __builtin_inff() : 1.0f + e);
+}
+
+// Workgroups go to the 8 XCDs in turn.  Each XCD takes a run of neighbouring tiles, token tiles first within
+// groups of 8, so that what runs on it at once shares its weight rows and tokens in its L2.
+SYN_DEV void i8_tile_of(int id, int tiles_w, int tiles_t, int& tw, int& tt) {
+    const int total = tiles_w * tiles_t, each = total / 8, rest = total % 8, x = id & 7;
+    int l = x * each + (x < rest ? x : rest) + id / 8;
+    const int group = 8 * tiles_w, gi = l / group, t8 = gi * 8;
+    const int in = tiles_t - t8 < 8 ? tiles_t - t8 : 8;
+    l -= gi * group;
+    tt = t8 + l % in;
+    tw = l / in;
+}
 
 void launch_i8_quantize(int xtype, const void* x, uint64_t ldx, int rows, int k, int8_t* codes, uint64_t ldc,
                         float* scales, hipStream_t stream);

@@ -158,7 +158,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_few(I8Args g) {
         if constexpr (GATED) {
             float u = i8_value(sum[1][e], sx, g.ws[g.n_out + n]);
             if (g.bias) u = u + g.bias[g.n_out + n];
-            v = ref_silu(v) * u;
+            v = i8_silu(v) * u;
         }
         i8_store(g.y, g.ytype, (uint64_t)(t0 + t) * g.ldy + n, v);
     }
