@@ -203,21 +203,25 @@ int syn_logits(uint32_t layout, int32_t wtype, const void* head, uint64_t head_b
  * syn_i8_quantize: rows of x to codes (rows code_stride bytes apart, a multiple of 16, at least k; zeros
  *   behind a row's last code up to a multiple of 128 or the stride, whichever is less) and scales [rows]:
  *   a token's rows, or a weight matrix's, whose rows are its channels.
+ * syn_i8_gemv_workspace_bytes: the workspace of the two calls below; 0 (ws may be NULL) where the product's
+ *   kernel quantizes the rows itself.  gated is 1 for syn_i8_gate_up_act, else 0.
  * syn_i8_gemv: the product, W [n_out, k_in] to y [rows, n_out] (F32, F16 or BF16, rows y_stride values
  *   apart).
  * syn_i8_gate_up_act: W [2 n_out, k_in] holds gate rows, then up rows: y = silu(g) u of the two F32
  *   values, silu(g) = g / (1 + exp(-g)) within four steps of F32, the product rounded once more to y's type.
  * syn_i8_act_quantize, then syn_i8_gemv_quantized: the product's two halves over a workspace of
- *   syn_i8_gemv_workspace_bytes, for several matrices on the same rows (one whose products share it one
+ *   syn_i8_gemv_quantized_workspace_bytes, for several matrices on the same rows (one whose products share it one
  *   after another; of the largest workspace of them, else K may be split less, to the same values).
  * syn_i8_logits: RmsNorm of F32 rows as syn_rms_norm (k_in <= 16384), then the head as syn_i8_gemv; the
  *   workspace holds the normalised rows first.
- * At most SYN_I8_MAX_ROWS activation rows and 2^24 - 1 weight rows.  Workspaces are 256-byte aligned; gated is 1 for syn_i8_gate_up_act, else 0. */
+ * At most SYN_I8_MAX_ROWS activation rows and 2^24 - 1 weight rows.  Workspaces are 256-byte
+ * aligned. */
 #define SYN_I8_MAX_K 131072
 #define SYN_I8_MAX_ROWS 2097120
 int syn_i8_quantize(int32_t xtype, const void* x, uint64_t x_stride, uint32_t rows, uint32_t k, int8_t* codes,
                     uint64_t code_stride, float* scales, void* stream);
 int syn_i8_gemv_workspace_bytes(uint32_t n_out, uint32_t k_in, uint32_t rows, int32_t gated, uint64_t* bytes);
+int syn_i8_gemv_quantized_workspace_bytes(uint32_t n_out, uint32_t k_in, uint32_t rows, uint64_t* bytes);
 int syn_i8_gemv(const int8_t* w, uint64_t w_bytes, uint64_t w_stride, const float* w_scales, const float* bias,
                 uint32_t n_out, uint32_t k_in, int32_t xtype, const void* x, uint64_t x_stride, uint32_t rows,
                 int32_t ytype, void* y, uint64_t y_stride, void* ws, uint64_t ws_bytes, void* stream);

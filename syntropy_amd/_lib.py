@@ -70,6 +70,7 @@ def lib():
         "syn_logits": [u32, i32, vp, u64, u32, u32, vp, C.c_float, vp, u32, vp, vp, u64, vp],
         "syn_i8_quantize": [i32, vp, u64, u32, u32, vp, u64, vp, vp],
         "syn_i8_gemv_workspace_bytes": [u32, u32, u32, i32, C.POINTER(C.c_uint64)],
+        "syn_i8_gemv_quantized_workspace_bytes": [u32, u32, u32, C.POINTER(C.c_uint64)],
         "syn_i8_gemv": [vp, u64, u64, vp, vp, u32, u32, i32, vp, u64, u32, i32, vp, u64, vp, u64, vp],
         "syn_i8_gate_up_act": [vp, u64, u64, vp, vp, u32, u32, i32, vp, u64, u32, i32, vp, u64, vp, u64, vp],
         "syn_i8_act_quantize": [i32, vp, u64, u32, u32, vp, u64, vp],

@@ -7,13 +7,18 @@
 //
 // One pass, bound by reading the logits once.  A wavefront takes steps of 64 lanes x 16 values; each lane
 // keeps its own running m, s and e and rescales them where its maximum grows, so that no lane waits for
-// another until the end.  The greatest ones are keys (ordered value, then the index from below), which are
-// all different: a wavefront holds its 64 greatest, a lane each in order, and their top-th is a bound that
-// almost no later value passes; a step is looked at closer only where a lane's maximum does.  What passes is
-// gathered in LDS and sorted in 64 at a time (bitonic, across lanes without LDS).  The bound of the first
-// step is the top-th of the lanes' maxima, and the wavefronts of a workgroup share the best bound.
+// another until the end.  For the greatest ones the pass keeps each lane's maximum over every few steps (a
+// group, at most 32 of them) in LDS and nothing more: the top-th of the 256 lanes' maxima is a bound that
+// only a few values besides those maxima reach, and the lanes that reach it read their groups that do again.
+// (Looking at each step's values as they come costs more than the sums: the bound is low at first, and a
+// step of 1024 values nearly always holds one above it.)  Those values as keys (ordered value, then the
+// index from below; all different) are gathered in LDS in any order, and each finds its place by counting
+// the greater ones: a few dozen, in less time and code than a sort across lanes.  Where equal values fill the
+// LDS, the `top` greatest of it stay and raise the bound.
 //
 // Few rows: a row is split over workgroups, whose parts a second launch joins.
+#include <type_traits>
+
 #include "common.hpp"
 #include "kernels.hpp"
 
@@ -24,6 +29,7 @@ namespace {
 constexpr int LP_WAVES = 4;
 constexpr int LP_VALUES = 16;              // a lane's values a step
 constexpr int LP_STEP = 64 * LP_VALUES;
+constexpr int LP_GROUPS = 32;
 constexpr float LOG2E = 1.44269504088896340736f;
 
 // A whole number that orders as the value does (-0 as +0, every NaN above +infinity), and the value again.
@@ -37,102 +43,70 @@ SYN_DEV float lp_value(uint32_t k) { return u2f(k >> 31 ? k ^ 0x80000000u : ~k);
 SYN_DEV uint64_t lp_key(float v, int i) { return (uint64_t)lp_order(v) << 32 | (0x7FFFFFFFu - (uint32_t)i); }
 SYN_DEV int lp_index(uint64_t k) { return (int)(0x7FFFFFFFu - (uint32_t)k); }
 
-// Lane l's word from lane l ^ D.
-template <int D>
-SYN_DEV uint32_t lane_xor(uint32_t v) {
-    if constexpr (D == 1) return dpp_u32<DPP_XOR1>(v);
-    if constexpr (D == 2) return dpp_u32<DPP_XOR2>(v);
-    if constexpr (D == 4) return dpp_u32<0x1B>(dpp_u32<DPP_HALF_MIRROR>(v));  // 7 - l, then l ^ 3
-    if constexpr (D == 8) return dpp_u32<0x128>(v);                           // rotated by 8 in a row of 16
-    if constexpr (D == 16) {
-        const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);  // rows 0, 0, 2, 2 and 1, 1, 3, 3
-        return threadIdx.x & 16 ? s[0] : s[1];
+// The greatest number that at least n of a wavefront's values (four a lane) reach, but for its last 14 bits
+// (which let a few more values pass).  Two bits a turn: a turn is the wait for the counts.
+SYN_DEV uint32_t reached_by(const uint32_t (&v)[4], int n) {
+    uint32_t r = 0;
+#pragma unroll 1
+    for (int at = 30; at >= 14; at -= 2) {
+        int c[3] = {0, 0, 0};
+#pragma unroll
+        for (uint32_t b = 1; b < 4; ++b)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) c[b - 1] += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[j] >= (r | b << at)));
+        r |= (c[2] >= n ? 3u : c[1] >= n ? 2u : c[0] >= n ? 1u : 0u) << at;
     }
-    if constexpr (D == 32) {
-        const auto s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-        return threadIdx.x & 32 ? s[0] : s[1];
-    }
-}
-template <int D>
-SYN_DEV uint64_t lane_xor64(uint64_t v) {
-    return (uint64_t)lane_xor<D>((uint32_t)(v >> 32)) << 32 | lane_xor<D>((uint32_t)v);
-}
-// One exchange of a bitonic network: the greater of the pair to the lower lane where `down`, else to the upper.
-template <int D>
-SYN_DEV void exchange(uint64_t& k, bool down) {
-    const uint64_t o = lane_xor64<D>(k);
-    const bool lower = (threadIdx.x & D) == 0;
-    k = (o > k) == (lower == down) ? o : k;
-}
-// 64 lanes' keys that rise to a lane and fall from it (or the other way): in descending order.
-SYN_DEV void merge64(uint64_t& k) {
-    exchange<32>(k, true);
-    exchange<16>(k, true);
-    exchange<8>(k, true);
-    exchange<4>(k, true);
-    exchange<2>(k, true);
-    exchange<1>(k, true);
-}
-SYN_DEV void sort64(uint64_t& k) {
-    const int l = threadIdx.x & 63;
-    exchange<1>(k, (l & 2) == 0);
-    exchange<2>(k, (l & 4) == 0);
-    exchange<1>(k, (l & 4) == 0);
-    exchange<4>(k, (l & 8) == 0);
-    exchange<2>(k, (l & 8) == 0);
-    exchange<1>(k, (l & 8) == 0);
-    exchange<8>(k, (l & 16) == 0);
-    exchange<4>(k, (l & 16) == 0);
-    exchange<2>(k, (l & 16) == 0);
-    exchange<1>(k, (l & 16) == 0);
-    exchange<16>(k, (l & 32) == 0);
-    exchange<8>(k, (l & 32) == 0);
-    exchange<4>(k, (l & 32) == 0);
-    exchange<2>(k, (l & 32) == 0);
-    exchange<1>(k, (l & 32) == 0);
-    merge64(k);
-}
-SYN_DEV uint64_t lane_key(uint64_t k, int lane) {  // uniform
-    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), lane) << 32 |
-           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, lane);
+    return r;
 }
 
-// A wavefront's greatest keys so far.
+constexpr int LP_ROOM = 512;
+// A workgroup's greatest keys so far, in LDS.
 struct Greatest {
-    uint64_t list = 0;   // lane l: the l-th greatest
-    uint64_t bound = 0;  // only a key above it can be among the `top` greatest
-    int waiting = 0;     // keys in buf
-    uint64_t* buf;       // LDS, 128 of this wavefront
-    int top;
+    uint64_t keys[LP_ROOM];                // in any order
+    uint64_t sorted[LOGPROB_MAX_TOP];      // of sort()
+    uint32_t most[64 * LP_WAVES];          // the lanes' greatest
+    int count;                             // of keys, and of those that found no room
+    int more[2][LP_WAVES];
 
-    SYN_DEV void take() {  // the first 64 of buf into the list
-        const int l = threadIdx.x & 63;
-        wave_lds_sync();
-        uint64_t k = l < waiting ? buf[l] : 0;
-        const uint64_t rest = buf[64 + l];
-        wave_lds_sync();
-        buf[l] = rest;
-        waiting = waiting > 64 ? waiting - 64 : 0;
-        // against the list in reverse, so that the pairs' greater ones are the 64 greatest
-        sort64(k);
-        const uint64_t rev = lane_xor64<32>(lane_xor64<16>(lane_xor64<8>(lane_xor64<4>(lane_xor64<2>(lane_xor64<1>(k))))));
-        list = rev > list ? rev : list;
-        merge64(list);
-        const uint64_t b = lane_key(list, top - 1);
-        bound = b > bound ? b : bound;
+    // (every thread; a barrier before and after) the `top` greatest in order; returns how many there are
+    SYN_DEV int sort(int top) {
+        const int n = count < LP_ROOM ? count : LP_ROOM;
+        for (int j = threadIdx.x; j < n; j += 64 * LP_WAVES) {
+            const uint64_t k = keys[j];
+            int rank = 0;
+#pragma unroll 4
+            for (int i = 0; i < n; ++i) rank += keys[i] > k ? 1 : 0;
+            if (rank < top) sorted[rank] = k;
+        }
+        return n < top ? n : top;
     }
-    SYN_DEV void push(uint64_t k, bool pass) {
-        const uint64_t m = __builtin_amdgcn_ballot_w64(pass);
-        if (m == 0) return;  // uniform
-        const int at = waiting + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
-        if (pass) buf[at] = k;
-        waiting += __builtin_popcountll(m);
-        if (waiting >= 64) take();
+    // true where it found no room
+    SYN_DEV bool put(uint64_t k) {
+        const int at = atomicAdd(&count, 1);
+        if (at < LP_ROOM) keys[at] = k;
+        return at >= LP_ROOM;
     }
-    SYN_DEV void finish() {
-        while (waiting > 0) take();
+    // (every thread, after put) whether any thread has more to put; where there is no room left, the bound is
+    // raised to the top-th of what there is, and only the greatest stay
+    SYN_DEV bool round(bool mine, int parity, int top, uint64_t& bound) {
+        const bool any = __builtin_amdgcn_ballot_w64(mine) != 0;
+        if ((threadIdx.x & 63) == 0) more[parity][threadIdx.x >> 6] = any;
+        __syncthreads();
+        bool go = false;
+        for (int w = 0; w < LP_WAVES; ++w) go |= more[parity][w] != 0;
+        if (count >= LP_ROOM) {  // uniform
+            sort(top);
+            __syncthreads();
+            const uint64_t b = sorted[top - 1];
+            bound = b > bound ? b : bound;
+            if ((int)threadIdx.x < top) keys[threadIdx.x] = sorted[threadIdx.x];
+            if (threadIdx.x == 0) count = top;
+            __syncthreads();
+        }
+        return go;
     }
 };
+static_assert(LP_ROOM > LOGPROB_MAX_TOP, "room behind those that stay");
 
 // A running softmax: the greatest, the sum of exponentials, the sum of exponentials times their arguments.
 struct Soft {
@@ -154,13 +128,15 @@ struct Soft {
     }
     SYN_DEV float base() const { return m == -__builtin_inff() ? 0.0f : m; }
 };
+SYN_DEV float max_of_lanes(float v) {
+    for (int d = 1; d < 64; d *= 2) v = fmaxf(v, __shfl_xor(v, d));
+    return v;
+}
 SYN_DEV Soft soft_of_lanes(Soft v) {
+    v.rebase(max_of_lanes(v.m));
     for (int d = 1; d < 64; d *= 2) {
-        Soft o;
-        o.m = __shfl_xor(v.m, d);
-        o.s = __shfl_xor(v.s, d);
-        o.e = __shfl_xor(v.e, d);
-        v.add(o);
+        v.s += __shfl_xor(v.s, d);
+        v.e += __shfl_xor(v.e, d);
     }
     return v;
 }
@@ -174,27 +150,32 @@ struct Values {
     static SYN_DEV int index(int first, int i) {
         return first + 64 * PER * (i / PER) + PER * (int)(threadIdx.x & 63) + i % PER;
     }
+    // The step's values, -infinity past the row's end; `first` may be another in every lane.  (The row's last
+    // step one value a load, each at an index that is there: a branch around each would wait for the one
+    // before.)
     SYN_DEV void load(const uint8_t* row, int first, int vocab) {
-        constexpr int ES = TY == T_F32 ? 4 : 2;
-        if (first + LP_STEP <= vocab) {  // uniform; pieces at any value's address
+        if (__builtin_amdgcn_ballot_w64(first + LP_STEP > vocab) == 0) {  // uniform
 #pragma unroll
-            for (int p = 0; p < LP_VALUES / PER; ++p)
-                __builtin_memcpy(w + 4 * p, row + (int64_t)index(first, PER * p) * ES, 16);
-        } else {
-#pragma unroll
-            for (int j = 0; j < WORDS; ++j) {
-                if constexpr (TY == T_F32) {
-                    const int i = index(first, j);
-                    w[j] = i < vocab ? ((const uint32_t*)row)[i] : 0xFF800000u;
-                } else {
-                    constexpr uint32_t NONE = TY == T_F16 ? 0xFC00u : 0xFF80u;
-                    const int i = index(first, 2 * j);
-                    const uint32_t lo = i < vocab ? ((const uint16_t*)row)[i] : NONE;
-                    const uint32_t hi = i + 1 < vocab ? ((const uint16_t*)row)[i + 1] : NONE;
-                    w[j] = lo | hi << 16;
-                }
-            }
+            for (int p = 0; p < LP_VALUES / PER; ++p)  // (pieces at any value's address)
+                __builtin_memcpy(w + 4 * p, row + (int64_t)index(first, PER * p) * (16 / PER), 16);
+            return;
         }
+        uint32_t v[LP_VALUES];
+#pragma unroll
+        for (int i = 0; i < LP_VALUES; ++i) {
+            const int id = index(first, i), in = id < vocab ? id : vocab - 1;
+            if constexpr (TY == T_F32)
+                v[i] = ((const uint32_t*)row)[in];
+            else
+                v[i] = ((const uint16_t*)row)[in];
+        }
+#pragma unroll
+        for (int i = 0; i < LP_VALUES; ++i) {
+            constexpr uint32_t NONE = TY == T_F32 ? 0xFF800000u : TY == T_F16 ? 0xFC00u : 0xFF80u;
+            v[i] = index(first, i) < vocab ? v[i] : NONE;
+        }
+#pragma unroll
+        for (int j = 0; j < WORDS; ++j) w[j] = TY == T_F32 ? v[j] : v[2 * j % LP_VALUES] | v[(2 * j + 1) % LP_VALUES] << 16;
     }
     SYN_DEV float at(int i) const {
         if constexpr (TY == T_F32) return u2f(w[i]);
@@ -215,15 +196,15 @@ SYN_DEV int64_t lp_token(const LogprobArgs& g, uint64_t row) {
     return g.wide ? ((const int64_t*)g.tokens)[row] : ((const int32_t*)g.tokens)[row];
 }
 
-// A part's results: m, s, e and the rank's count, then its `top` greatest keys.
+// A part's results: m, s, e and the rank's count; its `top` greatest keys lie behind all parts.
 struct Part {
     float m, s, e;
     uint32_t above;
 };
-SYN_HD inline uint64_t part_bytes(int top) { return sizeof(Part) + 8 * (uint64_t)top; }
 
-// The row's results from its softmax, count and list (lane l the l-th greatest), by one wavefront.
-SYN_DEV void lp_write(const LogprobArgs& g, uint64_t row, const Soft& v, uint32_t above, float xt, int64_t t, uint64_t list) {
+// The row's results from its softmax, count and sorted keys, by one wavefront.
+SYN_DEV void lp_write(const LogprobArgs& g, uint64_t row, const Soft& v, uint32_t above, float xt, int64_t t,
+                      const uint64_t* sorted) {
     const int lane = threadIdx.x & 63;
     const bool none = v.s == 0.0f;
     const float ls = logf(v.s), base = v.base();
@@ -234,27 +215,28 @@ SYN_DEV void lp_write(const LogprobArgs& g, uint64_t row, const Soft& v, uint32_
         g.entropy[row] = none ? 0.0f : ls - v.e / v.s;
     }
     if (lane < g.top) {
-        g.top_ids[row * g.top + lane] = lp_index(list);
-        g.top_logprobs[row * g.top + lane] =
-            none ? -__builtin_inff() : (lp_value((uint32_t)(list >> 32)) * g.scale - base) - ls;
+        const uint64_t k = sorted[lane];
+        g.top_ids[row * g.top + lane] = lp_index(k);
+        g.top_logprobs[row * g.top + lane] = none ? -__builtin_inff() : (lp_value((uint32_t)(k >> 32)) * g.scale - base) - ls;
     }
 }
 
 }  // namespace
 
 template <int TY, int TOP>
-__global__ __launch_bounds__(64 * LP_WAVES) void k_logprobs(LogprobArgs g, int parts, int part_steps) {
+__global__ __launch_bounds__(64 * LP_WAVES) void k_logprobs(LogprobArgs g, int parts, int part_steps, int group_steps) {
     const uint64_t row = blockIdx.x / (uint32_t)parts;
     const int part = (int)(blockIdx.x % (uint32_t)parts);
     const uint8_t* x = (const uint8_t*)g.x + row * g.ldx * (TY == T_F32 ? 4 : 2);
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    __shared__ uint64_t buf[TOP ? LP_WAVES : 1][TOP ? 128 : 1];
-    __shared__ unsigned long long shared_bound;
+    __shared__ uint32_t groups[TOP ? LP_WAVES : 1][TOP ? LP_GROUPS : 1][64];
+    __shared__ typename std::conditional<TOP != 0, Greatest, int>::type best;
     __shared__ Part sums[LP_WAVES];
     const int steps = (g.vocab + LP_STEP - 1) / LP_STEP;
     const int last = (part + 1) * part_steps < steps ? (part + 1) * part_steps : steps;
-    int step = part * part_steps + wave;
+    const int step0 = part * part_steps + wave;
+    int step = step0;
 
     using V = Values<TY>;
     V cur, nxt;
@@ -262,19 +244,12 @@ __global__ __launch_bounds__(64 * LP_WAVES) void k_logprobs(LogprobArgs g, int p
     const int64_t t = lp_token(g, row);
     const bool known = t >= 0 && t < g.vocab;
     const float xt = known ? lp_load<TY>(x, t) : __builtin_nanf("");  // (nothing is above a NaN)
-    if (TOP) {
-        if (threadIdx.x == 0) shared_bound = 0;
-        __syncthreads();
-    }
 
     Soft v;
     uint32_t above = 0;
-    Greatest best;
-    best.buf = buf[TOP ? wave : 0];
-    best.top = g.top;
-    bool first = true;
+    float most = -__builtin_inff(), group = most;  // the lane's greatest value, and that of its group
+    int in_group = 0, n_groups = 0;
     while (step < last) {  // uniform
-        const int at = step * LP_STEP;
         step += LP_WAVES;
         if (step < last) nxt.load(x, step * LP_STEP, g.vocab);
         float mx = cur.at(0);
@@ -291,41 +266,60 @@ __global__ __launch_bounds__(64 * LP_WAVES) void k_logprobs(LogprobArgs g, int p
             above += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(xi > xt));
         }
         if constexpr (TOP) {
-            if (first) {  // the bound from the lanes' greatest
-                uint64_t k = 0;
-#pragma unroll
-                for (int i = 0; i < LP_VALUES; ++i) {
-                    const int id = V::index(at, i);
-                    const uint64_t o = id < g.vocab ? lp_key(cur.at(i), id) : 0;
-                    k = o > k ? o : k;
-                }
-                sort64(k);
-                const uint64_t b = lane_key(k, g.top - 1);
-                best.bound = b ? b - 1 : 0;  // (that one passes too)
-                first = false;
-            }
-            const uint64_t sb = *(volatile unsigned long long*)&shared_bound;
-            best.bound = sb > best.bound ? sb : best.bound;
-            const float bv = lp_value((uint32_t)(best.bound >> 32));
-            // (the bound below a first key may be its neighbour's in value: not above, but equal)
-            if (__builtin_amdgcn_ballot_w64(!(mx < bv) || v.s != v.s) != 0) {
-#pragma unroll
-                for (int i = 0; i < LP_VALUES; ++i) {
-                    const int id = V::index(at, i);
-                    const uint64_t k = id < g.vocab ? lp_key(cur.at(i), id) : 0;
-                    best.push(k, k > best.bound);
-                }
-                if (lane == 0) atomicMax(&shared_bound, (unsigned long long)best.bound);
+            group = fmaxf(group, mx);
+            if (++in_group == group_steps || step >= last) {
+                most = fmaxf(most, group);
+                // (once a NaN or +infinity is in the sum, every group may hold a NaN)
+                groups[wave][n_groups++][lane] = v.s != v.s ? 0xFFFFFFFFu : lp_order(group);
+                group = -__builtin_inff();
+                in_group = 0;
             }
         }
         cur = nxt;
     }
+    if constexpr (TOP) {
+        best.most[threadIdx.x] = lp_order(most);
+        if (threadIdx.x == 0) best.count = 0;
+        __syncthreads();
+        uint32_t of[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) of[j] = best.most[lane + 64 * j];
+        const uint32_t b = reached_by(of, g.top);
+        uint64_t bound = b ? ((uint64_t)b << 32) - 1 : 0;  // all of that value are above it
+        uint32_t mine = 0;  // the lane's groups that reach it
+        for (int i = 0; i < n_groups; ++i) mine |= groups[wave][i][lane] >= b ? 1u << i : 0u;
+        uint32_t may = 0;  // the lane's values of `cur` that may pass (a NaN may)
+        int at = 0, in = 0;
+        bool go = true;
+#pragma unroll 1
+        for (int parity = 0; go; parity ^= 1) {  // uniform
+            if (may == 0 && mine != 0) {         // the lane's next step
+                const int gi = __builtin_ctz(mine), st = step0 + (gi * group_steps + in) * LP_WAVES;
+                at = st * LP_STEP;
+                // (equal values: a group behind the bound's index holds nothing before it)
+                if (st < last &&
+                    ((uint64_t)groups[wave][gi][lane] << 32 | (0x7FFFFFFFu - (uint32_t)V::index(at, 0))) > bound) {
+                    const float bv = lp_value((uint32_t)((bound + 1) >> 32));
+                    cur.load(x, at, g.vocab);
+#pragma unroll
+                    for (int i = 0; i < LP_VALUES; ++i) may |= !(cur.at(i) < bv) ? 1u << i : 0u;
+                }
+                if (++in == group_steps) in = 0, mine &= mine - 1;
+            }
+#pragma unroll 1
+            for (; may != 0; may &= may - 1) {  // each lane its own
+                const int i = __builtin_ctz(may), id = V::index(at, i);
+                if (id >= g.vocab) continue;
+                const uint64_t key = lp_key(lp_load<TY>(x, id), id);  // (a choice of the registers by lane costs more)
+                if (key > bound && best.put(key)) break;
+            }
+            go = best.round(may != 0 || mine != 0, parity, g.top, bound);
+        }
+        const int n = best.sort(g.top);
+        if ((int)threadIdx.x >= n && (int)threadIdx.x < g.top) best.sorted[threadIdx.x] = 0;
+    }
     v = soft_of_lanes(v);
     if (lane == 0) sums[wave] = Part{v.m, v.s, v.e, above};
-    if constexpr (TOP) {
-        best.finish();
-        buf[wave][lane] = best.list;
-    }
     __syncthreads();
     if (wave != 0) return;
 #pragma unroll
@@ -337,73 +331,76 @@ __global__ __launch_bounds__(64 * LP_WAVES) void k_logprobs(LogprobArgs g, int p
         ov.e = o.e;
         v.add(ov);
         above += o.above;
-        if constexpr (TOP) {
-            const uint64_t rev = buf[w][63 - lane];
-            best.list = rev > best.list ? rev : best.list;
-            merge64(best.list);
-        }
     }
+    const uint64_t* sorted = nullptr;
+    if constexpr (TOP) sorted = best.sorted;
     if (parts == 1) {
-        lp_write(g, row, v, above, xt, t, best.list);
+        lp_write(g, row, v, above, xt, t, sorted);
     } else {
-        uint8_t* to = g.ws + ((uint64_t)row * parts + part) * part_bytes(g.top);
-        if (lane == 0) *(Part*)to = Part{v.m, v.s, v.e, above};
-        if (lane < g.top) ((uint64_t*)(to + sizeof(Part)))[lane] = best.list;
+        if (lane == 0) ((Part*)g.ws)[row * parts + part] = Part{v.m, v.s, v.e, above};
+        uint64_t* keys = (uint64_t*)(g.ws + (uint64_t)g.rows * parts * sizeof(Part));
+        if (TOP && lane < g.top) keys[(row * parts + part) * g.top + lane] = sorted[lane];
     }
 }
 
-// The parts of a row, by one wavefront.
-template <int TY>
-__global__ __launch_bounds__(64) void k_logprobs_join(LogprobArgs g, int parts) {
+// The parts of a row.
+template <int TY, int TOP>
+__global__ __launch_bounds__(TOP ? 64 * LP_WAVES : 64) void k_logprobs_join(LogprobArgs g, int parts) {
     const uint64_t row = blockIdx.x;
-    const int lane = threadIdx.x;
-    __shared__ uint64_t buf[128];
-    const uint8_t* from = g.ws + row * parts * part_bytes(g.top);
+    const int lane = threadIdx.x & 63;
+    __shared__ typename std::conditional<TOP != 0, Greatest, int>::type best;
+    const Part* from = (const Part*)g.ws + row * parts;
     const int64_t t = lp_token(g, row);
     const float xt = t >= 0 && t < g.vocab ? lp_load<TY>((const uint8_t*)g.x + row * g.ldx * (TY == T_F32 ? 4 : 2), t) : 0.0f;
     Soft v;
     uint32_t above = 0;
-    for (int p = lane; p < parts; p += 64) {
-        const Part o = *(const Part*)(from + p * part_bytes(g.top));
-        Soft ov;
-        ov.m = o.m;
-        ov.s = o.s;
-        ov.e = o.e;
-        v.add(ov);
-        above += o.above;
+    if (lane < parts) {  // (at most 64)
+        const Part o = from[lane];
+        v.m = o.m;
+        v.s = o.s;
+        v.e = o.e;
+        above = o.above;
+    }
+    const uint64_t* sorted = nullptr;
+    if constexpr (TOP) {
+        const uint64_t* keys = (const uint64_t*)(g.ws + (uint64_t)g.rows * parts * sizeof(Part)) + row * parts * g.top;
+        const int n = parts * g.top;
+        uint64_t k = (int)threadIdx.x < n ? keys[threadIdx.x] : 0, mx = k;
+        for (int i = threadIdx.x + 64 * LP_WAVES; i < n; i += 64 * LP_WAVES) mx = keys[i] > mx ? keys[i] : mx;
+        best.most[threadIdx.x] = (uint32_t)(mx >> 32);
+        if (threadIdx.x == 0) best.count = 0;
+        __syncthreads();
+        uint32_t of[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) of[j] = best.most[lane + 64 * j];
+        const uint32_t b = reached_by(of, g.top);
+        uint64_t bound = b ? ((uint64_t)b << 32) - 1 : 0;
+        bool go = true;
+        int i = threadIdx.x;
+#pragma unroll 1
+        for (int parity = 0; go; parity ^= 1) {  // uniform
+            if (i < n && !(k > bound && best.put(k))) {
+                i += 64 * LP_WAVES;
+                k = i < n ? keys[i] : 0;
+            }
+            go = best.round(i < n, parity, g.top, bound);
+        }
+        best.sort(g.top);  // (at least `top` of them: the vocabulary has as many)
+        __syncthreads();
+        if (threadIdx.x >= 64) return;
+        sorted = best.sorted;
     }
     v = soft_of_lanes(v);
     for (int d = 1; d < 64; d *= 2) above += __shfl_xor(above, d);
-    Greatest best;
-    best.buf = buf;
-    best.top = g.top;
-    if (g.top) {
-        const int n = parts * g.top;
-        auto key = [&](int i) -> uint64_t {
-            return i < n ? ((const uint64_t*)(from + (uint64_t)(i / g.top) * part_bytes(g.top) + sizeof(Part)))[i % g.top] : 0;
-        };
-        uint64_t k = 0;
-        for (int i = lane; i < n; i += 64) {
-            const uint64_t o = key(i);
-            k = o > k ? o : k;
-        }
-        sort64(k);
-        const uint64_t b = lane_key(k, g.top - 1);
-        best.bound = b ? b - 1 : 0;
-        for (int i = 0; i < n; i += 64) {
-            const uint64_t o = key(i + lane);
-            best.push(o, o > best.bound);
-        }
-        best.finish();
-    }
-    lp_write(g, row, v, above, xt, t, best.list);
+    lp_write(g, row, v, above, xt, t, sorted);
 }
 
-// Parts a row: enough workgroups to keep reads in flight on every CU, each of at least a step a wavefront.
+// Parts a row: about 1024 workgroups keep reads in flight on every CU (256 rows of 128256 BF16, 20 greatest:
+// 36 us in parts for 256, 28 for 1024, 33 for 2048), each of at least a step a wavefront.
 static int lp_parts(int rows, int vocab) {
     const int steps = (vocab + LP_STEP - 1) / LP_STEP;
     const int most = (steps + LP_WAVES - 1) / LP_WAVES;
-    int p = 512 / rows;
+    int p = 1024 / rows;
     p = p < most ? p : most;
     p = p < 64 ? p : 64;
     return p < 1 ? 1 : p;
@@ -413,18 +410,22 @@ static int lp_part_steps(int parts, int vocab) { return ((vocab + LP_STEP - 1) /
 uint64_t logprob_ws_bytes(int rows, int vocab, int top) {
     if (rows == 0) return 0;
     const int p = lp_parts(rows, vocab);
-    return p > 1 ? align_up((uint64_t)rows * p * part_bytes(top), 256) : 0;
+    return p > 1 ? align_up((uint64_t)rows * p * (sizeof(Part) + 8 * (uint64_t)top), 256) : 0;
 }
 
 template <int TY>
 static void logprobs_as(const LogprobArgs& a, hipStream_t stream) {
     const int parts = lp_parts(a.rows, a.vocab), ps = lp_part_steps(parts, a.vocab);
+    const int wave_steps = (ps + LP_WAVES - 1) / LP_WAVES, gs = (wave_steps + LP_GROUPS - 1) / LP_GROUPS;
     const dim3 grid((uint32_t)a.rows * (uint32_t)parts);
     if (a.top)
-        hipLaunchKernelGGL((k_logprobs<TY, 1>), grid, dim3(64 * LP_WAVES), 0, stream, a, parts, ps);
+        hipLaunchKernelGGL((k_logprobs<TY, 1>), grid, dim3(64 * LP_WAVES), 0, stream, a, parts, ps, gs);
     else
-        hipLaunchKernelGGL((k_logprobs<TY, 0>), grid, dim3(64 * LP_WAVES), 0, stream, a, parts, ps);
-    if (parts > 1) hipLaunchKernelGGL(k_logprobs_join<TY>, dim3(a.rows), dim3(64), 0, stream, a, parts);
+        hipLaunchKernelGGL((k_logprobs<TY, 0>), grid, dim3(64 * LP_WAVES), 0, stream, a, parts, ps, gs);
+    if (parts > 1 && a.top)
+        hipLaunchKernelGGL((k_logprobs_join<TY, 1>), dim3(a.rows), dim3(64 * LP_WAVES), 0, stream, a, parts);
+    else if (parts > 1)
+        hipLaunchKernelGGL((k_logprobs_join<TY, 0>), dim3(a.rows), dim3(64), 0, stream, a, parts);
 }
 
 void launch_logprobs(const LogprobArgs& a, hipStream_t stream) {

@@ -250,46 +250,34 @@ def _value_type(t: torch.Tensor, what: str) -> int:
 def _ptr_rows(t: torch.Tensor, rows: int, n: int, what: str, device=None) -> int:
     """The row stride, in values, of a device tensor of at least `rows` rows of n values side by side: one
     of two dimensions with any row stride, or a contiguous one of enough values."""
-    if not t.is_cuda or (device is not None and t.device != device):
+    if not t.is_cuda or (device is not None and t.get_device() != device):
         raise GemvError("Len", f"`{what}` must be on the operands' device")
     if rows < 0:
         raise GemvError("Len", f"{rows} rows")
-    if t.dim() == 2 and t.shape[1] == n and t.shape[0] >= rows and (t.stride(1) == 1 or n == 1):
-        if rows <= 1 or t.stride(0) >= n:
-            return max(t.stride(0), n)
+    if t.dim() == 2 and t.shape[1] == n and t.shape[0] >= rows:
+        step, inner = t.stride()
+        if (inner == 1 or n == 1) and (rows <= 1 or step >= n):
+            return step if step > n else n
     if not t.is_contiguous() or t.numel() < rows * n:
         raise GemvError("Len", f"`{what}` holds {t.numel()} values, the op needs {rows} rows of {n} side by side")
     return n
 
 
-class _on:
-    """The stream a call runs on: `stream` (a torch stream or a handle), or the current one of t's device,
-    with that device current, and what torch allocates meanwhile belonging to that stream."""
-
-    __slots__ = ("device", "stream", "held")
-
-    def __init__(self, t: torch.Tensor, stream):
-        self.device, self.stream, self.held = t.device.index, stream, None
-
-    def __enter__(self) -> int:
-        if self.stream is None and self.device == torch.cuda.current_device():
-            return torch._C._cuda_getCurrentRawStream(self.device)
-        if self.stream is None:
-            self.held = torch.cuda.device(self.device)
-            self.held.__enter__()
-            return torch._C._cuda_getCurrentRawStream(self.device)
-        s = self.stream
-        if not hasattr(s, "cuda_stream"):
-            s = torch.cuda.ExternalStream(int(s), device=self.device)
-        if s.device.index != self.device:
-            raise GemvError("Len", f"the stream is of {s.device}, the operands of cuda:{self.device}")
-        self.held = torch.cuda.stream(s)
-        self.held.__enter__()
-        return s.cuda_stream
-
-    def __exit__(self, *e):
-        if self.held is not None:
-            self.held.__exit__(*e)
+def _on_stream(t: torch.Tensor, stream, body):
+    """body(handle) on `stream` (a torch stream or a handle), or on the current one of t's device, with that
+    device current, and what torch allocates meanwhile belonging to that stream."""
+    device = t.get_device()
+    if stream is None:
+        if device == torch._C._cuda_getDevice():
+            return body(torch._C._cuda_getCurrentRawStream(device))
+        with torch.cuda.device(device):
+            return body(torch._C._cuda_getCurrentRawStream(device))
+    if not hasattr(stream, "cuda_stream"):
+        stream = torch.cuda.ExternalStream(int(stream), device=device)
+    if stream.device.index != device:
+        raise GemvError("Len", f"the stream is of {stream.device}, the operands of cuda:{device}")
+    with torch.cuda.stream(stream):
+        return body(stream.cuda_stream)
 
 
 class TokenLogprobs(NamedTuple):
@@ -321,18 +309,20 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, sca
     if tokens.dtype not in (torch.int32, torch.int64) or not tokens.is_contiguous() or tokens.device != logits.device:
         raise GemvError("Len", "tokens must be contiguous int32 or int64 values beside the logits")
     ty, stride = _value_type(logits, "logits"), _ptr_rows(logits, rows, vocab, "logits")
-    with _on(logits, stream) as s:
-        dev = logits.device
-        values = torch.empty(2, rows, dtype=torch.float32, device=dev)
-        ranks = torch.empty(rows, dtype=torch.int32, device=dev)
-        ids = torch.empty(rows, top, dtype=torch.int32, device=dev)
-        lps = torch.empty(rows, top, dtype=torch.float32, device=dev)
+    dev = logits.device
+
+    def launch(handle):
+        f32, i32 = torch.float32, torch.int32
+        r = TokenLogprobs(torch.empty(rows, dtype=f32, device=dev), torch.empty(rows, dtype=i32, device=dev),
+                          torch.empty(rows, dtype=f32, device=dev), torch.empty(rows, top, dtype=i32, device=dev),
+                          torch.empty(rows, top, dtype=f32, device=dev))
         need = _need("syn_token_logprobs_workspace_bytes", ty, rows, vocab, top)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         call("syn_token_logprobs", ty, logits.data_ptr(), stride, rows, vocab, tokens.data_ptr(), tokens.element_size(),
-             scale, top, values.data_ptr(), ranks.data_ptr(), values.data_ptr() + 4 * rows, ids.data_ptr(), lps.data_ptr(),
-             ws.data_ptr() if need else None, need, s)
-    return TokenLogprobs(values[0], ranks, values[1], ids, lps)
+             scale, top, r.logprob.data_ptr(), r.rank.data_ptr(), r.entropy.data_ptr(), r.top_ids.data_ptr(),
+             r.top_logprobs.data_ptr(), ws.data_ptr() if need else None, need, handle)
+        return r
+    return _on_stream(logits, stream, launch)
 
 
 class GemvBatch:

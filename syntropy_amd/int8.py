@@ -17,12 +17,12 @@ from dataclasses import dataclass
 import torch
 
 from ._lib import SynError, call
-from .gemv import GemvError, _need, _on, _ptr_rows, _value_type
+from .gemv import GemvError, _need, _on_stream, _ptr_rows, _value_type
 
 MAX_K = 131072
 
 
-@dataclass
+@dataclass(eq=False)
 class Weights:
     """`codes` int8 [n_out, k_in] with F32 `scales` [n_out] and an optional F32 `bias` [n_out], device
     tensors: the row o stands for codes[o] * scales[o].  Rows lie side by side and start on 16 bytes: a
@@ -48,9 +48,14 @@ class Weights:
         if c.stride(1) != 1 or c.stride(0) < self.k_in or c.stride(0) % 16 or c.data_ptr() % 16:
             rows = torch.zeros(self.n_out, -(-self.k_in // 128) * 128, dtype=torch.int8, device=c.device)[:, :self.k_in]
             self.codes = c = rows.copy_(c)
-        self.stride = c.stride(0)
-        self.view_bytes = max(0, (self.n_out - 1) * self.stride + self.k_in)
-        self.bias_ptr = 0 if b is None else b.data_ptr()
+        self.device = c.get_device()
+
+    def view(self) -> tuple:
+        """The C ABI's arguments: the codes' view (address, bytes, stride), scales, bias."""
+        c, b = self.codes, self.bias
+        stride = c.stride(0)
+        return (c.data_ptr(), (self.n_out - 1) * stride + self.k_in if self.n_out else 0, stride, self.scales.data_ptr(),
+                0 if b is None else b.data_ptr())
 
 
 def quantize_rows(x: torch.Tensor, stream=None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -61,11 +66,13 @@ def quantize_rows(x: torch.Tensor, stream=None) -> tuple[torch.Tensor, torch.Ten
         raise GemvError("Len", "x must be rows of values")
     rows, k = x.shape
     ty, stride = _value_type(x, "x"), _ptr_rows(x, rows, k, "x")
-    with _on(x, stream) as s:
+
+    def launch(handle):
         codes = torch.empty(rows, -(-k // 128) * 128, dtype=torch.int8, device=x.device)
         scales = torch.empty(rows, dtype=torch.float32, device=x.device)
-        call("syn_i8_quantize", ty, x.data_ptr(), stride, rows, k, codes.data_ptr(), codes.shape[1], scales.data_ptr(), s)
-    return codes[:, :k], scales
+        call("syn_i8_quantize", ty, x.data_ptr(), stride, rows, k, codes.data_ptr(), codes.shape[1], scales.data_ptr(), handle)
+        return codes[:, :k], scales
+    return _on_stream(x, stream, launch)
 
 
 def quantize_weights(w: torch.Tensor, bias: torch.Tensor | None = None, stream=None) -> Weights:
@@ -75,30 +82,33 @@ def quantize_weights(w: torch.Tensor, bias: torch.Tensor | None = None, stream=N
 
 
 def workspace_bytes(n_out: int, k_in: int, rows: int, gated: bool = False) -> int:
-    """Scratch bytes of a call: the quantized rows, and partial sums where K is split."""
+    """Scratch bytes of a call: the quantized rows (none where the product's kernel quantizes them itself),
+    and partial sums where K is split."""
     return _need("syn_i8_gemv_workspace_bytes", n_out, k_in, rows, 1 if gated else 0)
 
 
-def _out(y, x, rows, n, dtype):
-    if y is None:
-        return torch.empty(rows, n, dtype=dtype or x.dtype, device=x.device)
-    if dtype is not None and dtype != y.dtype:
-        raise GemvError("Len", f"`y` is of {y.dtype}, not {dtype}")
-    return y
-
-
 def _product(name, gated, w, n, x, rows, y, ws, dtype, stream):
-    if x.device != w.codes.device:
-        raise GemvError("Len", f"x is on {x.device}, the weights on {w.codes.device}")
-    ty, xs = _value_type(x, "x"), _ptr_rows(x, rows, w.k_in, "x")
-    with _on(x, stream) as s:
-        y = _out(y, x, rows, n, dtype)
-        yty, ys = _value_type(y, "y"), _ptr_rows(y, rows, n, "y", x.device)
-        if ws is None:
-            ws = torch.empty(max(workspace_bytes(n, w.k_in, rows, gated), 256), dtype=torch.uint8, device=x.device)
-        call(name, w.codes.data_ptr(), w.view_bytes, w.stride, w.scales.data_ptr(), w.bias_ptr, n, w.k_in, ty, x.data_ptr(),
-             xs, rows, yty, y.data_ptr(), ys, ws.data_ptr(), ws.numel(), s)
-    return y
+    ty, xs = _value_type(x, "x"), _ptr_rows(x, rows, w.k_in, "x", w.device)
+    if y is not None:
+        if dtype is not None and dtype != y.dtype:
+            raise GemvError("Len", f"`y` is of {y.dtype}, not {dtype}")
+        yty, ys = _value_type(y, "y"), _ptr_rows(y, rows, n, "y", w.device)
+
+    def launch(handle):
+        if y is None:
+            out = torch.empty(rows, n, dtype=x.dtype if dtype is None else dtype, device=x.device)
+            oty, os = _value_type(out, "y"), n
+        else:
+            out, oty, os = y, yty, ys
+        if ws is not None:
+            wp, wb = ws.data_ptr(), ws.numel()
+        else:
+            wb = _need("syn_i8_gemv_workspace_bytes", n, w.k_in, rows, 1 if gated else 0)
+            scratch = torch.empty(wb, dtype=torch.uint8, device=x.device) if wb else None
+            wp = scratch.data_ptr() if wb else 0
+        call(name, *w.view(), n, w.k_in, ty, x.data_ptr(), xs, rows, oty, out.data_ptr(), os, wp, wb, handle)
+        return out
+    return _on_stream(x, stream, launch)
 
 
 def gemv(w: Weights, x: torch.Tensor, rows: int, y: torch.Tensor | None = None, ws: torch.Tensor | None = None,
@@ -123,27 +133,26 @@ class Rows:
 
     def __init__(self, rows: int, k_in: int, *n_outs: int, device="cuda"):
         self.rows, self.k_in = rows, k_in
-        need = max(workspace_bytes(n, k_in, rows) for n in n_outs or (1,))
+        need = max(_need("syn_i8_gemv_quantized_workspace_bytes", n, k_in, rows) for n in n_outs or (1,))
         self.ws = torch.empty(max(need, 256), dtype=torch.uint8, device=device)
 
 
 def quantize_into(x: torch.Tensor, r: Rows, stream=None) -> None:
     """The first r.rows rows of x into r."""
-    ty, xs = _value_type(x, "x"), _ptr_rows(x, r.rows, r.k_in, "x", r.ws.device)
-    with _on(x, stream) as s:
-        call("syn_i8_act_quantize", ty, x.data_ptr(), xs, r.rows, r.k_in, r.ws.data_ptr(), r.ws.numel(), s)
+    ty, xs = _value_type(x, "x"), _ptr_rows(x, r.rows, r.k_in, "x", r.ws.get_device())
+    _on_stream(x, stream, lambda handle: call("syn_i8_act_quantize", ty, x.data_ptr(), xs, r.rows, r.k_in, r.ws.data_ptr(),
+                                              r.ws.numel(), handle))
 
 
 def gemv_quantized(w: Weights, r: Rows, y: torch.Tensor, stream=None) -> torch.Tensor:
     """gemv over rows quantized before: the same values."""
     if w.k_in != r.k_in:
         raise GemvError("Len", f"the rows hold {r.k_in} codes, the weights {w.k_in}")
-    if w.codes.device != r.ws.device:
-        raise GemvError("Len", f"the rows are on {r.ws.device}, the weights on {w.codes.device}")
-    yty, ys = _value_type(y, "y"), _ptr_rows(y, r.rows, w.n_out, "y", r.ws.device)
-    with _on(y, stream) as s:
-        call("syn_i8_gemv_quantized", w.codes.data_ptr(), w.view_bytes, w.stride, w.scales.data_ptr(), w.bias_ptr, w.n_out,
-             w.k_in, r.rows, yty, y.data_ptr(), ys, r.ws.data_ptr(), r.ws.numel(), s)
+    if w.device != r.ws.get_device():
+        raise GemvError("Len", f"the rows are on {r.ws.device}, the weights on cuda:{w.device}")
+    yty, ys = _value_type(y, "y"), _ptr_rows(y, r.rows, w.n_out, "y", w.device)
+    _on_stream(y, stream, lambda handle: call("syn_i8_gemv_quantized", *w.view(), w.n_out, w.k_in, r.rows, yty, y.data_ptr(),
+                                              ys, r.ws.data_ptr(), r.ws.numel(), handle))
     return y
 
 
@@ -153,20 +162,22 @@ def logits(head: Weights, g: torch.Tensor, eps: float, x: torch.Tensor, rows: in
     y F32 [rows, vocab] = head x as gemv."""
     if not (x.is_cuda and x.dtype == torch.float32 and x.is_contiguous() and x.numel() >= rows * head.k_in):
         raise GemvError("Len", f"x must be a contiguous F32 device tensor of {rows * head.k_in} values")
-    if head.codes.device != x.device or g.device != x.device or g.dtype != torch.float32 or g.numel() != head.k_in:
+    if head.device != x.get_device() or g.device != x.device or g.dtype != torch.float32 or g.numel() != head.k_in:
         raise GemvError("Len", f"g must hold {head.k_in} F32 values beside x and the head")
     if head.bias is not None:
         raise GemvError("Activations", "a head has no bias")
-    with _on(x, stream) as s:
-        if y is None:
-            y = torch.empty(rows, head.n_out, dtype=torch.float32, device=x.device)
-        elif not (y.device == x.device and y.dtype == torch.float32 and y.is_contiguous() and y.numel() >= rows * head.n_out):
-            raise GemvError("Len", f"y must be a contiguous F32 device tensor of {rows * head.n_out} values")
+    if y is not None and not (y.device == x.device and y.dtype == torch.float32 and y.is_contiguous()
+                              and y.numel() >= rows * head.n_out):
+        raise GemvError("Len", f"y must be a contiguous F32 device tensor of {rows * head.n_out} values")
+
+    def launch(handle):
+        out = torch.empty(rows, head.n_out, dtype=torch.float32, device=x.device) if y is None else y
         need = _need("syn_i8_logits_workspace_bytes", head.n_out, head.k_in, rows)
         ws = torch.empty(max(need, 256), dtype=torch.uint8, device=x.device)
-        call("syn_i8_logits", head.codes.data_ptr(), head.view_bytes, head.stride, head.scales.data_ptr(), head.n_out,
-             head.k_in, g.data_ptr(), C.c_float(eps), x.data_ptr(), rows, y.data_ptr(), ws.data_ptr(), ws.numel(), s)
-    return y
+        call("syn_i8_logits", *head.view()[:4], head.n_out, head.k_in, g.data_ptr(), C.c_float(eps), x.data_ptr(), rows,
+             out.data_ptr(), ws.data_ptr(), ws.numel(), handle)
+        return out
+    return _on_stream(x, stream, launch)
 
 
 __all__ = ["Weights", "Rows", "SynError", "GemvError", "quantize_rows", "quantize_weights", "workspace_bytes", "gemv",

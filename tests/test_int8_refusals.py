@@ -24,7 +24,7 @@ def message():
 
 
 def gemv(name="syn_i8_gemv", **o):
-    d = dict(w=A, w_bytes=1 << 30, w_stride=256, scales=A, bias=0, n=8, k=256, xtype=F32, x=A, xs=256, rows=3, ytype=F32,
+    d = dict(w=A, w_bytes=1 << 30, w_stride=256, scales=A, bias=0, n=8, k=256, xtype=F32, x=A, xs=256, rows=40, ytype=F32,
              y=A, ys=8, ws=A, ws_bytes=1 << 20)
     assert set(o) <= set(d)
     return rc(name, *{**d, **o}.values(), None)
@@ -63,7 +63,10 @@ def test_nothing_to_do_is_no_error():
 
 def test_workspace_queries():
     out = C.c_uint64()
-    assert rc("syn_i8_gemv_workspace_bytes", 4096, 2011, 5, 0, C.byref(out)) == 0 and out.value >= 5 * 2048 + 20
+    assert rc("syn_i8_gemv_workspace_bytes", 4096, 2011, 50, 0, C.byref(out)) == 0 and out.value >= 50 * 2048 + 200
+    assert rc("syn_i8_gemv_quantized_workspace_bytes", 4096, 2011, 1, C.byref(out)) == 0 and out.value >= 2048 + 4
+    assert rc("syn_i8_gemv_workspace_bytes", 4096, 2011, 1, 0, C.byref(out)) == 0 and out.value == 0
+    assert rc("syn_i8_gemv_quantized_workspace_bytes", 4096, 131073, 1, C.byref(out)) == UNSUPPORTED
     assert rc("syn_i8_gemv_workspace_bytes", 4096, 0, 5, 0, C.byref(out)) == UNSUPPORTED
     assert rc("syn_i8_gemv_workspace_bytes", 4096, 2011, 5, 0, None) == INVALID
     assert rc("syn_i8_gemv_workspace_bytes", 1 << 23, 64, 5, 1, C.byref(out)) == UNSUPPORTED
