@@ -64,17 +64,21 @@ SYN_DEV void i8_load8(const uint8_t* xr, int i, int k, float (&v)[8]) {
                 v[j] = TY == T_F16 ? f16_to_f32(b) : u2f(b << 16);
             }
         }
-    } else {
+    } else if (i < k) {  // (loads at places that are there, all in flight: a branch around each would wait for the one before)
+        uint32_t h[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            v[j] = 0.0f;
-            if (i + j < k) {
-                if constexpr (TY == T_F32)
-                    v[j] = ((const float*)xr)[i + j];
-                else
-                    v[j] = TY == T_F16 ? f16_to_f32(((const uint16_t*)xr)[i + j]) : u2f((uint32_t)((const uint16_t*)xr)[i + j] << 16);
-            }
+            const int in = i + j < k ? i + j : k - 1;
+            h[j] = TY == T_F32 ? ((const uint32_t*)xr)[in] : ((const uint16_t*)xr)[in];
         }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float f = TY == T_F32 ? u2f(h[j]) : TY == T_F16 ? f16_to_f32(h[j]) : u2f(h[j] << 16);
+            v[j] = i + j < k ? f : 0.0f;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
     }
 }
 // BF16 by round to nearest even, a NaN kept one.
@@ -157,9 +161,9 @@ SYN_DEV void i8_tile_of(int id, int tiles_w, int tiles_t, int& tw, int& tt) {
 
 void launch_i8_quantize(int xtype, const void* x, uint64_t ldx, int rows, int k, int8_t* codes, uint64_t ldc,
                         float* scales, hipStream_t stream);
-// int8_few.hip: up to 32 tokens, weights straight to registers
+// int8_few.hip: up to 16 tokens, weights straight to registers
 bool i8_few_fits(int T);
-bool i8_few_fused(int rows_w, int k, int T, int gated);  // the kernel quantizes the rows itself
+bool i8_few_fused(int k, int T);  // the kernel quantizes the rows itself
 void launch_i8_few(const I8Args& a, hipStream_t stream);
 // int8_gemm.hip: tiles through LDS, K in one part or several
 struct I8Pick {
@@ -170,7 +174,7 @@ bool i8_gemm_reaches(int tile, const I8Args& a);
 void launch_i8_gemm(int tile, const I8Args& a, hipStream_t stream);
 // int8.hip
 int i8_splits(int rows_w, int k, int T, int gated);
-bool i8_fused(int rows_w, int k, int T, int gated);
+bool i8_fused(int k, int T);
 void launch_i8_gemv(const I8Args& a, hipStream_t stream);
 
 }  // namespace syn

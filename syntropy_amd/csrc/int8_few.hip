@@ -1,162 +1,174 @@
-// The int8 product at few tokens (one to 32): bound by reading the weights once from HBM.
+// The int8 product at few tokens (one to 16): bound by reading the weights once from HBM.
 //
-// v_mfma_i32_16x16x64_i8 takes 16 weight rows against 16 tokens, 64 values a step.  A lane loads its operand's
-// 16 codes straight from the weight row to registers (four lanes a row: 64 bytes of each of 16 rows an
-// instruction), since no other wavefront reads them.  The wavefronts of a workgroup share 16 RT rows and take
-// turns at K, U steps at a time, so that a small matrix still fills the chip; their sums, whole numbers, meet
-// in LDS.  Lanes of tokens that are not there load nothing.
+// v_mfma_i32_16x16x64_i8 multiplies 16 rows by 16 columns over 64 values, four lanes a row of 16 codes each.
+// Its rows are taken as 8 weight rows x the two halves of a 128-byte line and its columns as 8 tokens x the
+// same halves: where a row's half is a column's, the product is one that is wanted (the other half of the
+// matrix cores' work, which cost nothing here, is not looked at).  So a lane loads 16 codes of a weight row
+// straight to the registers that the instruction reads, and an instruction loads whole 128-byte lines of 8
+// rows: 14336 x 4096 read that way takes 12.2 us, 64 bytes of each of 16 rows 15.8, a row 11.9.  No other
+// wavefront reads those codes, so LDS would only be a detour.
+// The eight wavefronts of a workgroup share 8 RT rows and take turns at K, U lines at a time, so that a small
+// matrix still fills the chip, two turns in flight; their sums, whole numbers, meet in LDS.  A wavefront keeps to
+// few registers, so that most matrices are asked for whole at once.  Lanes of tokens that are not there load
+// nothing.
 //
-// FUSED: one launch.  Each workgroup quantizes the rows itself into LDS while its first weights fly, which
-// costs the chip little at one or a few short rows and saves a launch; at more the rows are quantized once,
-// before.
+// The tokens' codes of a turn are loaded with its weights: loads return in order, so that codes asked for when
+// they are needed would wait for the next turn's weights too.
+//
+// FUSED: one row in one launch.  Each workgroup quantizes it into LDS while its first weights fly, a launch
+// less.
 #include "int8.hpp"
 #include "kernels.hpp"
 
 namespace syn {
 
-constexpr int FEW_MAX_T = 32;
-constexpr int FEW_WAVES = 8;
-constexpr int FEW_FUSED_CODES = 49152;  // bytes of LDS for the rows' codes
+constexpr int FEW_MAX_T = 16;
 
-template <int RT, int TT, int U, int FUSED, int GATED>
-__global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_few(I8Args g) {
+template <int RT, int TG, int U, int NW, int FUSED, int GATED>
+__global__ __launch_bounds__(64 * NW, TG > 1 || U * RT > 4 ? 4 : 6) void k_i8_few(I8Args g) {
     static_assert(!GATED || RT == 2, "a gate tile and an up tile");
-    static_assert(!FUSED || TT == 1, "fused for up to 16 tokens");
+    static_assert(RT * TG <= 4, "the outputs of one wavefront");
+    static_assert(!FUSED || TG == 1, "one row");
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c = lane & 15, q = lane >> 4;
-    const int kp = (int)i8_padded(g.k), steps = kp / 64, last = (g.k - 1) & ~15;
-    const int t0 = (int)blockIdx.y * 16 * TT;
-    const int nt = g.T - t0 < 16 * TT ? g.T - t0 : 16 * TT;
-    const int64_t n0 = (int64_t)blockIdx.x * 16 * (GATED ? 1 : RT);
+    const int c = lane & 7;                                        // weight row, and token, of 8
+    const int piece = 16 * (4 * ((lane >> 3) & 1) + (lane >> 4));  // of a line
+    const int kp = (int)i8_padded(g.k), lines = kp / I8_LINE, last = (g.k - 1) & ~15;
+    const int t0 = (int)blockIdx.y * 8 * TG;
+    const int nt = g.T - t0 < 8 * TG ? g.T - t0 : 8 * TG;
+    const int64_t n0 = (int64_t)blockIdx.x * 8 * (GATED ? 1 : RT);
     const int8_t* wr[RT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-        int64_t n = n0 + (GATED ? 0 : 16 * i) + c;
+        int64_t n = n0 + (GATED ? 0 : 8 * i) + c;
         n = n < g.n_out ? n : g.n_out - 1;
         wr[i] = g.w + (uint64_t)(n + (GATED && i ? g.n_out : 0)) * g.ldw;
     }
-    // (a row's pieces past its end: its last one again, against zeros)
-    auto load = [&](int s, i8x16 (&to)[U][RT]) {
+    const int8_t* xr = FUSED ? nullptr : g.xq + (uint64_t)(t0 + c) * kp + piece;
+    constexpr int TURN = U * NW;  // lines
+    struct Turn {
+        i8x16 w[U][RT], x[FUSED ? 1 : U][TG];
+    };
+    auto load = [&](int s, Turn& to) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            int at = 64 * (s + u) + 16 * q;
-            at = at < last ? at : last;
+            if (s + u >= lines) break;  // uniform
+            int at = I8_LINE * (s + u) + piece;
+            at = at < last ? at : last;  // a row's pieces past its end: its last one again, against zeros
 #pragma unroll
             for (int i = 0; i < RT; ++i)
-                to[u][i] = __builtin_nontemporal_load(reinterpret_cast<const i8x16*>(wr[i] + at));
+                to.w[u][i] = __builtin_nontemporal_load(reinterpret_cast<const i8x16*>(wr[i] + at));
+            if constexpr (!FUSED) {
+#pragma unroll
+                for (int j = 0; j < TG; ++j) {
+                    to.x[u][j] = i8x16{0, 0, 0, 0};
+                    if (8 * j + c < nt)
+                        to.x[u][j] = *reinterpret_cast<const i8x16*>(xr + (uint64_t)(8 * j) * kp + I8_LINE * (s + u));
+                }
+            }
         }
     };
-    i8x16 cur[U][RT];
+    Turn cur, nxt;
     int s = wave * U;
-    if (s < steps) load(s, cur);
+    load(s, cur);
+    load(s + TURN, nxt);
 
-    const int cs = kp + 16;  // FUSED: the codes' rows in LDS, neighbouring tokens on other banks
-    const float* xs = g.xs + t0;
+    float* row_scale = reinterpret_cast<float*>(lds);  // FUSED: the row's scale, the wavefronts' maxima, its codes
+    uint8_t* codes = lds + 128;
     if constexpr (FUSED) {
-        float* fs = reinterpret_cast<float*>(lds);              // [16]
-        uint32_t* top = reinterpret_cast<uint32_t*>(lds + 64);  // [16][FEW_WAVES]
-        const int es = g.xtype == T_F32 ? 4 : 2;
-        auto rows = [&](auto type) {
+        uint32_t* top = reinterpret_cast<uint32_t*>(lds + 16);
+        auto row = [&](auto type) {
             constexpr int TY = decltype(type)::value;
-            for (int t = 0; t < nt; ++t) {
-                const uint8_t* xr = (const uint8_t*)g.x + (uint64_t)(t0 + t) * g.ldx * es;
-                uint32_t m = 0;
-                float v[8];
-                for (int i = threadIdx.x * 8; i < g.k; i += 64 * FEW_WAVES * 8) {
-                    i8_load8<TY>(xr, i, g.k, v);
-                    m = i8_max8(v, m);
-                }
-                m = group_max_u32<64>(m);
-                if (lane == 0) top[t * FEW_WAVES + wave] = m;
-            }
-            __syncthreads();
-            for (int t = 0; t < nt; ++t) {
-                const uint8_t* xr = (const uint8_t*)g.x + (uint64_t)(t0 + t) * g.ldx * es;
-                uint32_t m = 0;
+            const uint8_t* x = (const uint8_t*)g.x + (uint64_t)t0 * g.ldx * (TY == T_F32 ? 4 : 2);
+            float v[2][8];  // i8_few_fused: a row is at most two pieces of 8 a thread
+            uint32_t m = 0;
 #pragma unroll
-                for (int w = 0; w < FEW_WAVES; ++w) m = m > top[t * FEW_WAVES + w] ? m : top[t * FEW_WAVES + w];
-                const I8Scale sc = i8_scale(m);
-                if (threadIdx.x == 0) fs[t] = sc.s;
-                float v[8];
-                for (int i = threadIdx.x * 8; i < kp; i += 64 * FEW_WAVES * 8) {
-                    i8_load8<TY>(xr, i, g.k, v);
-                    *reinterpret_cast<uint2*>(lds + 1024 + t * cs + i) = i8_codes8(v, sc.inv);
-                }
+            for (int p = 0; p < 2; ++p) i8_load8<TY>(x, 8 * ((int)threadIdx.x + 64 * NW * p), g.k, v[p]);
+#pragma unroll
+            for (int p = 0; p < 2; ++p) m = i8_max8(v[p], m);
+            m = group_max_u32<64>(m);
+            if (lane == 0) top[wave] = m;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < NW; ++w) m = m > top[w] ? m : top[w];
+            const I8Scale sc = i8_scale(m);
+            if (threadIdx.x == 0) *row_scale = sc.s;
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const int i = 8 * ((int)threadIdx.x + 64 * NW * p);
+                if (i < kp) *reinterpret_cast<uint2*>(codes + i) = i8_codes8(v[p], sc.inv);
             }
         };
         if (g.xtype == T_F32)
-            rows(std::integral_constant<int, T_F32>{});
+            row(std::integral_constant<int, T_F32>{});
         else if (g.xtype == T_F16)
-            rows(std::integral_constant<int, T_F16>{});
+            row(std::integral_constant<int, T_F16>{});
         else
-            rows(std::integral_constant<int, T_BF16>{});
+            row(std::integral_constant<int, T_BF16>{});
         __syncthreads();
-        xs = fs;
     }
 
-    i8x16 acc[RT][TT] = {};
-    const int8_t* xr[TT];
+    i8x16 acc[RT][TG] = {};
+    auto product = [&](int s, const Turn& o) {
 #pragma unroll
-    for (int j = 0; j < TT; ++j) xr[j] = g.xq + (uint64_t)(t0 + 16 * j + c) * kp + 16 * q;
-    while (s < steps) {
-        const int next = s + U * FEW_WAVES;
-        i8x16 nxt[U][RT];
-        i8x16 b[U][TT];
+        for (int u = 0; u < U; ++u) {
+            if (s + u >= lines) break;  // uniform
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int j = 0; j < TT; ++j) {
-                b[u][j] = i8x16{0, 0, 0, 0};
-                if (16 * j + c < nt && s + u < steps) {
-                    if constexpr (FUSED)
-                        b[u][j] = *reinterpret_cast<const i8x16*>(lds + 1024 + c * cs + 64 * (s + u) + 16 * q);
-                    else
-                        b[u][j] = *reinterpret_cast<const i8x16*>(xr[j] + 64 * (s + u));
+            for (int j = 0; j < TG; ++j) {
+                i8x16 b;
+                if constexpr (FUSED) {
+                    b = i8x16{0, 0, 0, 0};
+                    if (c == 0) b = *reinterpret_cast<const i8x16*>(codes + I8_LINE * (s + u) + piece);
+                } else {
+                    b = o.x[u][j];
                 }
+#pragma unroll
+                for (int i = 0; i < RT; ++i)
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(o.w[u][i], b, acc[i][j], 0, 0, 0);
             }
-        if (next < steps) load(next, nxt);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int i = 0; i < RT; ++i)
-#pragma unroll
-                for (int j = 0; j < TT; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(cur[u][i], b[u][j], acc[i][j], 0, 0, 0);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int i = 0; i < RT; ++i) cur[u][i] = nxt[u][i];
-        s = next;
+        }
+    };
+    while (s < lines) {  // uniform
+        product(s, cur);
+        load(s + 2 * TURN, cur);
+        s += TURN;
+        product(s, nxt);
+        load(s + 2 * TURN, nxt);
+        s += TURN;
     }
 
-    // the wavefronts' sums
-    i8x16* red = reinterpret_cast<i8x16*>(lds + (FUSED ? 1024 + ((nt * cs + 15) & ~15) : 0));  // [wave][RT TT][64]
+    // The wavefronts' sums.  Lane l holds columns l & 15, rows 4 (l >> 4) .. + 3 of 16: those of the first half
+    // by the first (lanes 0..7 and 16..23) and of the second by the second (40..47 and 56..63).
+    i8x16* red = reinterpret_cast<i8x16*>(lds + (FUSED ? 128 + kp : 0));  // [wave][RT][TG][64]
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int j = 0; j < TT; ++j) red[(wave * RT * TT + i * TT + j) * 64 + lane] = acc[i][j];
+        for (int j = 0; j < TG; ++j) red[((wave * RT + i) * TG + j) * 64 + lane] = acc[i][j];
     __syncthreads();
-    constexpr int TILES = GATED ? TT : RT * TT;
-    if (wave >= TILES) return;
-    const int j = GATED ? wave : wave % TT, i = GATED ? 0 : wave / TT;
+    if (wave != 0) return;
+    // lane: tile l / 16 of the (RT or, gated, 1) x TG, rows 4 (l / 8 & 1) .. + 3, token l & 7
+    const int tile = lane >> 4, half = (lane >> 3) & 1;
+    if (tile >= (GATED ? 1 : RT) * TG) return;
+    const int i = GATED ? 0 : tile / TG, j = GATED ? tile : tile % TG, t = 8 * j + c;
     i8x16 sum[GATED ? 2 : 1] = {};
 #pragma unroll
     for (int m = 0; m < (GATED ? 2 : 1); ++m)
-#pragma unroll
-        for (int w = 0; w < FEW_WAVES; ++w) sum[m] += red[(w * RT * TT + (i + m) * TT + j) * 64 + lane];
-    const int t = 16 * j + c;
+#pragma unroll 4
+        for (int w = 0; w < NW; ++w) {
+            const i8x16* r = red + ((w * RT + i + m) * TG + j) * 64;
+            sum[m] += r[16 * half + c] + r[16 * half + 40 + c];
+        }
     if (t >= nt) return;
-    const float sx = xs[t];
+    const float sx = FUSED ? *row_scale : g.xs[t0 + t];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const int64_t n = n0 + 16 * i + 4 * q + e;
+        const int64_t n = n0 + 8 * i + 4 * half + e;
         if (n >= g.n_out) break;
         float v = i8_value(sum[0][e], sx, g.ws[n]);
         if (g.bias) v = v + g.bias[n];
         if constexpr (GATED) {
-            float u = i8_value(sum[1][e], sx, g.ws[g.n_out + n]);
+            float u = i8_value(sum[GATED ? 1 : 0][e], sx, g.ws[g.n_out + n]);
             if (g.bias) u = u + g.bias[g.n_out + n];
             v = i8_silu(v) * u;
         }
@@ -166,31 +178,52 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_few(I8Args g) {
 
 bool i8_few_fits(int T) { return T <= FEW_MAX_T; }
 
-bool i8_few_fused(int rows_w, int k, int T, int gated) {
-    (void)rows_w;
-    (void)gated;
-    return T <= 16 && (uint64_t)T * k <= 16384 && (uint64_t)T * (i8_padded(k) + 16) <= FEW_FUSED_CODES;
-}
+// One row of at most two pieces of 8 values a thread of the largest workgroup (4096 x 4096: 6.7 against 8.2 us
+// with the row quantized in a launch before).
+bool i8_few_fused(int k, int T) { return T == 1 && k <= 16384; }
 
-template <int RT, int TT, int U, int FUSED, int GATED>
+template <int RT, int TG, int U, int NW, int FUSED, int GATED>
 static void launch_few(const I8Args& a, hipStream_t stream) {
-    const int tiles = a.T < 16 * TT ? a.T : 16 * TT;
-    const int lds = FEW_WAVES * RT * TT * 1024 + (FUSED ? 1024 + (tiles * ((int)i8_padded(a.k) + 16) + 15) / 16 * 16 : 0);
-    const int per = 16 * (GATED ? 1 : RT);
-    static const hipError_t most = hipFuncSetAttribute((const void*)k_i8_few<RT, TT, U, FUSED, GATED>,
+    const int lds = NW * RT * TG * 1024 + (FUSED ? 128 + (int)i8_padded(a.k) : 0);
+    const int per = 8 * (GATED ? 1 : RT);
+    static const hipError_t most = hipFuncSetAttribute((const void*)k_i8_few<RT, TG, U, NW, FUSED, GATED>,
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     (void)most;  // a launch that the runtime refuses is reported by the caller
-    hipLaunchKernelGGL((k_i8_few<RT, TT, U, FUSED, GATED>), dim3((a.n_out + per - 1) / per, (a.T + 16 * TT - 1) / (16 * TT)),
-                       dim3(64 * FEW_WAVES), lds, stream, a);
+    hipLaunchKernelGGL((k_i8_few<RT, TG, U, NW, FUSED, GATED>), dim3((a.n_out + per - 1) / per, (a.T + 8 * TG - 1) / (8 * TG)),
+                       dim3(64 * NW), lds, stream, a);
 }
 
-void launch_i8_few(const I8Args& a, hipStream_t stream) {
-    if (a.x)
-        a.gated ? launch_few<2, 1, 4, 1, 1>(a, stream) : launch_few<1, 1, 8, 1, 0>(a, stream);
-    else if (a.T <= 16)
-        a.gated ? launch_few<2, 1, 4, 0, 1>(a, stream) : launch_few<1, 1, 8, 0, 0>(a, stream);
+// Rows of weights a workgroup: 8 for one or two tokens (14336 x 4096 at 1 token 12.5 us against 13.3 for 16, at 2
+// 14.4 against 15.0), else 16, which share the tokens' codes (at 8 tokens 17.7 against 19.0).  Two lines a
+// turn: with four the registers leave too few wavefronts (1 token, 8 rows, 15.3).  Long fused rows on 16
+// wavefronts, for the quantization's sake.
+static void launch_some(const I8Args& a, hipStream_t stream) {
+    const bool wide = a.x && a.k > 8192;
+    if (a.T > 8)
+        a.gated ? launch_few<2, 2, 2, 8, 0, 1>(a, stream) : launch_few<2, 2, 2, 8, 0, 0>(a, stream);
+    else if (a.gated && a.x)
+        wide ? launch_few<2, 1, 2, 16, 1, 1>(a, stream) : launch_few<2, 1, 2, 8, 1, 1>(a, stream);
+    else if (a.gated)
+        launch_few<2, 1, 2, 8, 0, 1>(a, stream);
+    else if (a.x)
+        wide ? launch_few<1, 1, 2, 16, 1, 0>(a, stream) : launch_few<1, 1, 2, 8, 1, 0>(a, stream);
+    else if (a.T <= 2)
+        launch_few<1, 1, 2, 8, 0, 0>(a, stream);
     else
-        a.gated ? launch_few<2, 2, 4, 0, 1>(a, stream) : launch_few<1, 2, 4, 0, 0>(a, stream);
+        launch_few<2, 1, 2, 8, 0, 0>(a, stream);
+}
+
+// (any number of tokens, for weight rows that a tile's offsets do not reach: as many a launch as a grid holds)
+void launch_i8_few(const I8Args& a, hipStream_t stream) {
+    constexpr int MOST = 1 << 19;
+    for (int t = 0; t < a.T; t += MOST) {
+        I8Args g = a;
+        g.T = a.T - t < MOST ? a.T - t : MOST;
+        g.xq = a.xq + (uint64_t)t * i8_padded(a.k);
+        g.xs = a.xs + t;
+        g.y = (uint8_t*)a.y + (uint64_t)t * a.ldy * (a.ytype == T_F32 ? 4 : 2);
+        launch_some(g, stream);
+    }
 }
 
 }  // namespace syn

@@ -245,7 +245,7 @@ def test_codes_held_on_odd_bytes_are_laid_out_once(I, rows):
     odd = make(n, k, 2)[0].contiguous()
     for codes in (odd, make(n, k + 3, 2)[0][:, 3:], odd.t().contiguous().t()):
         W = I.Weights(codes, torch.ones(n, device="cuda"))
-        assert W.stride % 16 == 0 and W.codes.data_ptr() % 16 == 0 and (W.codes == codes).all()
+        assert W.codes.stride(0) % 16 == 0 and W.codes.data_ptr() % 16 == 0 and (W.codes == codes).all()
     check(I, (odd, torch.ones(n, device="cuda"), None), rows_of(rows, k, torch.float32, 1).cuda(), rows, "odd codes")
 
 
