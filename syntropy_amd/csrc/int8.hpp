@@ -11,10 +11,10 @@ namespace syn {
 typedef int i8x16 __attribute__((ext_vector_type(4)));  // sixteen int8 codes
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
-// The tokens' codes are held in rows of whole 128-byte lines, zeros behind the last value, so that what
-// a kernel reads of a weight row past its end is multiplied by zero.
+// The tokens' codes are held in rows of whole pairs of 128-byte lines, zeros behind the last value, so that
+// what a kernel reads of a weight row past its end is multiplied by zero.
 constexpr int I8_LINE = 128;
-SYN_HD inline uint64_t i8_padded(uint64_t k) { return align_up(k, I8_LINE); }
+SYN_HD inline uint64_t i8_padded(uint64_t k) { return align_up(k, 2 * I8_LINE); }
 // |sum| <= 128 * 127 * k stays below 2^31.
 constexpr uint32_t I8_MAX_K = 131072;
 
