@@ -240,7 +240,7 @@ int syn_i8_logits(const int8_t* head, uint64_t head_bytes, uint64_t head_stride,
 
 /* ---- Log probabilities of given tokens -----------------------------------------------------------
  * For each row of logits x [rows, vocab] (F32, F16 or BF16, rows x_stride values apart; -infinity hides
- * a token), with z = x scale (scale: the inverse of a sampling temperature, finite and above 0):
+ * a token), with z = x scale, a real number (scale: the inverse of a sampling temperature, finite and above 0):
  *   logprob [rows] F32: log softmax(z) at tokens[row];
  *   rank [rows] I32: how many of the row's logits are greater than the token's (0: none is);
  *   entropy [rows] F32: of softmax(z), in nats;

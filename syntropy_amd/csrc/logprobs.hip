@@ -1,5 +1,5 @@
 // Log probabilities of given tokens, entropy and most probable tokens of each row of logits x [rows][vocab]:
-//   z = x scale, m = max z, s = sum exp(z - m), e = sum exp(z - m) (z - m);  log p_i = (z_i - m) - log s;
+//   m = max x, d_i = (x_i - m) scale, s = sum exp d_i, e = sum exp(d_i) d_i;  log p_i = d_i - log s;
 //   H = log s - e / s;  rank = the number of logits above the token's;
 //   the `top` first tokens by (logit descending, index ascending).
 // A row with nothing visible (all -infinity) has log probabilities of -infinity and the entropy 0; a NaN or
@@ -16,7 +16,7 @@
 // the greater ones: a few dozen, in less time and code than a sort across lanes.  Where equal values fill the
 // LDS, the `top` greatest of it stay and raise the bound.
 //
-// Few rows: a row is split over workgroups, whose parts a second launch joins.
+// Few long rows are split over workgroups, whose parts a second launch joins.
 #include <type_traits>
 
 #include "common.hpp"
@@ -26,11 +26,10 @@ namespace syn {
 
 namespace {
 
-constexpr int LP_WAVES = 4;
 constexpr int LP_VALUES = 16;              // a lane's values a step
 constexpr int LP_STEP = 64 * LP_VALUES;
-constexpr int LP_GROUPS = 32;
-constexpr float LOG2E = 1.44269504088896340736f;
+constexpr int lp_groups(int waves) { return waves > 4 ? 16 : 32; }
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 // A whole number that orders as the value does (-0 as +0, every NaN above +infinity), and the value again.
 SYN_DEV uint32_t lp_order(float v) {
@@ -60,18 +59,34 @@ SYN_DEV uint32_t reached_by(const uint32_t (&v)[4], int n) {
 }
 
 constexpr int LP_ROOM = 512;
-// A workgroup's greatest keys so far, in LDS.
+// The greatest keys so far of a workgroup of W wavefronts, in LDS.
+template <int W>
 struct Greatest {
     uint64_t keys[LP_ROOM];                // in any order
     uint64_t sorted[LOGPROB_MAX_TOP];      // of sort()
-    uint32_t most[64 * LP_WAVES];          // the lanes' greatest
+    uint32_t most[64 * W];                 // the lanes' greatest
     int count;                             // of keys, and of those that found no room
-    int more[2][LP_WAVES];
+    int more[2][W];
 
+    // (after a barrier behind the lanes' `most`) a number that at least `top` keys' values reach: 256 values, of
+    // W / 4 lanes each
+    SYN_DEV uint32_t bound(int top) const {
+        uint32_t of[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            of[j] = 0;
+#pragma unroll
+            for (int w = j; w < W; w += 4) {
+                const uint32_t v = most[64 * w + (threadIdx.x & 63)];
+                of[j] = v > of[j] ? v : of[j];
+            }
+        }
+        return reached_by(of, top);
+    }
     // (every thread; a barrier before and after) the `top` greatest in order; returns how many there are
     SYN_DEV int sort(int top) {
         const int n = count < LP_ROOM ? count : LP_ROOM;
-        for (int j = threadIdx.x; j < n; j += 64 * LP_WAVES) {
+        for (int j = threadIdx.x; j < n; j += 64 * W) {
             const uint64_t k = keys[j];
             int rank = 0;
 #pragma unroll 4
@@ -93,7 +108,7 @@ struct Greatest {
         if ((threadIdx.x & 63) == 0) more[parity][threadIdx.x >> 6] = any;
         __syncthreads();
         bool go = false;
-        for (int w = 0; w < LP_WAVES; ++w) go |= more[parity][w] != 0;
+        for (int w = 0; w < W; ++w) go |= more[parity][w] != 0;
         if (count >= LP_ROOM) {  // uniform
             sort(top);
             __syncthreads();
@@ -108,21 +123,24 @@ struct Greatest {
 };
 static_assert(LP_ROOM > LOGPROB_MAX_TOP, "room behind those that stay");
 
-// A running softmax: the greatest, the sum of exponentials, the sum of exponentials times their arguments.
+// A running softmax: the greatest value m; with t_i = (x_i - m) c, c = scale log2(e), the sum of 2^t_i and that
+// of 2^t_i t_i.  (A t below -150 has the power 0, and one of -300 stands for it in the second sum, for
+// -infinity times 0 is a NaN.)
+constexpr float LP_LEAST = -300.0f;
 struct Soft {
     float m = -__builtin_inff(), s = 0.0f, e = 0.0f;
     // to the maximum n >= m (a lane that has seen nothing but -infinity and NaN keeps its sums, 0 or NaN)
-    SYN_DEV void rebase(float n) {
-        const float d = m == -__builtin_inff() ? 0.0f : fmaxf(m - n, -200.0f);  // (from -104 on the factor is 0)
-        const float f = __builtin_amdgcn_exp2f(d * LOG2E);
-        e = f * __builtin_fmaf(d, s, e);
+    SYN_DEV void rebase(float n, float c) {
+        const float t = m == -__builtin_inff() ? 0.0f : fmaxf((m - n) * c, LP_LEAST);
+        const float f = __builtin_amdgcn_exp2f(t);
+        e = f * __builtin_fmaf(t, s, e);
         s = f * s;
         m = n;
     }
-    SYN_DEV void add(Soft o) {
+    SYN_DEV void add(Soft o, float c) {
         const float n = fmaxf(m, o.m);
-        rebase(n);
-        o.rebase(n);
+        rebase(n, c);
+        o.rebase(n, c);
         s += o.s;
         e += o.e;
     }
@@ -132,8 +150,8 @@ SYN_DEV float max_of_lanes(float v) {
     for (int d = 1; d < 64; d *= 2) v = fmaxf(v, __shfl_xor(v, d));
     return v;
 }
-SYN_DEV Soft soft_of_lanes(Soft v) {
-    v.rebase(max_of_lanes(v.m));
+SYN_DEV Soft soft_of_lanes(Soft v, float c) {
+    v.rebase(max_of_lanes(v.m), c);
     for (int d = 1; d < 64; d *= 2) {
         v.s += __shfl_xor(v.s, d);
         v.e += __shfl_xor(v.e, d);
@@ -210,29 +228,29 @@ SYN_DEV void lp_write(const LogprobArgs& g, uint64_t row, const Soft& v, uint32_
     const float ls = logf(v.s), base = v.base();
     if (lane == 0) {
         const bool known = t >= 0 && t < g.vocab;
-        g.logprob[row] = t < 0 ? 0.0f : !known ? __builtin_nanf("") : none ? -__builtin_inff() : (xt * g.scale - base) - ls;
+        g.logprob[row] = t < 0 ? 0.0f : !known ? __builtin_nanf("") : none ? -__builtin_inff() : (xt - base) * g.scale - ls;
         g.rank[row] = known ? (int)above : -1;
-        g.entropy[row] = none ? 0.0f : ls - v.e / v.s;
+        g.entropy[row] = none ? 0.0f : ls - v.e / v.s * LN2;
     }
     if (lane < g.top) {
         const uint64_t k = sorted[lane];
         g.top_ids[row * g.top + lane] = lp_index(k);
-        g.top_logprobs[row * g.top + lane] = none ? -__builtin_inff() : (lp_value((uint32_t)(k >> 32)) * g.scale - base) - ls;
+        g.top_logprobs[row * g.top + lane] = none ? -__builtin_inff() : (lp_value((uint32_t)(k >> 32)) - base) * g.scale - ls;
     }
 }
 
 }  // namespace
 
-template <int TY, int TOP>
-__global__ __launch_bounds__(64 * LP_WAVES) void k_logprobs(LogprobArgs g, int parts, int part_steps, int group_steps) {
+template <int TY, int TOP, int W>
+__global__ __launch_bounds__(64 * W) void k_logprobs(LogprobArgs g, int parts, int part_steps, int group_steps) {
     const uint64_t row = blockIdx.x / (uint32_t)parts;
     const int part = (int)(blockIdx.x % (uint32_t)parts);
     const uint8_t* x = (const uint8_t*)g.x + row * g.ldx * (TY == T_F32 ? 4 : 2);
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    __shared__ uint32_t groups[TOP ? LP_WAVES : 1][TOP ? LP_GROUPS : 1][64];
-    __shared__ typename std::conditional<TOP != 0, Greatest, int>::type best;
-    __shared__ Part sums[LP_WAVES];
+    __shared__ uint32_t groups[TOP ? W : 1][TOP ? lp_groups(W) : 1][64];
+    __shared__ typename std::conditional<TOP != 0, Greatest<W>, int>::type best;
+    __shared__ Part sums[W];
     const int steps = (g.vocab + LP_STEP - 1) / LP_STEP;
     const int last = (part + 1) * part_steps < steps ? (part + 1) * part_steps : steps;
     const int step0 = part * part_steps + wave;
@@ -245,24 +263,25 @@ __global__ __launch_bounds__(64 * LP_WAVES) void k_logprobs(LogprobArgs g, int p
     const bool known = t >= 0 && t < g.vocab;
     const float xt = known ? lp_load<TY>(x, t) : __builtin_nanf("");  // (nothing is above a NaN)
 
+    const float c = g.scale * LOG2E;
     Soft v;
     uint32_t above = 0;
     float most = -__builtin_inff(), group = most;  // the lane's greatest value, and that of its group
     int in_group = 0, n_groups = 0;
     while (step < last) {  // uniform
-        step += LP_WAVES;
+        step += W;
         if (step < last) nxt.load(x, step * LP_STEP, g.vocab);
         float mx = cur.at(0);
 #pragma unroll
         for (int i = 1; i < LP_VALUES; ++i) mx = fmaxf(mx, cur.at(i));
-        const float n = fmaxf(v.m, mx * g.scale);
-        if (__builtin_amdgcn_ballot_w64(n > v.m) != 0) v.rebase(n);
+        const float n = fmaxf(v.m, mx);
+        if (__builtin_amdgcn_ballot_w64(n > v.m) != 0) v.rebase(n, c);
         const float base = v.base();
 #pragma unroll
         for (int i = 0; i < LP_VALUES; ++i) {
-            const float xi = cur.at(i), d = xi * g.scale - base, p = __builtin_amdgcn_exp2f(d * LOG2E);
+            const float xi = cur.at(i), t2 = (xi - base) * c, p = __builtin_amdgcn_exp2f(t2);
             v.s += p;
-            v.e = __builtin_fmaf(p, fmaxf(d, -200.0f), v.e);  // (p is 0 from -104 on: nothing, not 0 times -infinity)
+            v.e = __builtin_fmaf(p, fmaxf(t2, LP_LEAST), v.e);
             above += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(xi > xt));
         }
         if constexpr (TOP) {
@@ -281,10 +300,7 @@ __global__ __launch_bounds__(64 * LP_WAVES) void k_logprobs(LogprobArgs g, int p
         best.most[threadIdx.x] = lp_order(most);
         if (threadIdx.x == 0) best.count = 0;
         __syncthreads();
-        uint32_t of[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) of[j] = best.most[lane + 64 * j];
-        const uint32_t b = reached_by(of, g.top);
+        const uint32_t b = best.bound(g.top);
         uint64_t bound = b ? ((uint64_t)b << 32) - 1 : 0;  // all of that value are above it
         uint32_t mine = 0;  // the lane's groups that reach it
         for (int i = 0; i < n_groups; ++i) mine |= groups[wave][i][lane] >= b ? 1u << i : 0u;
@@ -294,7 +310,7 @@ __global__ __launch_bounds__(64 * LP_WAVES) void k_logprobs(LogprobArgs g, int p
 #pragma unroll 1
         for (int parity = 0; go; parity ^= 1) {  // uniform
             if (may == 0 && mine != 0) {         // the lane's next step
-                const int gi = __builtin_ctz(mine), st = step0 + (gi * group_steps + in) * LP_WAVES;
+                const int gi = __builtin_ctz(mine), st = step0 + (gi * group_steps + in) * W;
                 at = st * LP_STEP;
                 // (equal values: a group behind the bound's index holds nothing before it)
                 if (st < last &&
@@ -318,18 +334,18 @@ __global__ __launch_bounds__(64 * LP_WAVES) void k_logprobs(LogprobArgs g, int p
         const int n = best.sort(g.top);
         if ((int)threadIdx.x >= n && (int)threadIdx.x < g.top) best.sorted[threadIdx.x] = 0;
     }
-    v = soft_of_lanes(v);
+    v = soft_of_lanes(v, c);
     if (lane == 0) sums[wave] = Part{v.m, v.s, v.e, above};
     __syncthreads();
     if (wave != 0) return;
 #pragma unroll
-    for (int w = 1; w < LP_WAVES; ++w) {
+    for (int w = 1; w < W; ++w) {
         const Part o = sums[w];
         Soft ov;
         ov.m = o.m;
         ov.s = o.s;
         ov.e = o.e;
-        v.add(ov);
+        v.add(ov, c);
         above += o.above;
     }
     const uint64_t* sorted = nullptr;
@@ -345,13 +361,14 @@ __global__ __launch_bounds__(64 * LP_WAVES) void k_logprobs(LogprobArgs g, int p
 
 // The parts of a row.
 template <int TY, int TOP>
-__global__ __launch_bounds__(TOP ? 64 * LP_WAVES : 64) void k_logprobs_join(LogprobArgs g, int parts) {
+__global__ __launch_bounds__(TOP ? 256 : 64) void k_logprobs_join(LogprobArgs g, int parts) {
     const uint64_t row = blockIdx.x;
     const int lane = threadIdx.x & 63;
-    __shared__ typename std::conditional<TOP != 0, Greatest, int>::type best;
+    __shared__ typename std::conditional<TOP != 0, Greatest<4>, int>::type best;
     const Part* from = (const Part*)g.ws + row * parts;
     const int64_t t = lp_token(g, row);
     const float xt = t >= 0 && t < g.vocab ? lp_load<TY>((const uint8_t*)g.x + row * g.ldx * (TY == T_F32 ? 4 : 2), t) : 0.0f;
+    const float c = g.scale * LOG2E;
     Soft v;
     uint32_t above = 0;
     if (lane < parts) {  // (at most 64)
@@ -366,21 +383,18 @@ __global__ __launch_bounds__(TOP ? 64 * LP_WAVES : 64) void k_logprobs_join(Logp
         const uint64_t* keys = (const uint64_t*)(g.ws + (uint64_t)g.rows * parts * sizeof(Part)) + row * parts * g.top;
         const int n = parts * g.top;
         uint64_t k = (int)threadIdx.x < n ? keys[threadIdx.x] : 0, mx = k;
-        for (int i = threadIdx.x + 64 * LP_WAVES; i < n; i += 64 * LP_WAVES) mx = keys[i] > mx ? keys[i] : mx;
+        for (int i = threadIdx.x + 256; i < n; i += 256) mx = keys[i] > mx ? keys[i] : mx;
         best.most[threadIdx.x] = (uint32_t)(mx >> 32);
         if (threadIdx.x == 0) best.count = 0;
         __syncthreads();
-        uint32_t of[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) of[j] = best.most[lane + 64 * j];
-        const uint32_t b = reached_by(of, g.top);
+        const uint32_t b = best.bound(g.top);
         uint64_t bound = b ? ((uint64_t)b << 32) - 1 : 0;
         bool go = true;
         int i = threadIdx.x;
 #pragma unroll 1
         for (int parity = 0; go; parity ^= 1) {  // uniform
             if (i < n && !(k > bound && best.put(k))) {
-                i += 64 * LP_WAVES;
+                i += 256;
                 k = i < n ? keys[i] : 0;
             }
             go = best.round(i < n, parity, g.top, bound);
@@ -390,42 +404,56 @@ __global__ __launch_bounds__(TOP ? 64 * LP_WAVES : 64) void k_logprobs_join(Logp
         if (threadIdx.x >= 64) return;
         sorted = best.sorted;
     }
-    v = soft_of_lanes(v);
+    v = soft_of_lanes(v, c);
     for (int d = 1; d < 64; d *= 2) above += __shfl_xor(above, d);
     lp_write(g, row, v, above, xt, t, sorted);
 }
 
-// Parts a row: about 1024 workgroups keep reads in flight on every CU (256 rows of 128256 BF16, 20 greatest:
-// 36 us in parts for 256, 28 for 1024, 33 for 2048), each of at least a step a wavefront.
-static int lp_parts(int rows, int vocab) {
+// How a call runs: wavefronts a workgroup, parts of a row.  A workgroup of 16 wavefronts takes a whole row where
+// the rows are few and not long, or nearly fill the chip: one launch (64 rows of 32064, 64 greatest, 14.9 us
+// against 17.2 in parts; 256 rows of 128256 BF16 24.6 against 28.6; 24 rows of 128256 22.1 against 16.8).  Other
+// few and long rows are in parts, so that about 1024 workgroups of four keep reads in flight.
+struct LpPlan {
+    int waves, parts, part_steps, group_steps;
+};
+static LpPlan lp_plan(int rows, int vocab) {
     const int steps = (vocab + LP_STEP - 1) / LP_STEP;
-    const int most = (steps + LP_WAVES - 1) / LP_WAVES;
-    int p = 1024 / rows;
-    p = p < most ? p : most;
-    p = p < 64 ? p : 64;
-    return p < 1 ? 1 : p;
+    LpPlan p{4, 1, 0, 0};
+    if (rows <= 256 && steps > 4 && (steps <= 64 || rows > 160)) {
+        p.waves = 16;
+    } else if (steps > 32) {
+        const int most = (steps + 3) / 4 < 64 ? (steps + 3) / 4 : 64;
+        p.parts = 1024 / rows < most ? 1024 / rows : most;
+        p.parts = p.parts < 1 ? 1 : p.parts;
+    }
+    p.part_steps = (steps + p.parts - 1) / p.parts;
+    const int wave_steps = (p.part_steps + p.waves - 1) / p.waves;
+    p.group_steps = (wave_steps + lp_groups(p.waves) - 1) / lp_groups(p.waves);
+    return p;
 }
-static int lp_part_steps(int parts, int vocab) { return ((vocab + LP_STEP - 1) / LP_STEP + parts - 1) / parts; }
 
 uint64_t logprob_ws_bytes(int rows, int vocab, int top) {
     if (rows == 0) return 0;
-    const int p = lp_parts(rows, vocab);
+    const int p = lp_plan(rows, vocab).parts;
     return p > 1 ? align_up((uint64_t)rows * p * (sizeof(Part) + 8 * (uint64_t)top), 256) : 0;
 }
 
+template <int TY, int W>
+static void logprobs_of(const LogprobArgs& a, const LpPlan& p, hipStream_t stream) {
+    const dim3 grid((uint32_t)a.rows * (uint32_t)p.parts);
+    if (a.top)
+        hipLaunchKernelGGL((k_logprobs<TY, 1, W>), grid, dim3(64 * W), 0, stream, a, p.parts, p.part_steps, p.group_steps);
+    else
+        hipLaunchKernelGGL((k_logprobs<TY, 0, W>), grid, dim3(64 * W), 0, stream, a, p.parts, p.part_steps, p.group_steps);
+}
 template <int TY>
 static void logprobs_as(const LogprobArgs& a, hipStream_t stream) {
-    const int parts = lp_parts(a.rows, a.vocab), ps = lp_part_steps(parts, a.vocab);
-    const int wave_steps = (ps + LP_WAVES - 1) / LP_WAVES, gs = (wave_steps + LP_GROUPS - 1) / LP_GROUPS;
-    const dim3 grid((uint32_t)a.rows * (uint32_t)parts);
-    if (a.top)
-        hipLaunchKernelGGL((k_logprobs<TY, 1>), grid, dim3(64 * LP_WAVES), 0, stream, a, parts, ps, gs);
-    else
-        hipLaunchKernelGGL((k_logprobs<TY, 0>), grid, dim3(64 * LP_WAVES), 0, stream, a, parts, ps, gs);
-    if (parts > 1 && a.top)
-        hipLaunchKernelGGL((k_logprobs_join<TY, 1>), dim3(a.rows), dim3(64 * LP_WAVES), 0, stream, a, parts);
-    else if (parts > 1)
-        hipLaunchKernelGGL((k_logprobs_join<TY, 0>), dim3(a.rows), dim3(64), 0, stream, a, parts);
+    const LpPlan p = lp_plan(a.rows, a.vocab);
+    p.waves == 16 ? logprobs_of<TY, 16>(a, p, stream) : logprobs_of<TY, 4>(a, p, stream);
+    if (p.parts > 1 && a.top)
+        hipLaunchKernelGGL((k_logprobs_join<TY, 1>), dim3(a.rows), dim3(256), 0, stream, a, p.parts);
+    else if (p.parts > 1)
+        hipLaunchKernelGGL((k_logprobs_join<TY, 0>), dim3(a.rows), dim3(64), 0, stream, a, p.parts);
 }
 
 void launch_logprobs(const LogprobArgs& a, hipStream_t stream) {

@@ -25,8 +25,6 @@ def exact(x, tokens, top, scale):
     rows, vocab = v.shape
     with np.errstate(all="ignore"):
         z = v * scale
-        # (in F32 a product may pass the range: such a logit is hidden, or makes the row NaN)
-        z = np.where(np.abs(z) >= 2.0 ** 128 * (1 - U / 2), np.sign(z) * np.inf, z)  # half a step past the greatest
         m = z.max(1, keepdims=True)
         none = (m == -np.inf)[:, 0]
         d = np.where(none[:, None], -np.inf, z - m)
@@ -49,8 +47,9 @@ def exact(x, tokens, top, scale):
     # greatest first, the lower index first among equals, a NaN before all (a stable sort puts them so)
     ids = torch.sort(x.double().cpu() + 0.0, dim=1, descending=True, stable=True).indices[:, :top].numpy()
     toplp = np.where(bad[:, None], np.nan, np.where(none[:, None], -np.inf, np.take_along_axis(lp, ids, 1)))
-    # What the F32 steps move: z and d are rounded (U |z|, U |d|), an exponential is within 2 steps and follows
-    # its argument, a lane adds at most vocab / 64 terms in a chain and the lanes' sums in 16 more.
+    # What the F32 steps move: x - m and its products by the scale and by log2(e) are rounded (3 U |d|), an
+    # exponential is within 2 steps and follows its argument, a lane adds at most vocab / 64 terms in a chain and
+    # the lanes' sums in 16 more; Z, U |z| twice, is room for the rescaling of a running sum.
     with np.errstate(all="ignore"):
         live = p > 0
         Z = np.where(live, np.abs(z), 0).max(1)
@@ -72,6 +71,7 @@ def near(got, want, tol, what):
     got = got.double().cpu().numpy()
     assert got.shape == want.shape, what
     with np.errstate(invalid="ignore"):
+        want = np.where(np.abs(want) >= 2.0 ** 128 * (1 - U / 2), np.sign(want) * np.inf, want)  # past F32's range
         ok = (np.abs(got - want) <= tol) | (got == want) | (np.isnan(got) & np.isnan(want))
     assert ok.all(), f"{what}: {int((~ok).sum())} of {ok.size}: {got[~ok][:3]} for {want[~ok][:3]} +- {np.asarray(tol)[~ok][:3]}"
 
