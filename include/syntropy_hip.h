@@ -250,9 +250,11 @@ int syn_i8_logits(const int8_t* head, uint64_t head_bytes, uint64_t head_stride,
  * vocab or more gives NaN and -1.  Where every logit of a row is -infinity, its log probabilities are
  * -infinity and its entropy 0; a NaN or +infinity in it makes its log probabilities and its entropy NaN.
  * Among the greatest a NaN stands above +infinity; compared for the rank it is neither greater nor less.
- * Sums are held in F32 (rank: exact).  A row's results do not depend on the other rows.
+ * Sums are held in F32 (rank: exact), in an order fixed by vocab and the number of rows.  Fewer than 2^24
+ * rows of at most SYN_LOGPROBS_MAX_VOCAB logits.
  * ws: 256-byte aligned, syn_token_logprobs_workspace_bytes.  No counterpart in the reference. */
 #define SYN_LOGPROBS_MAX_TOP 64
+#define SYN_LOGPROBS_MAX_VOCAB (1 << 30)
 int syn_token_logprobs_workspace_bytes(int32_t xtype, uint32_t rows, uint32_t vocab, uint32_t top, uint64_t* bytes);
 int syn_token_logprobs(int32_t xtype, const void* x, uint64_t x_stride, uint32_t rows, uint32_t vocab,
                        const void* tokens, uint32_t token_bytes, float scale, uint32_t top, float* logprob,

@@ -1226,7 +1226,9 @@ SYN_EXPORT int syn_i8_logits(const int8_t* head, uint64_t head_bytes, uint64_t h
 namespace {
 int check_logprobs(const char* W, int32_t xtype, uint32_t rows, uint32_t vocab, uint32_t top) {
     if (xtype != SYN_F32 && !float_type(xtype)) return fail(SYN_E_UNSUPPORTED, "%s: logits of type %d are not F32, F16 or BF16", W, xtype);
-    if (vocab == 0 || vocab > 0x7FFFFF00u || rows > 0x7FFFFF00u) return fail(SYN_E_INVALID, "%s: %u rows of %u logits", W, rows, vocab);
+    if (vocab == 0) return fail(SYN_E_INVALID, "%s: rows of no logits", W);
+    if (vocab > SYN_LOGPROBS_MAX_VOCAB || rows >= 1u << 24)
+        return fail(SYN_E_UNSUPPORTED, "%s: %u rows (below 2^24) of %u logits (at most %d)", W, rows, vocab, SYN_LOGPROBS_MAX_VOCAB);
     if (top > SYN_LOGPROBS_MAX_TOP || top > vocab)
         return fail(SYN_E_UNSUPPORTED, "%s: the %u greatest of %u logits (at most %d)", W, top, vocab, SYN_LOGPROBS_MAX_TOP);
     return SYN_OK;

@@ -66,7 +66,7 @@ struct Greatest {
     uint64_t sorted[LOGPROB_MAX_TOP];      // of sort()
     uint32_t most[64 * W];                 // the lanes' greatest
     int count;                             // of keys, and of those that found no room
-    int more[2][W];
+    int more[W];
 
     // (after a barrier behind the lanes' `most`) a number that at least `top` keys' values reach: 256 values, of
     // W / 4 lanes each
@@ -103,13 +103,15 @@ struct Greatest {
     }
     // (every thread, after put) whether any thread has more to put; where there is no room left, the bound is
     // raised to the top-th of what there is, and only the greatest stay
-    SYN_DEV bool round(bool mine, int parity, int top, uint64_t& bound) {
+    SYN_DEV bool round(bool mine, int top, uint64_t& bound) {
         const bool any = __builtin_amdgcn_ballot_w64(mine) != 0;
-        if ((threadIdx.x & 63) == 0) more[parity][threadIdx.x >> 6] = any;
+        if ((threadIdx.x & 63) == 0) more[threadIdx.x >> 6] = any;
         __syncthreads();
         bool go = false;
-        for (int w = 0; w < W; ++w) go |= more[parity][w] != 0;
-        if (count >= LP_ROOM) {  // uniform
+        for (int w = 0; w < W; ++w) go |= more[w] != 0;
+        const bool full = count >= LP_ROOM;
+        if (go || full) __syncthreads();  // uniform: everyone has read what the next round writes
+        if (full) {
             sort(top);
             __syncthreads();
             const uint64_t b = sorted[top - 1];
@@ -308,8 +310,8 @@ __global__ __launch_bounds__(64 * W) void k_logprobs(LogprobArgs g, int parts, i
         int at = 0, in = 0;
         bool go = true;
 #pragma unroll 1
-        for (int parity = 0; go; parity ^= 1) {  // uniform
-            if (may == 0 && mine != 0) {         // the lane's next step
+        while (go) {  // uniform
+            if (may == 0 && mine != 0) {  // the lane's next step
                 const int gi = __builtin_ctz(mine), st = step0 + (gi * group_steps + in) * W;
                 at = st * LP_STEP;
                 // (equal values: a group behind the bound's index holds nothing before it)
@@ -329,7 +331,7 @@ __global__ __launch_bounds__(64 * W) void k_logprobs(LogprobArgs g, int parts, i
                 const uint64_t key = lp_key(lp_load<TY>(x, id), id);  // (a choice of the registers by lane costs more)
                 if (key > bound && best.put(key)) break;
             }
-            go = best.round(may != 0 || mine != 0, parity, g.top, bound);
+            go = best.round(may != 0 || mine != 0, g.top, bound);
         }
         const int n = best.sort(g.top);
         if ((int)threadIdx.x >= n && (int)threadIdx.x < g.top) best.sorted[threadIdx.x] = 0;
@@ -392,12 +394,12 @@ __global__ __launch_bounds__(TOP ? 256 : 64) void k_logprobs_join(LogprobArgs g,
         bool go = true;
         int i = threadIdx.x;
 #pragma unroll 1
-        for (int parity = 0; go; parity ^= 1) {  // uniform
+        while (go) {  // uniform
             if (i < n && !(k > bound && best.put(k))) {
                 i += 256;
                 k = i < n ? keys[i] : 0;
             }
-            go = best.round(i < n, parity, g.top, bound);
+            go = best.round(i < n, g.top, bound);
         }
         best.sort(g.top);  // (at least `top` of them: the vocabulary has as many)
         __syncthreads();

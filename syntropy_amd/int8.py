@@ -22,7 +22,7 @@ from .gemv import GemvError, _need, _on_stream, _ptr_rows, _value_type
 MAX_K = 131072
 
 
-@dataclass(eq=False)
+@dataclass(frozen=True, eq=False)
 class Weights:
     """`codes` int8 [n_out, k_in] with F32 `scales` [n_out] and an optional F32 `bias` [n_out], device
     tensors: the row o stands for codes[o] * scales[o].  Rows lie side by side and start on 16 bytes: a
@@ -37,18 +37,19 @@ class Weights:
         c, s, b = self.codes, self.scales, self.bias
         if not (c.is_cuda and c.dtype == torch.int8 and c.dim() == 2):
             raise GemvError("Len", "codes must be an int8 device tensor of rows")
-        self.n_out, self.k_in = c.shape
-        if not 1 <= self.k_in <= MAX_K:
-            raise GemvError("RowLength", f"rows of {self.k_in} codes (1 to {MAX_K})")
+        n_out, k_in = c.shape
+        if not 1 <= k_in <= MAX_K:
+            raise GemvError("RowLength", f"rows of {k_in} codes (1 to {MAX_K})")
         for what, t in (("scales", s), ("bias", b)):
             if t is None and what == "bias":
                 continue
-            if not (t.device == c.device and t.dtype == torch.float32 and t.is_contiguous()) or t.shape != (self.n_out,):
-                raise GemvError("Len", f"{what} must be a contiguous F32 tensor of {self.n_out} values beside the codes")
-        if c.stride(1) != 1 or c.stride(0) < self.k_in or c.stride(0) % 16 or c.data_ptr() % 16:
-            rows = torch.zeros(self.n_out, -(-self.k_in // 128) * 128, dtype=torch.int8, device=c.device)[:, :self.k_in]
-            self.codes = c = rows.copy_(c)
-        self.device = c.get_device()
+            if not (t.device == c.device and t.dtype == torch.float32 and t.is_contiguous()) or t.shape != (n_out,):
+                raise GemvError("Len", f"{what} must be a contiguous F32 tensor of {n_out} values beside the codes")
+        if c.stride(1) != 1 or c.stride(0) < k_in or c.stride(0) % 16 or c.data_ptr() % 16:
+            rows = torch.zeros(n_out, -(-k_in // 128) * 128, dtype=torch.int8, device=c.device)[:, :k_in]
+            c = rows.copy_(c)
+        for name, v in (("codes", c), ("n_out", n_out), ("k_in", k_in), ("device", c.get_device())):
+            object.__setattr__(self, name, v)
 
     def view(self) -> tuple:
         """The C ABI's arguments: the codes' view (address, bytes, stride), scales, bias."""
@@ -101,6 +102,8 @@ def _product(name, gated, w, n, x, rows, y, ws, dtype, stream):
         else:
             out, oty, os = y, yty, ys
         if ws is not None:
+            if ws.get_device() != w.device or ws.dtype != torch.uint8 or not ws.is_contiguous():
+                raise GemvError("Len", "`ws` must be a contiguous uint8 tensor on the operands' device")
             wp, wb = ws.data_ptr(), ws.numel()
         else:
             wb = _need("syn_i8_gemv_workspace_bytes", n, w.k_in, rows, 1 if gated else 0)

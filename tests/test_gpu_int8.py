@@ -239,6 +239,23 @@ def test_offsets_past_32_bits(I):
         check(I, (codes, w[1], None), x[rows - r:], r, "gated", gated=True, y=y[rows - r:, :n // 2])
 
 
+@pytest.mark.parametrize("far", [False, True])
+def test_the_most_rows(I, far):
+    """2,097,120 rows, over weights side by side and over weight rows too far apart for a tile."""
+    rows, n, k = 2097120, 8, 16
+    w = make(n, k, 5)
+    codes = torch.empty(n << 28, dtype=torch.int8, device="cuda").as_strided((n, k), (1 << 28, 1)) if far else w[0]
+    codes.copy_(w[0].clone())
+    x = torch.randn(rows, k, generator=torch.Generator("cuda").manual_seed(1), device="cuda")
+    announce(f"most rows, far {far}")
+    y = I.gemv(I.Weights(codes, w[1]), x, rows)
+    q, sx = I.quantize_rows(x)
+    S = (q.double() @ w[0].double().t()).float()
+    assert torch.equal(y, S * sx[:, None] * w[1])
+    with pytest.raises(I.SynError):
+        I.gemv(I.Weights(codes, w[1]), torch.empty(rows + 1, k, device="cuda"), rows + 1)
+
+
 @pytest.mark.parametrize("rows", [1, 6, 33, 256])
 def test_codes_held_on_odd_bytes_are_laid_out_once(I, rows):
     k, n = 77, 50
@@ -271,6 +288,32 @@ def test_a_row_does_not_depend_on_the_others(I):
     for rows in (1, 2, 3, 8, 16, 17, 32, 40, 64, 90, 128, 200):
         announce(f"alone and among {rows}")
         same(I.gemv(W, x[100:], rows), whole[100:100 + rows].cpu(), f"{rows}")
+
+
+def test_refusals_on_the_device(I):
+    """What is wrong with operands that are on the device; nothing is written."""
+    W = I.Weights(*make(8, 64, 1))
+    x, y = torch.ones(4, 64, device="cuda"), torch.full((4, 8), 7.0, device="cuda")
+    for bad in (dict(x=x[:, :63]), dict(x=x.double()), dict(x=x.cpu()), dict(rows=5), dict(y=y[:3]), dict(y=y.int()),
+                dict(y=y.bfloat16(), dtype=torch.float32), dict(dtype=torch.float64), dict(y=y[:, ::2]),
+                dict(x=x[:1].expand(4, 64)), dict(y=y.cpu()), dict(ws=torch.empty(1 << 20, device="cuda"), rows=2),
+                dict(ws=torch.empty(1 << 20, dtype=torch.uint8), rows=2), dict(rows=-1)):
+        with pytest.raises(I.GemvError):
+            I.gemv(W, **{**dict(x=x, rows=4, y=y if "dtype" not in bad else None), **bad})
+    with pytest.raises(I.SynError):
+        I.gemv(W, x, 4, y=y, ws=torch.empty(256, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(I.GemvError):
+        I.gate_up_act(I.Weights(*make(9, 64, 1)), x, 4)
+    for codes, scales in ((W.codes, W.scales[:7]), (W.codes, W.scales.double()), (W.codes.float(), W.scales),
+                          (W.codes, W.scales.cpu()), (W.codes[0], W.scales)):
+        with pytest.raises(I.GemvError):
+            I.Weights(codes, scales)
+    with pytest.raises(I.GemvError):
+        I.Weights(torch.empty(1, 131073, dtype=torch.int8, device="cuda"), torch.ones(1, device="cuda"))
+    with pytest.raises(AttributeError):
+        W.codes = W.codes[:4]
+    torch.cuda.synchronize()
+    assert (y == 7.0).all()
 
 
 def test_no_rows_and_no_outputs(I):

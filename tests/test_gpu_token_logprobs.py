@@ -175,6 +175,21 @@ def test_equal_values_go_by_index(S):
             check(S, x.bfloat16().cuda(), torch.tensor([5, vocab - 1, 96]).cuda(), top, what="ties")
 
 
+@pytest.mark.parametrize("rows,vocab", [(2, 700), (3, 40000), (1, 128256), (300, 900)])
+def test_more_candidates_than_are_held_at_once(S, rows, vocab):
+    """Rows whose greatest values rise along the row, or are as many as half of it, so that what passes the first
+    bound is many times what is gathered at once; the same call gives the same bits."""
+    i = torch.arange(vocab, device="cuda")
+    for x in ((i // 8).float(), (i % 16 == 3).float(), (i % 2).float(), (i // 1024).float(), (vocab - i).float() // 100):
+        x = (x * 2.0 ** -7).repeat(rows, 1)
+        x[0, vocab // 2] = 5000.0
+        t = torch.full((rows,), vocab - 1, device="cuda")
+        r = check(S, x, t, 64, what="many candidates")
+        for _ in range(3):
+            again = S.token_logprobs(x, t, top=64)
+            assert all(torch.equal(a, b) for a, b in zip(r, again))
+
+
 def test_strided_unaligned_and_far_rows(S):
     x, t = logits(9, 3100, torch.float32, 2)
     for dt in (torch.float32, torch.bfloat16, torch.float16):
