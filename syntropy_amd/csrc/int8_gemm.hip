@@ -343,10 +343,9 @@ I8Pick i8_gemm_pick(int rows_w, int k, int T, int gated) {
             const int64_t wgs = tw * tt * s, rounds = (wgs + 255) / 256;
             if (s > 1 && (kp < 1024 * s || wgs > 256)) break;  // (a part has four stages and more)
             const float last = (float)(wgs - 256 * (rounds - 1)) / 256.0f, turns = (float)rounds - 0.25f + 0.25f * last;
-            float us = (float)rounds * t.base + turns * t.per_k * (float)kp / (float)s;
+            const float work = (float)rounds * t.base + turns * t.per_k * (float)kp / (float)s;
             const float rate = EACH * (float)wgs < HBM ? EACH * (float)wgs : HBM;
-            us = us > bytes / rate ? us : bytes / rate;
-            us += LAUNCH;
+            float us = LAUNCH + (work > bytes / rate ? work : bytes / rate + 0.1f * work);
             if (s > 1) us += FOLD + 8.0f * (float)s * (float)T * (float)rows_w / SUMS;
             if (least == 0.0f || us < least) {
                 least = us;

@@ -67,21 +67,30 @@ struct Greatest {
     uint32_t most[64 * W];                 // the lanes' greatest
     int count;                             // of keys, and of those that found no room
     int more[W];
+    uint32_t reached;                      // of bound()
 
-    // (after a barrier behind the lanes' `most`) a number that at least `top` keys' values reach: 256 values, of
-    // W / 4 lanes each
-    SYN_DEV uint32_t bound(int top) const {
-        uint32_t of[4];
+    // (every thread) a number that at least `top` keys reach, from the lanes' greatest values' orders: of 256
+    // values, each of W / 4 lanes.  One wavefront counts; all of them would be in each other's way.
+    SYN_DEV uint32_t bound(uint32_t mine, int top) {
+        most[threadIdx.x] = mine;
+        if (threadIdx.x == 0) count = 0;
+        __syncthreads();
+        if (threadIdx.x < 64) {
+            uint32_t of[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            of[j] = 0;
+            for (int j = 0; j < 4; ++j) {
+                of[j] = 0;
 #pragma unroll
-            for (int w = j; w < W; w += 4) {
-                const uint32_t v = most[64 * w + (threadIdx.x & 63)];
-                of[j] = v > of[j] ? v : of[j];
+                for (int w = j; w < W; w += 4) {
+                    const uint32_t v = most[64 * w + threadIdx.x];
+                    of[j] = v > of[j] ? v : of[j];
+                }
             }
+            const uint32_t r = reached_by(of, top);
+            if (threadIdx.x == 0) reached = r;
         }
-        return reached_by(of, top);
+        __syncthreads();
+        return reached;
     }
     // (every thread; a barrier before and after) the `top` greatest in order; returns how many there are
     SYN_DEV int sort(int top) {
@@ -299,10 +308,7 @@ __global__ __launch_bounds__(64 * W) void k_logprobs(LogprobArgs g, int parts, i
         cur = nxt;
     }
     if constexpr (TOP) {
-        best.most[threadIdx.x] = lp_order(most);
-        if (threadIdx.x == 0) best.count = 0;
-        __syncthreads();
-        const uint32_t b = best.bound(g.top);
+        const uint32_t b = best.bound(lp_order(most), g.top);
         uint64_t bound = b ? ((uint64_t)b << 32) - 1 : 0;  // all of that value are above it
         uint32_t mine = 0;  // the lane's groups that reach it
         for (int i = 0; i < n_groups; ++i) mine |= groups[wave][i][lane] >= b ? 1u << i : 0u;
@@ -386,10 +392,7 @@ __global__ __launch_bounds__(TOP ? 256 : 64) void k_logprobs_join(LogprobArgs g,
         const int n = parts * g.top;
         uint64_t k = (int)threadIdx.x < n ? keys[threadIdx.x] : 0, mx = k;
         for (int i = threadIdx.x + 256; i < n; i += 256) mx = keys[i] > mx ? keys[i] : mx;
-        best.most[threadIdx.x] = (uint32_t)(mx >> 32);
-        if (threadIdx.x == 0) best.count = 0;
-        __syncthreads();
-        const uint32_t b = best.bound(g.top);
+        const uint32_t b = best.bound((uint32_t)(mx >> 32), g.top);
         uint64_t bound = b ? ((uint64_t)b << 32) - 1 : 0;
         bool go = true;
         int i = threadIdx.x;
