@@ -252,15 +252,19 @@ def _ptr_rows(t: torch.Tensor, rows: int, n: int, what: str, device=None) -> int
     of two dimensions with any row stride, or a contiguous one of enough values."""
     if not t.is_cuda or (device is not None and t.get_device() != device):
         raise GemvError("Len", f"`{what}` must be on the operands' device")
+    shape = t.shape
+    if len(shape) == 2 and shape[1] == n and 0 <= rows <= shape[0]:
+        step, inner = t.stride()
+        if (inner == 1 or n == 1) and (step >= n or rows <= 1):
+            return step if step > n else n
     if rows < 0:
         raise GemvError("Len", f"{rows} rows")
-    if t.dim() == 2 and t.shape[1] == n and t.shape[0] >= rows:
-        step, inner = t.stride()
-        if (inner == 1 or n == 1) and (rows <= 1 or step >= n):
-            return step if step > n else n
     if not t.is_contiguous() or t.numel() < rows * n:
         raise GemvError("Len", f"`{what}` holds {t.numel()} values, the op needs {rows} rows of {n} side by side")
     return n
+
+
+_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def _on_stream(t: torch.Tensor, stream, body):
@@ -268,10 +272,10 @@ def _on_stream(t: torch.Tensor, stream, body):
     device current, and what torch allocates meanwhile belonging to that stream."""
     device = t.get_device()
     if stream is None:
-        if device == torch._C._cuda_getDevice():
-            return body(torch._C._cuda_getCurrentRawStream(device))
+        if device == _current_device():
+            return body(_current_stream(device))
         with torch.cuda.device(device):
-            return body(torch._C._cuda_getCurrentRawStream(device))
+            return body(_current_stream(device))
     if not hasattr(stream, "cuda_stream"):
         stream = torch.cuda.ExternalStream(int(stream), device=device)
     if stream.device.index != device:
@@ -309,20 +313,19 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, sca
     if tokens.dtype not in (torch.int32, torch.int64) or not tokens.is_contiguous() or tokens.device != logits.device:
         raise GemvError("Len", "tokens must be contiguous int32 or int64 values beside the logits")
     ty, stride = _value_type(logits, "logits"), _ptr_rows(logits, rows, vocab, "logits")
-    dev = logits.device
+    return _on_stream(logits, stream, lambda handle: _logprobs(logits, ty, stride, rows, vocab, tokens, top, scale, handle))
 
-    def launch(handle):
-        f32, i32 = torch.float32, torch.int32
-        r = TokenLogprobs(torch.empty(rows, dtype=f32, device=dev), torch.empty(rows, dtype=i32, device=dev),
-                          torch.empty(rows, dtype=f32, device=dev), torch.empty(rows, top, dtype=i32, device=dev),
-                          torch.empty(rows, top, dtype=f32, device=dev))
-        need = _need("syn_token_logprobs_workspace_bytes", ty, rows, vocab, top)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        call("syn_token_logprobs", ty, logits.data_ptr(), stride, rows, vocab, tokens.data_ptr(), tokens.element_size(),
-             scale, top, r.logprob.data_ptr(), r.rank.data_ptr(), r.entropy.data_ptr(), r.top_ids.data_ptr(),
-             r.top_logprobs.data_ptr(), ws.data_ptr() if need else None, need, handle)
-        return r
-    return _on_stream(logits, stream, launch)
+
+def _logprobs(logits, ty, stride, rows, vocab, tokens, top, scale, handle) -> TokenLogprobs:
+    dev, f32, i32, new = logits.device, torch.float32, torch.int32, torch.empty
+    lp, rank, entropy = new(rows, dtype=f32, device=dev), new(rows, dtype=i32, device=dev), new(rows, dtype=f32, device=dev)
+    ids, lps = new((rows, top), dtype=i32, device=dev), new((rows, top), dtype=f32, device=dev)
+    need = _need("syn_token_logprobs_workspace_bytes", ty, rows, vocab, top)
+    ws = new(need, dtype=torch.uint8, device=dev) if need else None
+    call("syn_token_logprobs", ty, logits.data_ptr(), stride, rows, vocab, tokens.data_ptr(), tokens.element_size(), scale,
+         top, lp.data_ptr(), rank.data_ptr(), entropy.data_ptr(), ids.data_ptr(), lps.data_ptr(),
+         ws.data_ptr() if need else None, need, handle)
+    return TokenLogprobs(lp, rank, entropy, ids, lps)
 
 
 class GemvBatch:

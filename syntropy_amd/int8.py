@@ -17,7 +17,7 @@ from dataclasses import dataclass
 import torch
 
 from ._lib import SynError, call
-from .gemv import GemvError, _need, _on_stream, _ptr_rows, _value_type
+from .gemv import GemvError, _current_device, _current_stream, _need, _on_stream, _ptr_rows, _value_type
 
 MAX_K = 131072
 
@@ -48,15 +48,12 @@ class Weights:
         if c.stride(1) != 1 or c.stride(0) < k_in or c.stride(0) % 16 or c.data_ptr() % 16:
             rows = torch.zeros(n_out, -(-k_in // 128) * 128, dtype=torch.int8, device=c.device)[:, :k_in]
             c = rows.copy_(c)
-        for name, v in (("codes", c), ("n_out", n_out), ("k_in", k_in), ("device", c.get_device())):
-            object.__setattr__(self, name, v)
-
-    def view(self) -> tuple:
-        """The C ABI's arguments: the codes' view (address, bytes, stride), scales, bias."""
-        c, b = self.codes, self.bias
         stride = c.stride(0)
-        return (c.data_ptr(), (self.n_out - 1) * stride + self.k_in if self.n_out else 0, stride, self.scales.data_ptr(),
+        # the C ABI's arguments: the codes' view (address, bytes, stride), scales, bias
+        view = (c.data_ptr(), (n_out - 1) * stride + k_in if n_out else 0, stride, s.data_ptr(),
                 0 if b is None else b.data_ptr())
+        for name, v in (("codes", c), ("n_out", n_out), ("k_in", k_in), ("device", c.get_device()), ("view", view)):
+            object.__setattr__(self, name, v)
 
 
 def quantize_rows(x: torch.Tensor, stream=None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -90,35 +87,37 @@ def workspace_bytes(n_out: int, k_in: int, rows: int, gated: bool = False) -> in
 
 def _product(name, gated, w, n, x, rows, y, ws, dtype, stream):
     ty, xs = _value_type(x, "x"), _ptr_rows(x, rows, w.k_in, "x", w.device)
-    if y is not None:
+    if stream is not None or w.device != _current_device():
+        return _on_stream(x, stream, lambda handle: _launch(name, gated, w, n, x, ty, xs, rows, y, ws, dtype, handle))
+    return _launch(name, gated, w, n, x, ty, xs, rows, y, ws, dtype, _current_stream(w.device))
+
+
+def _launch(name, gated, w, n, x, ty, xs, rows, y, ws, dtype, handle):
+    if y is None:
+        y = torch.empty(rows, n, dtype=x.dtype if dtype is None else dtype, device=x.device)
+        yty, ys = _value_type(y, "y"), n
+    else:
         if dtype is not None and dtype != y.dtype:
             raise GemvError("Len", f"`y` is of {y.dtype}, not {dtype}")
         yty, ys = _value_type(y, "y"), _ptr_rows(y, rows, n, "y", w.device)
-
-    def launch(handle):
-        if y is None:
-            out = torch.empty(rows, n, dtype=x.dtype if dtype is None else dtype, device=x.device)
-            oty, os = _value_type(out, "y"), n
-        else:
-            out, oty, os = y, yty, ys
-        if ws is not None:
-            if ws.get_device() != w.device or ws.dtype != torch.uint8 or not ws.is_contiguous():
-                raise GemvError("Len", "`ws` must be a contiguous uint8 tensor on the operands' device")
-            wp, wb = ws.data_ptr(), ws.numel()
-        else:
-            wb = _need("syn_i8_gemv_workspace_bytes", n, w.k_in, rows, 1 if gated else 0)
-            scratch = torch.empty(wb, dtype=torch.uint8, device=x.device) if wb else None
-            wp = scratch.data_ptr() if wb else 0
-        call(name, *w.view(), n, w.k_in, ty, x.data_ptr(), xs, rows, oty, out.data_ptr(), os, wp, wb, handle)
-        return out
-    return _on_stream(x, stream, launch)
+    if ws is None:
+        wp, wb = 0, _need("syn_i8_gemv_workspace_bytes", n, w.k_in, rows, gated)
+        if wb:
+            ws = torch.empty(wb, dtype=torch.uint8, device=x.device)
+            wp = ws.data_ptr()
+    else:
+        if ws.get_device() != w.device or ws.dtype != torch.uint8 or not ws.is_contiguous():
+            raise GemvError("Len", "`ws` must be a contiguous uint8 tensor on the operands' device")
+        wp, wb = ws.data_ptr(), ws.numel()
+    call(name, *w.view, n, w.k_in, ty, x.data_ptr(), xs, rows, yty, y.data_ptr(), ys, wp, wb, handle)
+    return y
 
 
 def gemv(w: Weights, x: torch.Tensor, rows: int, y: torch.Tensor | None = None, ws: torch.Tensor | None = None,
          dtype: torch.dtype | None = None, stream=None) -> torch.Tensor:
     """y [rows, n_out] = x W^T (+ bias) for the first `rows` rows of x [., k_in], of x's type, y's or
     `dtype` (F32, F16, BF16).  x and y may have strided rows."""
-    return _product("syn_i8_gemv", False, w, w.n_out, x, rows, y, ws, dtype, stream)
+    return _product("syn_i8_gemv", 0, w, w.n_out, x, rows, y, ws, dtype, stream)
 
 
 def gate_up_act(w: Weights, x: torch.Tensor, rows: int, y: torch.Tensor | None = None, ws: torch.Tensor | None = None,
@@ -127,7 +126,7 @@ def gate_up_act(w: Weights, x: torch.Tensor, rows: int, y: torch.Tensor | None =
     silu(gate x) * (up x), both products the F32 values of gemv."""
     if w.n_out % 2:
         raise GemvError("Len", f"a stacked gate/up matrix has an even row count, not {w.n_out}")
-    return _product("syn_i8_gate_up_act", True, w, w.n_out // 2, x, rows, y, ws, dtype, stream)
+    return _product("syn_i8_gate_up_act", 1, w, w.n_out // 2, x, rows, y, ws, dtype, stream)
 
 
 class Rows:
@@ -154,7 +153,7 @@ def gemv_quantized(w: Weights, r: Rows, y: torch.Tensor, stream=None) -> torch.T
     if w.device != r.ws.get_device():
         raise GemvError("Len", f"the rows are on {r.ws.device}, the weights on cuda:{w.device}")
     yty, ys = _value_type(y, "y"), _ptr_rows(y, r.rows, w.n_out, "y", w.device)
-    _on_stream(y, stream, lambda handle: call("syn_i8_gemv_quantized", *w.view(), w.n_out, w.k_in, r.rows, yty, y.data_ptr(),
+    _on_stream(y, stream, lambda handle: call("syn_i8_gemv_quantized", *w.view, w.n_out, w.k_in, r.rows, yty, y.data_ptr(),
                                               ys, r.ws.data_ptr(), r.ws.numel(), handle))
     return y
 
@@ -177,7 +176,7 @@ def logits(head: Weights, g: torch.Tensor, eps: float, x: torch.Tensor, rows: in
         out = torch.empty(rows, head.n_out, dtype=torch.float32, device=x.device) if y is None else y
         need = _need("syn_i8_logits_workspace_bytes", head.n_out, head.k_in, rows)
         ws = torch.empty(max(need, 256), dtype=torch.uint8, device=x.device)
-        call("syn_i8_logits", *head.view()[:4], head.n_out, head.k_in, g.data_ptr(), C.c_float(eps), x.data_ptr(), rows,
+        call("syn_i8_logits", *head.view[:4], head.n_out, head.k_in, g.data_ptr(), C.c_float(eps), x.data_ptr(), rows,
              out.data_ptr(), ws.data_ptr(), ws.numel(), handle)
         return out
     return _on_stream(x, stream, launch)
