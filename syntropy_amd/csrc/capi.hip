@@ -1048,7 +1048,7 @@ int check_i8_shape(const char* W, uint64_t w_rows, uint32_t k, uint32_t rows) {
 
 uint64_t i8_ws_bytes(uint64_t w_rows, uint32_t k, uint32_t rows, int gated, bool quantized = false) {
     if (rows == 0 || (w_rows == 0 && !quantized)) return 0;
-    if (!quantized && syn::i8_fused((int)k, (int)rows)) return 0;
+    if (!quantized && syn::i8_fused((int)w_rows, (int)k, (int)rows)) return 0;
     uint64_t b = syn::i8_act_layout(rows, k).partial;
     const uint64_t splits = (uint64_t)syn::i8_splits((int)w_rows, (int)k, (int)rows, gated);
     if (splits > 1) b += 4 * splits * rows * w_rows;
@@ -1111,7 +1111,7 @@ int i8_product(const char* W, int gated, const int8_t* w, uint64_t w_bytes, uint
     a.partial = a.splits > 1 ? (int*)(base + l.partial) : nullptr;
     a.gated = gated;
     if (!quantized) {
-        if (syn::i8_fused((int)k_in, (int)rows)) {
+        if (syn::i8_fused((int)w_rows, (int)k_in, (int)rows)) {
             a.x = x;
             a.ldx = x_stride;
             a.xtype = xtype;

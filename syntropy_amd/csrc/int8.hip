@@ -115,7 +115,7 @@ static void launch_i8_fold(const I8Args& a, hipStream_t stream) {
 }
 
 // ---- the choice ----------------------------------------------------------------------------------------
-bool i8_fused(int k, int T) { return i8_few_fits(T) && i8_few_fused(k, T); }
+bool i8_fused(int rows_w, int k, int T) { return i8_few_fits(T) && i8_few_fused(rows_w, k, T); }
 
 int i8_splits(int rows_w, int k, int T, int gated) { return i8_few_fits(T) ? 1 : i8_gemm_pick(rows_w, k, T, gated).splits; }
 

@@ -163,7 +163,7 @@ void launch_i8_quantize(int xtype, const void* x, uint64_t ldx, int rows, int k,
                         float* scales, hipStream_t stream);
 // int8_few.hip: up to 16 tokens, weights straight to registers
 bool i8_few_fits(int T);
-bool i8_few_fused(int k, int T);  // the kernel quantizes the rows itself
+bool i8_few_fused(int rows_w, int k, int T);  // the kernel quantizes the rows itself
 void launch_i8_few(const I8Args& a, hipStream_t stream);
 // int8_gemm.hip: tiles through LDS, K in one part or several
 struct I8Pick {
@@ -174,7 +174,7 @@ bool i8_gemm_reaches(int tile, const I8Args& a);
 void launch_i8_gemm(int tile, const I8Args& a, hipStream_t stream);
 // int8.hip
 int i8_splits(int rows_w, int k, int T, int gated);
-bool i8_fused(int k, int T);
+bool i8_fused(int rows_w, int k, int T);
 void launch_i8_gemv(const I8Args& a, hipStream_t stream);
 
 }  // namespace syn

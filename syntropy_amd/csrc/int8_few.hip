@@ -15,20 +15,26 @@
 // The tokens' codes of a turn are loaded with its weights: loads return in order, so that codes asked for when
 // they are needed would wait for the next turn's weights too.
 //
-// FUSED: one row in one launch.  Each workgroup quantizes it into LDS while its first weights fly, a launch
-// less.
+// FUSED: up to eight short rows in one launch.  Each workgroup quantizes them into LDS while its first weights
+// fly, NW / rows wavefronts a row, a launch less.
 #include "int8.hpp"
 #include "kernels.hpp"
 
 namespace syn {
 
 constexpr int FEW_MAX_T = 16;
+// A fused row's values a wavefront, whole pieces of 8: at most four pieces a lane.
+constexpr int FEW_PIECES = 4, FEW_FUSED_WAVES = 8;
+constexpr uint64_t FEW_FUSED_MOST = 150000000;
+// log2 of the wavefronts a row: eight for one row, four for two, two for three and four, one.
+SYN_HD inline int few_share(int rows) { return rows == 1 ? 3 : rows == 2 ? 2 : rows <= 4 ? 1 : 0; }
+SYN_HD inline int few_part(int k, int rows) { return (((k + 7) / 8 + (1 << few_share(rows)) - 1) >> few_share(rows)) * 8; }
 
-template <int RT, int TG, int U, int NW, int FUSED, int GATED>
+template <int RT, int TG, int U, int NW, int FUSED, int GATED>  // FUSED: pieces of 8 values a lane, or 0
 __global__ __launch_bounds__(64 * NW, TG > 1 || U * RT > 4 ? 4 : 6) void k_i8_few(I8Args g) {
     static_assert(!GATED || RT == 2, "a gate tile and an up tile");
     static_assert(RT * TG <= 4, "the outputs of one wavefront");
-    static_assert(!FUSED || TG == 1, "one row");
+    static_assert(!FUSED || TG == 1, "up to eight rows");
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -74,38 +80,55 @@ __global__ __launch_bounds__(64 * NW, TG > 1 || U * RT > 4 ? 4 : 6) void k_i8_fe
     load(s, cur);
     load(s + TURN, nxt);
 
-    float* row_scale = reinterpret_cast<float*>(lds);  // FUSED: the row's scale, the wavefronts' maxima, its codes
+    // FUSED: the rows' scales, the wavefronts' maxima, the rows' codes (neighbouring rows on other banks)
+    float* row_scale = reinterpret_cast<float*>(lds);
     uint8_t* codes = lds + 128;
+    const int cs = kp + 16;
     if constexpr (FUSED) {
-        uint32_t* top = reinterpret_cast<uint32_t*>(lds + 16);
-        auto row = [&](auto type) {
+        uint32_t* top = reinterpret_cast<uint32_t*>(lds + 32);
+        auto rows = [&](auto type) {
             constexpr int TY = decltype(type)::value;
-            const uint8_t* x = (const uint8_t*)g.x + (uint64_t)t0 * g.ldx * (TY == T_F32 ? 4 : 2);
-            float v[2][8];  // i8_few_fused: a row is at most two pieces of 8 a thread
+            const int share = 1 << few_share(nt), r = wave >> few_share(nt), part = wave & (share - 1);  // uniform
+            const int len = few_part(g.k, nt), end = (part + 1) * len < g.k ? (part + 1) * len : g.k;
+            const uint8_t* x = (const uint8_t*)g.x + (uint64_t)(t0 + r) * g.ldx * (TY == T_F32 ? 4 : 2);
+            float v[FUSED][8];
             uint32_t m = 0;
+            if (r < nt) {  // uniform
 #pragma unroll
-            for (int p = 0; p < 2; ++p) i8_load8<TY>(x, 8 * ((int)threadIdx.x + 64 * NW * p), g.k, v[p]);
+                for (int p = 0; p < FUSED; ++p) {
+                    if (512 * p >= len) break;  // uniform
+                    i8_load8<TY>(x, part * len + 8 * (lane + 64 * p), end, v[p]);
+                }
 #pragma unroll
-            for (int p = 0; p < 2; ++p) m = i8_max8(v[p], m);
-            m = group_max_u32<64>(m);
+                for (int p = 0; p < FUSED; ++p) {
+                    if (512 * p >= len) break;
+                    m = i8_max8(v[p], m);
+                }
+                m = group_max_u32<64>(m);
+            }
             if (lane == 0) top[wave] = m;
             __syncthreads();
+            if (r < nt) {
+                const I8Scale sc = i8_scale(group_max_u32<64>(top[(r << few_share(nt)) + (lane & (share - 1))]));
+                if (lane == 0 && part == 0) row_scale[r] = sc.s;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) m = m > top[w] ? m : top[w];
-            const I8Scale sc = i8_scale(m);
-            if (threadIdx.x == 0) *row_scale = sc.s;
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                const int i = 8 * ((int)threadIdx.x + 64 * NW * p);
-                if (i < kp) *reinterpret_cast<uint2*>(codes + i) = i8_codes8(v[p], sc.inv);
+                for (int p = 0; p < FUSED; ++p) {
+                    if (512 * p >= len) break;
+                    const int i = part * len + 8 * (lane + 64 * p);
+                    if (8 * (lane + 64 * p) < len && i < kp)
+                        *reinterpret_cast<uint2*>(codes + r * cs + i) = i8_codes8(v[p], sc.inv);
+                }
+                // (zeros from the last part's end to the row's)
+                if (part == share - 1)
+                    for (int i = share * len + 8 * lane; i < kp; i += 512) *reinterpret_cast<uint2*>(codes + r * cs + i) = uint2{0, 0};
             }
         };
         if (g.xtype == T_F32)
-            row(std::integral_constant<int, T_F32>{});
+            rows(std::integral_constant<int, T_F32>{});
         else if (g.xtype == T_F16)
-            row(std::integral_constant<int, T_F16>{});
+            rows(std::integral_constant<int, T_F16>{});
         else
-            row(std::integral_constant<int, T_BF16>{});
+            rows(std::integral_constant<int, T_BF16>{});
         __syncthreads();
     }
 
@@ -119,7 +142,7 @@ __global__ __launch_bounds__(64 * NW, TG > 1 || U * RT > 4 ? 4 : 6) void k_i8_fe
                 i8x16 b;
                 if constexpr (FUSED) {
                     b = i8x16{0, 0, 0, 0};
-                    if (c == 0) b = *reinterpret_cast<const i8x16*>(codes + I8_LINE * (s + u) + piece);
+                    if (c < nt) b = *reinterpret_cast<const i8x16*>(codes + c * cs + I8_LINE * (s + u) + piece);
                 } else {
                     b = o.x[u][j];
                 }
@@ -140,7 +163,7 @@ __global__ __launch_bounds__(64 * NW, TG > 1 || U * RT > 4 ? 4 : 6) void k_i8_fe
 
     // The wavefronts' sums.  Lane l holds columns l & 15, rows 4 (l >> 4) .. + 3 of 16: those of the first half
     // by the first (lanes 0..7 and 16..23) and of the second by the second (40..47 and 56..63).
-    i8x16* red = reinterpret_cast<i8x16*>(lds + (FUSED ? 128 + kp : 0));  // [wave][RT][TG][64]
+    i8x16* red = reinterpret_cast<i8x16*>(lds + (FUSED ? 128 + nt * cs : 0));  // [wave][RT][TG][64]
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -160,7 +183,7 @@ __global__ __launch_bounds__(64 * NW, TG > 1 || U * RT > 4 ? 4 : 6) void k_i8_fe
             sum[m] += r[16 * half + c] + r[16 * half + 40 + c];
         }
     if (t >= nt) return;
-    const float sx = FUSED ? *row_scale : g.xs[t0 + t];
+    const float sx = FUSED ? row_scale[t] : g.xs[t0 + t];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const int64_t n = n0 + 8 * i + 4 * half + e;
@@ -178,13 +201,17 @@ __global__ __launch_bounds__(64 * NW, TG > 1 || U * RT > 4 ? 4 : 6) void k_i8_fe
 
 bool i8_few_fits(int T) { return T <= FEW_MAX_T; }
 
-// One row of at most two pieces of 8 values a thread of the largest workgroup (4096 x 4096: 6.7 against 8.2 us
-// with the row quantized in a launch before).
-bool i8_few_fused(int k, int T) { return T == 1 && k <= 16384; }
+// One row, or as many as take each workgroup no longer than a launch (a value costs a workgroup's wavefronts
+// about eight operations), where the wavefronts' registers hold them.  4096 x 4096 at one row 6.7 us against 8.2
+// with the row quantized in a launch before.
+bool i8_few_fused(int rows_w, int k, int T) {
+    if (T < 1 || T > 8 || few_part(k, T) > 512 * FEW_PIECES) return false;
+    return T == 1 || (uint64_t)rows_w * (uint64_t)T * (uint64_t)k <= FEW_FUSED_MOST;
+}
 
 template <int RT, int TG, int U, int NW, int FUSED, int GATED>
 static void launch_few(const I8Args& a, hipStream_t stream) {
-    const int lds = NW * RT * TG * 1024 + (FUSED ? 128 + (int)i8_padded(a.k) : 0);
+    const int lds = NW * RT * TG * 1024 + (FUSED ? 128 + a.T * ((int)i8_padded(a.k) + 16) : 0);
     const int per = 8 * (GATED ? 1 : RT);
     static const hipError_t most = hipFuncSetAttribute((const void*)k_i8_few<RT, TG, U, NW, FUSED, GATED>,
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
@@ -193,24 +220,28 @@ static void launch_few(const I8Args& a, hipStream_t stream) {
                        dim3(64 * NW), lds, stream, a);
 }
 
+template <int RT, int GATED>
+static void launch_rows(const I8Args& a, hipStream_t stream) {
+    if (a.T > 8)
+        launch_few<2, 2, 2, 8, 0, GATED>(a, stream);
+    else if (!a.x)
+        launch_few<RT, 1, 2, 8, 0, GATED>(a, stream);
+    else if (few_part(a.k, a.T) <= 512)  // (with the registers of more, fewer workgroups a CU)
+        launch_few<RT, 1, 2, FEW_FUSED_WAVES, 1, GATED>(a, stream);
+    else
+        launch_few<RT, 1, 2, FEW_FUSED_WAVES, FEW_PIECES, GATED>(a, stream);
+}
+
 // Rows of weights a workgroup: 8 for one or two tokens (14336 x 4096 at 1 token 12.5 us against 13.3 for 16, at 2
 // 14.4 against 15.0), else 16, which share the tokens' codes (at 8 tokens 17.7 against 19.0).  Two lines a
-// turn: with four the registers leave too few wavefronts (1 token, 8 rows, 15.3).  Long fused rows on 16
-// wavefronts, for the quantization's sake.
+// turn: with four the registers leave too few wavefronts (1 token, 8 rows, 15.3).
 static void launch_some(const I8Args& a, hipStream_t stream) {
-    const bool wide = a.x && a.k > 8192;
-    if (a.T > 8)
-        a.gated ? launch_few<2, 2, 2, 8, 0, 1>(a, stream) : launch_few<2, 2, 2, 8, 0, 0>(a, stream);
-    else if (a.gated && a.x)
-        wide ? launch_few<2, 1, 2, 16, 1, 1>(a, stream) : launch_few<2, 1, 2, 8, 1, 1>(a, stream);
-    else if (a.gated)
-        launch_few<2, 1, 2, 8, 0, 1>(a, stream);
-    else if (a.x)
-        wide ? launch_few<1, 1, 2, 16, 1, 0>(a, stream) : launch_few<1, 1, 2, 8, 1, 0>(a, stream);
+    if (a.gated)
+        launch_rows<2, 1>(a, stream);
     else if (a.T <= 2)
-        launch_few<1, 1, 2, 8, 0, 0>(a, stream);
+        launch_rows<1, 0>(a, stream);
     else
-        launch_few<2, 1, 2, 8, 0, 0>(a, stream);
+        launch_rows<2, 0>(a, stream);
 }
 
 // (any number of tokens, for weight rows that a tile's offsets do not reach: as many a launch as a grid holds)

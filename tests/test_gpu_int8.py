@@ -301,7 +301,8 @@ def test_refusals_on_the_device(I):
         with pytest.raises(I.GemvError):
             I.gemv(W, **{**dict(x=x, rows=4, y=y if "dtype" not in bad else None), **bad})
     with pytest.raises(I.SynError):
-        I.gemv(W, x, 4, y=y, ws=torch.empty(256, dtype=torch.uint8, device="cuda"))
+        I.gemv(W, torch.ones(20, 64, device="cuda"), 20, y=torch.empty(20, 8, device="cuda"),
+               ws=torch.empty(256, dtype=torch.uint8, device="cuda"))
     with pytest.raises(I.GemvError):
         I.gate_up_act(I.Weights(*make(9, 64, 1)), x, 4)
     for codes, scales in ((W.codes, W.scales[:7]), (W.codes, W.scales.double()), (W.codes.float(), W.scales),
