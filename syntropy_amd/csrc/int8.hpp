@@ -162,7 +162,7 @@ SYN_DEV void i8_tile_of(int id, int tiles_w, int tiles_t, int& tw, int& tt) {
 void launch_i8_quantize(int xtype, const void* x, uint64_t ldx, int rows, int k, int8_t* codes, uint64_t ldc,
                         float* scales, hipStream_t stream);
 // int8_few.hip: up to 16 tokens, weights straight to registers
-bool i8_few_fits(int T);
+bool i8_few_fits(int rows_w, int T);
 bool i8_few_fused(int rows_w, int k, int T);  // the kernel quantizes the rows itself
 void launch_i8_few(const I8Args& a, hipStream_t stream);
 // int8_gemm.hip: tiles through LDS, K in one part or several

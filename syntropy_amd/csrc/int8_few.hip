@@ -22,7 +22,6 @@
 
 namespace syn {
 
-constexpr int FEW_MAX_T = 16;
 // A fused row's values a wavefront, whole pieces of 8: at most four pieces a lane.
 constexpr int FEW_PIECES = 4, FEW_FUSED_WAVES = 8;
 constexpr uint64_t FEW_FUSED_MOST = 150000000;
@@ -199,7 +198,9 @@ __global__ __launch_bounds__(64 * NW, TG > 1 || U * RT > 4 ? 4 : 6) void k_i8_fe
     }
 }
 
-bool i8_few_fits(int T) { return T <= FEW_MAX_T; }
+// Up to 8 tokens; up to 16 over matrices that have too few tiles for the chip (4096 x 4096 at 16 tokens 7.5 us
+// against 9.5 in tiles, 6144 x 4096 11.0 against 7.9).
+bool i8_few_fits(int rows_w, int T) { return T <= 8 || (T <= 16 && rows_w <= 5120); }
 
 // One row, or as many as take each workgroup no longer than a launch (a value costs a workgroup's wavefronts
 // about eight operations), where the wavefronts' registers hold them.  4096 x 4096 at one row 6.7 us against 8.2

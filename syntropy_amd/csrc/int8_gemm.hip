@@ -323,7 +323,7 @@ static const TileOf TILES[] = {SYN_I8_TILES(SYN_I8_TILE)};
 
 // The tile and the parts of K that are estimated to take least: rounds of 256 workgroups, the last one's a
 // little faster the fewer there are in it, but no less than the weights take from HBM (4.9 TB/s beside
-// products, 36 GB/s a workgroup, and part of a reading more for every further tile of tokens); K in parts costs
+// products, 45 GB/s a workgroup, and part of a reading more for every further tile of tokens); K in parts costs
 // the fold's launch and its partial sums' writing and reading.  Large tiles read less from L2 for an output,
 // small ones fill the chip: 4096 x 4096 at 512 tokens takes 16 us in 256 tiles of 64 x 128 and 50 in 32 of 256
 // x 256, 14336 x 4096 at 2048 tokens 133 in 448 of 256 x 256 and 167 in 1792 of 128 x 128; 4096 x 14336 at 64
@@ -331,7 +331,7 @@ static const TileOf TILES[] = {SYN_I8_TILES(SYN_I8_TILE)};
 I8Pick i8_gemm_pick(int rows_w, int k, int T, int gated) {
     (void)gated;
     constexpr float LAUNCH = 3.0f, FOLD = 3.5f;                     // us
-    constexpr float HBM = 4.9e6f, EACH = 3.6e4f, SUMS = 4.0e6f;     // bytes a us
+    constexpr float HBM = 4.9e6f, EACH = 4.5e4f, SUMS = 4.0e6f;     // bytes a us
     const int kp = (int)i8_padded(k);
     I8Pick best{0, 1};
     float least = 0.0f;
@@ -345,7 +345,8 @@ I8Pick i8_gemm_pick(int rows_w, int k, int T, int gated) {
             const float last = (float)(wgs - 256 * (rounds - 1)) / 256.0f, turns = (float)rounds - 0.25f + 0.25f * last;
             const float work = (float)rounds * t.base + turns * t.per_k * (float)kp / (float)s;
             const float rate = EACH * (float)wgs < HBM ? EACH * (float)wgs : HBM;
-            float us = LAUNCH + (work > bytes / rate ? work : bytes / rate + 0.1f * work);
+            const float read = bytes / rate;
+            float us = LAUNCH + (work > read ? work + 0.25f * read : read + 0.25f * work);  // (they overlap in part)
             if (s > 1) us += FOLD + 8.0f * (float)s * (float)T * (float)rows_w / SUMS;
             if (least == 0.0f || us < least) {
                 least = us;
