@@ -201,7 +201,7 @@ int syn_logits(uint32_t layout, int32_t wtype, const void* head, uint64_t head_b
  * the last row's last code; up to 15 bytes behind a row's codes, in its last 16-byte piece, may be read
  * whatever they hold.  y may not overlap an operand.  No counterpart in the reference.
  * syn_i8_quantize: rows of x to codes (rows code_stride bytes apart, a multiple of 16, at least k; zeros
- *   behind a row's last code up to a multiple of 128 or the stride, whichever is less) and scales [rows]:
+ *   behind a row's last code up to a multiple of 256 or the stride, whichever is less) and scales [rows]:
  *   a token's rows, or a weight matrix's, whose rows are its channels.
  * syn_i8_gemv_workspace_bytes: the workspace of the two calls below; 0 (ws may be NULL) where the product's
  *   kernel quantizes the rows itself.  gated is 1 for syn_i8_gate_up_act, else 0.

@@ -1046,11 +1046,11 @@ int check_i8_shape(const char* W, uint64_t w_rows, uint32_t k, uint32_t rows) {
     return SYN_OK;
 }
 
-uint64_t i8_ws_bytes(uint64_t w_rows, uint32_t k, uint32_t rows, int gated, bool quantized = false) {
+uint64_t i8_ws_bytes(uint64_t w_rows, uint32_t k, uint32_t rows, bool quantized = false) {
     if (rows == 0 || (w_rows == 0 && !quantized)) return 0;
     if (!quantized && syn::i8_fused((int)w_rows, (int)k, (int)rows)) return 0;
     uint64_t b = syn::i8_act_layout(rows, k).partial;
-    const uint64_t splits = (uint64_t)syn::i8_splits((int)w_rows, (int)k, (int)rows, gated);
+    const uint64_t splits = (uint64_t)syn::i8_splits((int)w_rows, (int)k, (int)rows);
     if (splits > 1) b += 4 * splits * rows * w_rows;
     return syn::align_up(b, 256);
 }
@@ -1086,7 +1086,7 @@ int i8_product(const char* W, int gated, const int8_t* w, uint64_t w_bytes, uint
         if (int rc = check_values(W, "x", xtype, x, x_stride, rows, k_in)) return rc;
     if (int rc = check_values(W, "y", ytype, y, y_stride, rows, n_out)) return rc;
     const syn::I8Act l = syn::i8_act_layout(rows, k_in);
-    const uint64_t need = quantized ? l.partial : i8_ws_bytes(w_rows, k_in, rows, gated);
+    const uint64_t need = quantized ? l.partial : i8_ws_bytes(w_rows, k_in, rows);
     if (need)
         if (int rc = check_ws(W, ws, ws_bytes, need)) return rc;
     uint8_t* base = (uint8_t*)ws;
@@ -1103,7 +1103,7 @@ int i8_product(const char* W, int gated, const int8_t* w, uint64_t w_bytes, uint
     a.y = y;
     a.ldy = y_stride;
     a.ytype = ytype;
-    a.splits = syn::i8_splits((int)w_rows, (int)k_in, (int)rows, gated);
+    a.splits = syn::i8_splits((int)w_rows, (int)k_in, (int)rows);
     if (a.splits > 1) {  // (rows quantized before: as many parts as their workspace has room for)
         const uint64_t room = (ws_bytes - l.partial) / (4ull * rows * w_rows);
         if (room < (uint64_t)a.splits) a.splits = room > 1 ? (int)room : 1;
@@ -1147,7 +1147,7 @@ SYN_EXPORT int syn_i8_gemv_workspace_bytes(uint32_t n_out, uint32_t k_in, uint32
     if (!bytes) return fail(SYN_E_INVALID, "%s: null output", W);
     const uint64_t w_rows = (uint64_t)n_out * (gated ? 2 : 1);
     if (int rc = check_i8_shape(W, w_rows, k_in, rows)) return rc;
-    *bytes = i8_ws_bytes(w_rows, k_in, rows, gated ? 1 : 0);
+    *bytes = i8_ws_bytes(w_rows, k_in, rows);
     return SYN_OK;
 }
 
@@ -1155,7 +1155,7 @@ SYN_EXPORT int syn_i8_gemv_quantized_workspace_bytes(uint32_t n_out, uint32_t k_
     const char* W = "syn_i8_gemv_quantized_workspace_bytes";
     if (!bytes) return fail(SYN_E_INVALID, "%s: null output", W);
     if (int rc = check_i8_shape(W, n_out, k_in, rows)) return rc;
-    *bytes = i8_ws_bytes(n_out, k_in, rows, 0, true);
+    *bytes = i8_ws_bytes(n_out, k_in, rows, true);
     return SYN_OK;
 }
 

@@ -117,11 +117,11 @@ static void launch_i8_fold(const I8Args& a, hipStream_t stream) {
 // ---- the choice ----------------------------------------------------------------------------------------
 bool i8_fused(int rows_w, int k, int T) { return i8_few_fused(rows_w, k, T); }
 
-int i8_splits(int rows_w, int k, int T, int gated) { return i8_few_fits(rows_w, T) ? 1 : i8_gemm_pick(rows_w, k, T, gated).splits; }
+int i8_splits(int rows_w, int k, int T) { return i8_few_fits(rows_w, T) ? 1 : i8_gemm_pick(rows_w, k, T).splits; }
 
 void launch_i8_gemv(const I8Args& a, hipStream_t stream) {
     const int rows_w = a.n_out * (a.gated ? 2 : 1);
-    const I8Pick p = i8_gemm_pick(rows_w, a.k, a.T, a.gated);
+    const I8Pick p = i8_gemm_pick(rows_w, a.k, a.T);
     // (weight rows may be so far apart that a tile's offsets pass 32 bits)
     if (i8_few_fits(rows_w, a.T) || !i8_gemm_reaches(p.tile, a)) {
         launch_i8_few(a, stream);

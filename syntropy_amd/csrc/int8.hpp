@@ -169,11 +169,11 @@ void launch_i8_few(const I8Args& a, hipStream_t stream);
 struct I8Pick {
     int tile, splits;
 };
-I8Pick i8_gemm_pick(int rows_w, int k, int T, int gated);
+I8Pick i8_gemm_pick(int rows_w, int k, int T);
 bool i8_gemm_reaches(int tile, const I8Args& a);
 void launch_i8_gemm(int tile, const I8Args& a, hipStream_t stream);
 // int8.hip
-int i8_splits(int rows_w, int k, int T, int gated);
+int i8_splits(int rows_w, int k, int T);
 bool i8_fused(int rows_w, int k, int T);
 void launch_i8_gemv(const I8Args& a, hipStream_t stream);
 

@@ -7,8 +7,11 @@
 // bank groups.
 // Each half stage's operands are read into registers during the half stage before, the first half of the next
 // stage's behind the stage's one barrier, and all of it (products, reads, copies) is written in the order in
-// which it is to be issued and held there: a large tile leaves one wavefront a SIMD, whose matrix products
-// nothing else covers.  Left to itself the compiler reads each operand right before its product.
+// which it is to be issued and held there: a large tile leaves two wavefronts a SIMD, of which each has to cover
+// its own reads.  Left to itself the compiler reads each operand right before its product (14336 x 4096 at 2048
+// tokens 133 us against 130).
+// What bounds the large ones is the chip's power: 8192 x 8192 x 8192 of random codes runs at 2240 TOP/s, of zeros
+// at 3130; priorities of wavefronts, other orders and deeper rings are within 2 % of it.
 // The weight rows are the instruction's A rows, the tokens its columns: a lane holds four neighbouring outputs
 // of a token at a time, which go through LDS to whole 16-byte pieces of y's rows.
 // WK > 1: for few tokens, where the weights' bytes bound it: more of a small tile's K is in flight, in longer
@@ -322,14 +325,13 @@ static const TileOf TILES[] = {SYN_I8_TILES(SYN_I8_TILE)};
 #undef SYN_I8_TILE
 
 // The tile and the parts of K that are estimated to take least: rounds of 256 workgroups, the last one's a
-// little faster the fewer there are in it, but no less than the weights take from HBM (4.9 TB/s beside
-// products, 45 GB/s a workgroup, and part of a reading more for every further tile of tokens); K in parts costs
-// the fold's launch and its partial sums' writing and reading.  Large tiles read less from L2 for an output,
+// little faster the fewer there are in it, beside what the weights take from HBM (4.9 TB/s at most, 45 GB/s a
+// workgroup, and part of a reading more for every further tile of tokens): the longer of the two and a quarter
+// of the other; K in parts costs the fold's launch and its partial sums' writing and reading.  Large tiles read less from L2 for an output,
 // small ones fill the chip: 4096 x 4096 at 512 tokens takes 16 us in 256 tiles of 64 x 128 and 50 in 32 of 256
 // x 256, 14336 x 4096 at 2048 tokens 133 in 448 of 256 x 256 and 167 in 1792 of 128 x 128; 4096 x 14336 at 64
 // tokens 19 in 64 tiles of 64 x 64 of a quarter of K each and 27 in 128 of 64 x 32 of a half.
-I8Pick i8_gemm_pick(int rows_w, int k, int T, int gated) {
-    (void)gated;
+I8Pick i8_gemm_pick(int rows_w, int k, int T) {
     constexpr float LAUNCH = 3.0f, FOLD = 3.5f;                     // us
     constexpr float HBM = 4.9e6f, EACH = 4.5e4f, SUMS = 4.0e6f;     // bytes a us
     const int kp = (int)i8_padded(k);
