@@ -240,7 +240,7 @@ int syn_i8_logits(const int8_t* head, uint64_t head_bytes, uint64_t head_stride,
 
 /* ---- Log probabilities of given tokens -----------------------------------------------------------
  * For each row of logits x [rows, vocab] (F32, F16 or BF16, rows x_stride values apart; -infinity hides
- * a token), with z = x scale, a real number (scale: the inverse of a sampling temperature, finite and above 0):
+ * a token), with z = x scale, a real number (scale: the inverse of a sampling temperature, 2^-64 to 2^64):
  *   logprob [rows] F32: log softmax(z) at tokens[row];
  *   rank [rows] I32: how many of the row's logits are greater than the token's (0: none is);
  *   entropy [rows] F32: of softmax(z), in nats;
@@ -250,6 +250,7 @@ int syn_i8_logits(const int8_t* head, uint64_t head_bytes, uint64_t head_stride,
  * vocab or more gives NaN and -1.  Where every logit of a row is -infinity, its log probabilities are
  * -infinity and its entropy 0; a NaN or +infinity in it makes its log probabilities and its entropy NaN.
  * Among the greatest a NaN stands above +infinity; compared for the rank it is neither greater nor less.
+ * A logit whose distance from its row's greatest passes F32's range counts as -infinity but for rank and order.
  * Sums are held in F32 (rank: exact), in an order fixed by vocab and the number of rows.  Fewer than 2^24
  * rows of at most SYN_LOGPROBS_MAX_VOCAB logits.
  * ws: 256-byte aligned, syn_token_logprobs_workspace_bytes.  No counterpart in the reference. */

@@ -1253,7 +1253,8 @@ SYN_EXPORT int syn_token_logprobs(int32_t xtype, const void* x, uint64_t x_strid
     const char* W = "syn_token_logprobs";
     if (int rc = check_logprobs(W, xtype, rows, vocab, top)) return rc;
     if (token_bytes != 4 && token_bytes != 8) return fail(SYN_E_UNSUPPORTED, "%s: tokens of %u bytes (4 or 8)", W, token_bytes);
-    if (!(scale > 0.0f && scale < __builtin_inff())) return fail(SYN_E_INVALID, "%s: the scale %g is not finite and above 0", W, scale);
+    if (!(scale >= 0x1p-64f && scale <= 0x1p64f))  // (scale log2(e) is to be an ordinary number)
+        return fail(SYN_E_INVALID, "%s: the scale %g is not from 2^-64 to 2^64", W, scale);
     if (rows == 0) return SYN_OK;
     if (int rc = check_values(W, "x", xtype, x, x_stride, rows, vocab)) return rc;
     if (!tokens || !logprob || !rank || !entropy || (top && (!top_ids || !top_logprobs)))

@@ -298,7 +298,7 @@ class TokenLogprobs(NamedTuple):
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, scale: float = 1.0,
                    stream=None) -> TokenLogprobs:
     """Of each row of logits [rows, vocab] (F32, F16 or BF16; strided rows; -infinity hides a token), with z =
-    logits * scale (the inverse of a sampling temperature): log softmax(z) at tokens[row] (int32 or int64), the
+    logits * scale (the inverse of a sampling temperature, 2^-64 to 2^64): log softmax(z) at tokens[row] (int32 or int64), the
     number of logits greater than that token's, the entropy of softmax(z) in nats, and the `top` (0 to 64)
     greatest logits' indices, the lower one first among equals, with their log probabilities.
 

@@ -107,6 +107,21 @@ SIZES = [(1, 1, 1), (1, 2, 2), (3, 7, 5), (1, 64, 64), (2, 65, 20), (5, 100, 64)
          (300, 2000, 3), (700, 515, 10), (2100, 129, 2), (64, 20011, 17)]
 
 
+@pytest.mark.parametrize("scale", [2.0 ** -64, 2.0 ** -20, 2.0 ** 20, 2.0 ** 64])
+def test_scales_at_their_ends(S, scale):
+    x, t = logits(7, 3001, torch.float32, 5, 0.3)
+    check(S, x, t, 9, scale, "scale")
+    check(S, x * min(1 / scale, 2.0 ** 120), t, 9, scale, "scale, logits as far apart as before")
+
+
+def test_a_distance_past_f32_counts_as_hidden(S):
+    big = torch.finfo(torch.float32).max
+    x = torch.tensor([[big, -big, 0.0], [big, -big, 0.0]], device="cuda")
+    r = S.token_logprobs(x, torch.tensor([1, 0], device="cuda"), top=3, scale=2.0 ** -20)
+    assert r.logprob.tolist() == [-float("inf"), 0.0] and r.rank.tolist() == [2, 0] and r.entropy.tolist() == [0.0, 0.0]
+    assert r.top_ids.tolist() == [[0, 2, 1]] * 2 and r.top_logprobs[0].tolist() == [0.0, -big * 2.0 ** -20, -float("inf")]
+
+
 @pytest.mark.parametrize("rows,vocab,top", SIZES)
 def test_is_its_definition(S, rows, vocab, top):
     for i, (dt, scale) in enumerate(((torch.float32, 1.0), (torch.bfloat16, 0.7), (torch.float16, 1.3))):

@@ -104,6 +104,7 @@ def test_logits_refuse(o, code):
     (dict(ty=2), UNSUPPORTED), (dict(x=0), INVALID), (dict(x=A + 2), INVALID), (dict(xs=49), INVALID),
     (dict(tokens=0), INVALID), (dict(tokens=A + 4), INVALID), (dict(tb=2), UNSUPPORTED), (dict(scale=0.0), INVALID),
     (dict(scale=-1.0), INVALID), (dict(scale=float("nan")), INVALID), (dict(scale=float("inf")), INVALID),
+    (dict(scale=2.0 ** -65), INVALID), (dict(scale=2.0 ** 65), INVALID), (dict(scale=3e38), INVALID),
     (dict(top=51), UNSUPPORTED), (dict(vocab=100, xs=100, top=65), UNSUPPORTED), (dict(vocab=0), INVALID), (dict(vocab=(1 << 30) + 1, xs=1 << 31), UNSUPPORTED), (dict(rows=1 << 24), UNSUPPORTED),
     (dict(ids=0), INVALID), (dict(lps=0), INVALID), (dict(lps=A + 2), INVALID), (dict(lp=0), INVALID),
     (dict(rank=0), INVALID), (dict(ent=0), INVALID)])
