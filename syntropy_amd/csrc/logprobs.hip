@@ -416,15 +416,16 @@ __global__ __launch_bounds__(TOP ? 256 : 64) void k_logprobs_join(LogprobArgs g,
 
 // How a call runs: wavefronts a workgroup, parts of a row.  A workgroup of 16 wavefronts takes a whole row where
 // the rows are few and not long, or nearly fill the chip: one launch (64 rows of 32064, 64 greatest, 14.9 us
-// against 17.2 in parts; 256 rows of 128256 BF16 24.6 against 28.6; 24 rows of 128256 22.1 against 16.8).  Other
-// few and long rows are in parts, so that about 1024 workgroups of four keep reads in flight.
+// against 17.2 in parts; 256 rows of 128256 BF16 24.6 against 28.6, 145 F32 21.4 against 25.4; but 24 rows of
+// 128256 22.1 against 16.8, 145 of 250000 BF16 31.0 against 27.3).  Other few
+// and long rows are in parts, so that about 1024 workgroups of four keep reads in flight.
 struct LpPlan {
     int waves, parts, part_steps, group_steps;
 };
 static LpPlan lp_plan(int rows, int vocab) {
     const int steps = (vocab + LP_STEP - 1) / LP_STEP;
     LpPlan p{4, 1, 0, 0};
-    if (rows <= 256 && steps > 4 && (steps <= 64 || rows > 160)) {
+    if (rows <= 256 && steps > 4 && (steps <= 64 || rows > 160 || (rows > 110 && steps <= 160))) {
         p.waves = 16;
     } else if (steps > 32) {
         const int most = (steps + 3) / 4 < 64 ? (steps + 3) / 4 : 64;

@@ -104,7 +104,7 @@ def logits(rows, vocab, dtype, seed, hidden=0.0):
 
 SIZES = [(1, 1, 1), (1, 2, 2), (3, 7, 5), (1, 64, 64), (2, 65, 20), (5, 100, 64), (1, 1000, 0), (4, 1023, 1),
          (17, 4096, 5), (1, 8192, 20), (2, 8193, 33), (1, 32064, 20), (9, 50257, 64), (1, 128256, 8), (30, 32064, 64),
-         (300, 2000, 3), (700, 515, 10), (2100, 129, 2), (64, 20011, 17)]
+         (300, 2000, 3), (700, 515, 10), (2100, 129, 2), (64, 20011, 17), (130, 70001, 20)]
 
 
 @pytest.mark.parametrize("scale", [2.0 ** -64, 2.0 ** -20, 2.0 ** 20, 2.0 ** 64])
