@@ -208,7 +208,8 @@ int syn_logits(uint32_t layout, int32_t wtype, const void* head, uint64_t head_b
  * syn_i8_gemv: the product, W [n_out, k_in] to y [rows, n_out] (F32, F16 or BF16, rows y_stride values
  *   apart).
  * syn_i8_gate_up_act: W [2 n_out, k_in] holds gate rows, then up rows: y = silu(g) u of the two F32
- *   values, silu(g) = g / (1 + exp(-g)) within four steps of F32, the product rounded once more to y's type.
+ *   values, silu(g) = g / (1 + exp(-g)) within 2^-21 of its value and, where that is subnormal, 2^-150 (a NaN at
+ *   -infinity, as the formula), the product rounded to F32, then to y's type.
  * syn_i8_act_quantize, then syn_i8_gemv_quantized: the product's two halves over a workspace of
  *   syn_i8_gemv_quantized_workspace_bytes, for several matrices on the same rows (one whose products share it one
  *   after another; of the largest workspace of them, else K may be split less, to the same values).

@@ -135,16 +135,20 @@ SYN_DEV uint2 i8_codes8(const float (&v)[8], float inv) {
 // rounding is the conversion's.
 SYN_DEV float i8_value(int sum, float sx, float sw) { return ((float)sum * sx) * sw; }
 
-// silu(g) = g / (1 + exp(-g)): the exponential as 2^t of the rounded product t = -g log2(e) and a factor for
-// what the rounding left, within a step; the reciprocal within a step.  Below -88, where the exponential
-// nears F32's end, the quotient is 0 (for a value below 2^-120); an infinite or NaN g is met in the product.
+// silu(g) = g / (1 + exp(-g)) within 2^-21 of its value, to F32's least subnormal: exp(-g) as 2^t of the rounded
+// product t = -g log2(e) and a factor for what that leaves, the rounding and what F32's log2(e) lacks (1.9e-8:
+// at g = -88 ten steps of the result).  Below -80 the power is taken 2^32 times less, beside which the 1 still
+// counts for nothing, and the quotient brought back by one product: v_rcp_f32 keeps few bits of a subnormal
+// result, and a quotient that is one rounds once.  Below -111 the power is infinite and the quotient 0 (a value
+// below 2^-150).  An infinite or NaN g is met in the product with g.
 SYN_DEV float i8_silu(float g) {
-    const float gc = __builtin_amdgcn_fmed3f(g, -88.0f, 100.0f);
-    const float t = gc * -1.44269504088896340736f;
-    const float r = __builtin_fmaf(gc, -1.44269504088896340736f, -t);
-    const float e0 = __builtin_amdgcn_exp2f(t);
-    const float e = __builtin_fmaf(e0, r * 0.69314718055994530942f, e0);
-    return g * __builtin_amdgcn_rcpf(g < -88.0f ? __builtin_inff() : 1.0f + e);
+    constexpr float LOG2E = 1.44269504088896340736f, LOG2E_REST = (float)(1.44269504088896340736 - (double)LOG2E);
+    const bool far = g < -80.0f;
+    const float gc = __builtin_amdgcn_fmed3f(g, -180.0f, 100.0f);
+    const float t = gc * -LOG2E;
+    const float r = __builtin_fmaf(gc, -LOG2E_REST, __builtin_fmaf(gc, -LOG2E, -t));
+    const float e = __builtin_amdgcn_exp2f(t + (far ? -32.0f : 0.0f)) * __builtin_fmaf(r, 0.69314718055994530942f, 1.0f);
+    return g * __builtin_amdgcn_rcpf(1.0f + e) * (far ? 0x1p-32f : 1.0f);
 }
 
 // Workgroups go to the 8 XCDs in turn.  Each XCD takes a run of neighbouring tiles, token tiles first within
