@@ -164,8 +164,9 @@ def logits(head: Weights, g: torch.Tensor, eps: float, x: torch.Tensor, rows: in
     y F32 [rows, vocab] = head x as gemv."""
     if not (x.is_cuda and x.dtype == torch.float32 and x.is_contiguous() and x.numel() >= rows * head.k_in):
         raise GemvError("Len", f"x must be a contiguous F32 device tensor of {rows * head.k_in} values")
-    if head.device != x.get_device() or g.device != x.device or g.dtype != torch.float32 or g.numel() != head.k_in:
-        raise GemvError("Len", f"g must hold {head.k_in} F32 values beside x and the head")
+    if not (head.device == x.get_device() and g.device == x.device and g.dtype == torch.float32 and g.is_contiguous()
+            and g.numel() == head.k_in):
+        raise GemvError("Len", f"g must be a contiguous F32 tensor of {head.k_in} values beside x and the head")
     if head.bias is not None:
         raise GemvError("Activations", "a head has no bias")
     if y is not None and not (y.device == x.device and y.dtype == torch.float32 and y.is_contiguous()
