@@ -2,6 +2,7 @@
 // a scale a token: shared geometry and device helpers.
 #pragma once
 
+#include <atomic>
 #include <type_traits>
 
 #include "common.hpp"
@@ -161,6 +162,17 @@ SYN_DEV void i8_tile_of(int id, int tiles_w, int tiles_t, int& tw, int& tt) {
     l -= gi * group;
     tt = t8 + l % in;
     tw = l / in;
+}
+
+// Before a launch of `kernel`: allows it so much dynamic LDS on the current device, whose attribute the limit is;
+// `said`, the kernel's own, holds a bit for each device that it was said to.  A refusal shows as the launch's error.
+inline void i8_allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& said) {
+    int device = 0;
+    if (hipGetDevice(&device) != hipSuccess) return;
+    const uint64_t bit = device < 64 ? 1ull << device : 0;  // (a device past those is told every time)
+    if (said.load(std::memory_order_acquire) & bit) return;
+    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess)
+        said.fetch_or(bit, std::memory_order_release);
 }
 
 void launch_i8_quantize(int xtype, const void* x, uint64_t ldx, int rows, int k, int8_t* codes, uint64_t ldc,

@@ -214,9 +214,8 @@ template <int RT, int TG, int U, int NW, int FUSED, int GATED>
 static void launch_few(const I8Args& a, hipStream_t stream) {
     const int lds = NW * RT * TG * 1024 + (FUSED ? 128 + a.T * ((int)i8_padded(a.k) + 16) : 0);
     const int per = 8 * (GATED ? 1 : RT);
-    static const hipError_t most = hipFuncSetAttribute((const void*)k_i8_few<RT, TG, U, NW, FUSED, GATED>,
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-    (void)most;  // a launch that the runtime refuses is reported by the caller
+    static std::atomic<uint64_t> said{0};
+    i8_allow_lds((const void*)k_i8_few<RT, TG, U, NW, FUSED, GATED>, 160 * 1024, said);
     hipLaunchKernelGGL((k_i8_few<RT, TG, U, NW, FUSED, GATED>), dim3((a.n_out + per - 1) / per, (a.T + 8 * TG - 1) / (8 * TG)),
                        dim3(64 * NW), lds, stream, a);
 }

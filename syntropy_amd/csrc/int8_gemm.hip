@@ -367,9 +367,8 @@ template <class C, int GATED, int TY>
 static void launch_as(const I8Args& a, hipStream_t stream) {
     const int bm = GATED ? C::BM / 2 : C::BM;
     const int tw = (a.n_out + bm - 1) / bm, tt = (a.T + C::BN - 1) / C::BN;
-    static const hipError_t lds =
-        hipFuncSetAttribute((const void*)k_i8_gemm<C, GATED, TY>, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
-    (void)lds;  // a launch that the runtime refuses is reported by the caller
+    static std::atomic<uint64_t> said{0};
+    i8_allow_lds((const void*)k_i8_gemm<C, GATED, TY>, C::LDS, said);
     hipLaunchKernelGGL((k_i8_gemm<C, GATED, TY>), dim3((uint32_t)tw * (uint32_t)tt, 1, a.splits), dim3(64 * C::NW), C::LDS,
                        stream, a, tw, tt);
 }

@@ -1,0 +1,28 @@
+"""How the int8 products' calls are launched, on the CPU (host_launches.py)."""
+import pytest
+
+import host_launches as H
+
+pytestmark = pytest.mark.skipif(H.MISSING, reason="needs the built library and ROCm's clang++")
+
+
+@pytest.fixture(scope="module")
+def exe(tmp_path_factory):
+    return H.build(tmp_path_factory.mktemp("launches"))
+
+
+def test_lds_is_allowed_on_every_device(exe):
+    """A kernel's limit of dynamic LDS is its device's: said on each device before the first launch there."""
+    calls = [f"i8 {gated} {n} {k} {rows} {H.BF16} {H.F32} 0" for gated in (0, 1)
+             for n, k, rows in ((512, 512, 1), (512, 512, 6), (512, 16384, 1), (512, 512, 12), (4096, 4096, 20), (4096, 4096, 100),
+                                (14336, 1024, 2048), (1000, 8192, 100))]
+    for device in (0, 1, 7, 0, 200):
+        calls += [f"device {device}"] + calls[:16]
+    seen = set()
+    for c, answer in zip(calls, H.run(exe, calls)):
+        assert answer[-1] == "rc 0", c
+        for device, lds, limit, name in H.launches(answer):
+            if lds > 65536:
+                seen.add((device, name))
+                assert limit >= lds, f"{c}: {name} asks for {lds} bytes of LDS on device {device}, allowed {limit}"
+    assert {d for d, _ in seen} == {0, 1, 7, 200} and len(seen) >= 4 * 4
