@@ -338,6 +338,7 @@ I8Pick i8_gemm_pick(int rows_w, int k, int T) {
     constexpr float HBM = 4.9e6f, EACH = 4.5e4f, SUMS = 4.0e6f;     // bytes a us
     const int kp = (int)i8_padded(k);
     I8Pick best{0, 1};
+    if (rows_w == 0) return best;  // nothing to estimate (0 / 0)
     float least = 0.0f;
     for (int i = 0; i < (int)(sizeof TILES / sizeof TILES[0]); ++i) {
         const TileOf& t = TILES[i];

@@ -26,3 +26,14 @@ def test_lds_is_allowed_on_every_device(exe):
                 seen.add((device, name))
                 assert limit >= lds, f"{c}: {name} asks for {lds} bytes of LDS on device {device}, allowed {limit}"
     assert {d for d, _ in seen} == {0, 1, 7, 200} and len(seen) >= 4 * 4
+
+
+@pytest.mark.parametrize("rows", [0, 1, 17, 2097120])
+@pytest.mark.parametrize("k", [1, 1000, 131072])
+def test_a_matrix_without_rows_needs_its_tokens_alone(exe, k, rows):
+    """No estimate is made of no weights (0 / 0), and nothing is launched."""
+    need, call = H.run(exe, [f"need 0 {k} {rows}", f"i8q 0 {k} {rows} {H.F32}"])
+    bytes_, invalid = need[0].split()[1:]
+    assert need[-1] == call[-1] == "rc 0" and not H.launches(call)
+    assert int(bytes_) >= rows * (k + 4) and (int(bytes_) == 0) == (rows == 0)
+    assert invalid == "0", "the host's arithmetic raised the invalid-operation flag"
