@@ -37,3 +37,14 @@ def test_a_matrix_without_rows_needs_its_tokens_alone(exe, k, rows):
     assert need[-1] == call[-1] == "rc 0" and not H.launches(call)
     assert int(bytes_) >= rows * (k + 4) and (int(bytes_) == 0) == (rows == 0)
     assert invalid == "0", "the host's arithmetic raised the invalid-operation flag"
+
+
+def test_the_cases_of_the_device_tests_reach_every_kernel(exe):
+    """test_gpu_int8_tiles.py's: each form of each kernel, in each output type, is launched by one of them."""
+    from test_gpu_int8_tiles import CASES
+    kernels = {line[len("kernel "):] for line in H.run(exe, ["kernels"])[0] if "syn::k_i8_" in line}
+    assert sum("k_i8_gemm" in k for k in kernels) >= 64
+    calls = [f"i8 {gated} {n} {k} {rows} {t} {t} {int(t == H.BF16)}" for gated, n, k, rows in CASES for t in (H.F32, H.F16, H.BF16)]
+    calls += [f"i8quantize {k} {rows} {t}" for rows, k in ((257, 5001), (301, 9001)) for t in (H.F32, H.F16, H.BF16)]
+    run = {name for answer in H.run(exe, calls) for *_, name in H.launches(answer)}
+    assert kernels <= run, "not launched: " + ", ".join(sorted(kernels - run))
