@@ -1097,8 +1097,10 @@ int i8_product(const char* W, int gated, const int8_t* w, uint64_t w_bytes, uint
     a.bias = bias;
     a.n_out = (int)n_out;
     a.k = (int)k_in;
-    a.xq = (const int8_t*)base;
-    a.xs = (const float*)(base + l.scales);
+    if (need) {  // (rows quantized in the product's workgroups are held nowhere)
+        a.xq = (const int8_t*)base;
+        a.xs = (const float*)(base + l.scales);
+    }
     a.T = (int)rows;
     a.y = y;
     a.ldy = y_stride;

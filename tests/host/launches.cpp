@@ -8,6 +8,9 @@
 //   i8 GATED N K ROWS XTYPE YTYPE BIAS       syn_i8_gemv, or syn_i8_gate_up_act over 2 N rows
 //   i8q N K ROWS YTYPE                       syn_i8_gemv_quantized with the largest workspace it asks for
 //   i8quantize K ROWS XTYPE                  syn_i8_quantize
+//   i8act K ROWS XTYPE                       syn_i8_act_quantize
+//   i8logits VOCAB HIDDEN ROWS               syn_i8_logits
+//   logprobs XTYPE ROWS VOCAB TOP BYTES      syn_token_logprobs, tokens of BYTES bytes
 //   need N K ROWS                            syn_i8_gemv_quantized_workspace_bytes: "need BYTES INVALID", the latter 1 where
 //                                            the host's arithmetic raised the invalid-operation flag
 // A launch: "launch DEVICE LDS LIMIT NAME", LIMIT the dynamic LDS allowed on that device for it (-1: never said).
@@ -107,18 +110,37 @@ int main() {
             uint64_t need = 0;
             rc = syn_i8_gemv_workspace_bytes(n, k, rows, static_cast<int>(v.at(0)), &need);
             if (rc == 0)
-                rc = call(w, all, (k + 15) / 16 * 16, scales, v.at(6) ? scales : nullptr, n, k, static_cast<int>(v.at(4)), A, k,
+                rc = call(w, all, (uint64_t(k) + 15) / 16 * 16, scales, v.at(6) ? scales : nullptr, n, k, static_cast<int>(v.at(4)), A, k,
                           rows, static_cast<int>(v.at(5)), A, n, need ? A : nullptr, need, nullptr);
         } else if (what == "i8q") {
             const uint32_t n = v.at(0), k = v.at(1), rows = v.at(2);
             uint64_t need = 0;
             rc = syn_i8_gemv_quantized_workspace_bytes(n, k, rows, &need);
             if (rc == 0)
-                rc = syn_i8_gemv_quantized(w, all, (k + 15) / 16 * 16, scales, nullptr, n, k, rows, static_cast<int>(v.at(3)), A, n,
+                rc = syn_i8_gemv_quantized(w, all, (uint64_t(k) + 15) / 16 * 16, scales, nullptr, n, k, rows, static_cast<int>(v.at(3)), A, n,
                                            A, need, nullptr);
         } else if (what == "i8quantize") {
             rc = syn_i8_quantize(static_cast<int>(v.at(2)), A, v.at(0), v.at(1), v.at(0), static_cast<int8_t*>(A),
-                                 (v.at(0) + 127) / 128 * 128, static_cast<float*>(A), nullptr);
+                                 (uint64_t(v.at(0)) + 127) / 128 * 128, static_cast<float*>(A), nullptr);
+        } else if (what == "i8act") {
+            uint64_t need = 0;
+            rc = syn_i8_gemv_quantized_workspace_bytes(1, v.at(0), v.at(1), &need);
+            if (rc == 0) rc = syn_i8_act_quantize(static_cast<int>(v.at(2)), A, v.at(0), v.at(1), v.at(0), A, need, nullptr);
+        } else if (what == "i8logits") {
+            const uint32_t n = v.at(0), k = v.at(1), rows = v.at(2);
+            uint64_t need = 0;
+            rc = syn_i8_logits_workspace_bytes(n, k, rows, &need);
+            if (rc == 0)
+                rc = syn_i8_logits(w, all, (uint64_t(k) + 15) / 16 * 16, scales, n, k, scales, 1e-5f, scales, rows,
+                                   static_cast<float*>(A), A, need, nullptr);
+        } else if (what == "logprobs") {
+            const uint32_t rows = v.at(1), vocab = v.at(2), top = v.at(3);
+            uint64_t need = 0;
+            rc = syn_token_logprobs_workspace_bytes(static_cast<int>(v.at(0)), rows, vocab, top, &need);
+            if (rc == 0)
+                rc = syn_token_logprobs(static_cast<int>(v.at(0)), A, vocab, rows, vocab, A, v.at(4), 1.0f, top,
+                                        static_cast<float*>(A), static_cast<int32_t*>(A), static_cast<float*>(A),
+                                        static_cast<int32_t*>(A), static_cast<float*>(A), need ? A : nullptr, need, nullptr);
         } else if (what == "need") {
             uint64_t need = 0;
             std::feclearexcept(FE_ALL_EXCEPT);

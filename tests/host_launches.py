@@ -12,18 +12,19 @@ MISSING = not (os.path.exists(CLANG) and os.path.exists(_lib.LIB_PATH))
 F32, F16, BF16 = 0, 1, 30
 
 
-def build(out_dir) -> str:
-    exe, where = os.path.join(str(out_dir), "launches"), os.path.dirname(_lib.LIB_PATH)
-    subprocess.run([CLANG, "-std=c++17", "-O1", "-Wall", os.path.join(HERE, "host", "launches.cpp"), "-o", exe, f"-L{where}",
+def build(out_dir, where=os.path.dirname(_lib.LIB_PATH), flags=()) -> str:
+    """The program over the library in `where`, into out_dir."""
+    exe = os.path.join(str(out_dir), "launches")
+    subprocess.run([CLANG, "-std=c++17", "-O1", "-Wall", *flags, os.path.join(HERE, "host", "launches.cpp"), "-o", exe, f"-L{where}",
                     "-l:libsyntropy_hip.so", f"-Wl,-rpath,{where}", "-Wl,--allow-shlib-undefined", "-rdynamic"], check=True, capture_output=True,
                    text=True)
     return exe
 
 
-def run(exe: str, commands) -> list[list[str]]:
+def run(exe: str, commands, env=None) -> list[list[str]]:
     """The answers' lines of each command, its "rc" last."""
-    r = subprocess.run([exe], input="\n".join(commands) + "\n", capture_output=True, text=True, timeout=120)
-    assert r.returncode == 0, r.stderr[-2000:]
+    r = subprocess.run([exe], input="\n".join(commands) + "\n", capture_output=True, text=True, timeout=300, env=env)
+    assert r.returncode == 0 and not r.stderr, r.stderr[-6000:]
     out, at = [], []
     for line in r.stdout.splitlines():
         at.append(line)
