@@ -141,7 +141,8 @@ SYN_DEV float i8_value(int sum, float sx, float sw) { return ((float)sum * sx) *
 // at g = -88 ten steps of the result).  Below -80 the power is taken 2^32 times less, beside which the 1 still
 // counts for nothing, and the quotient brought back by one product: v_rcp_f32 keeps few bits of a subnormal
 // result, and a quotient that is one rounds once.  Below -111 the power is infinite and the quotient 0 (a value
-// below 2^-150).  An infinite or NaN g is met in the product with g.
+// below 2^-150).  An infinite or NaN g is met in the product with g.  (14336 x 4096 gated at 1024 tokens 138.7 us;
+// 137.2 with neither the rest of log2(e) nor the values below -88.)
 SYN_DEV float i8_silu(float g) {
     constexpr float LOG2E = 1.44269504088896340736f, LOG2E_REST = (float)(1.44269504088896340736 - (double)LOG2E);
     const bool far = g < -80.0f;

@@ -308,7 +308,7 @@ __global__ __launch_bounds__(64 * C::NW, C::MT* C::NT >= 16 ? 1 : 2) void k_i8_g
 // microsecond (product alone, 256 workgroups: 4096 x 4096 and 4096 x 14336 matrices at 128 to 2048 tokens).
 // Every tile's ring leaves room for one workgroup a CU.
 // Of 41 calls over matrices of 1024 to 32064 rows at 17 to 3900 tokens 36 run on the fastest tile, the others within
-// 7 % of it.
+// 8 % of it (profiles/int8_products_and_token_logprobs.md).
 #define SYN_I8_TILES(X)              \
     X(0, 4, 2, 1, 2, 4, 4, 50, 147)  \
     X(1, 4, 2, 1, 2, 2, 4, 27, 100)  \

@@ -116,14 +116,15 @@ def _launch(name, gated, w, n, x, ty, xs, rows, y, ws, dtype, handle):
 def gemv(w: Weights, x: torch.Tensor, rows: int, y: torch.Tensor | None = None, ws: torch.Tensor | None = None,
          dtype: torch.dtype | None = None, stream=None) -> torch.Tensor:
     """y [rows, n_out] = x W^T (+ bias) for the first `rows` rows of x [., k_in], of x's type, y's or
-    `dtype` (F32, F16, BF16).  x and y may have strided rows."""
+    `dtype` (F32, F16, BF16).  x and y may have strided rows; no value of y lies in x or another operand."""
     return _product("syn_i8_gemv", 0, w, w.n_out, x, rows, y, ws, dtype, stream)
 
 
 def gate_up_act(w: Weights, x: torch.Tensor, rows: int, y: torch.Tensor | None = None, ws: torch.Tensor | None = None,
                 dtype: torch.dtype | None = None, stream=None) -> torch.Tensor:
     """GateUpAct{Silu} over a stacked matrix (gate rows, then up rows: w.n_out = 2 n): y [rows, n] =
-    silu(gate x) * (up x), both products the F32 values of gemv."""
+    silu(gate x) * (up x), both products the F32 values of gemv, silu(g) = g / (1 + exp(-g)) within 2^-21 of its
+    value (a NaN at -infinity).  Operands as gemv's."""
     if w.n_out % 2:
         raise GemvError("Len", f"a stacked gate/up matrix has an even row count, not {w.n_out}")
     return _product("syn_i8_gate_up_act", 1, w, w.n_out // 2, x, rows, y, ws, dtype, stream)
@@ -161,7 +162,7 @@ def gemv_quantized(w: Weights, r: Rows, y: torch.Tensor, stream=None) -> torch.T
 def logits(head: Weights, g: torch.Tensor, eps: float, x: torch.Tensor, rows: int, y: torch.Tensor | None = None,
            stream=None) -> torch.Tensor:
     """Logits over an int8 head: each F32 row of x [., hidden] normalised by (g, eps) as gemv.rms_norm, then
-    y F32 [rows, vocab] = head x as gemv."""
+    y F32 [rows, vocab] = head x as gemv.  x, g and y hold their values side by side."""
     if not (x.is_cuda and x.dtype == torch.float32 and x.is_contiguous() and x.numel() >= rows * head.k_in):
         raise GemvError("Len", f"x must be a contiguous F32 device tensor of {rows * head.k_in} values")
     if not (head.device == x.get_device() and g.device == x.device and g.dtype == torch.float32 and g.is_contiguous()
