@@ -263,6 +263,74 @@ int syn_token_logprobs(int32_t xtype, const void* x, uint64_t x_stride, uint32_t
                        int32_t* rank, float* entropy, int32_t* top_ids, float* top_logprobs, void* ws,
                        uint64_t ws_bytes, void* stream);
 
+/* ---- Products over half-precision weights with an epilogue ---------------------------------------
+ * y = act(x W^T + bias) gate + residual over W [n_out, k_in] and x [rows, k_in] of wtype (SYN_F16 or SYN_BF16):
+ * products of the values as they are, sums in F32 (in an order that depends on n_out, k_in and rows alone), then the
+ * epilogue in F32, rounded once, to y's type.  syn_gemv over F16 and BF16 weights is the product of F32 activations in the
+ * reference's order; this one has no counterpart there.
+ *   act: SYN_ACT_*: none, relu, silu(v) = v / (1 + exp(-v)), gelu(v) = v Phi(v), and its tanh form
+ *     v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2;
+ *   bias F32 [n_out], gate and residual [rows, n_out] (F32, F16 or BF16): each may be NULL.
+ * W's rows are w_stride values apart, a multiple of 8, each on 16 bytes and followed by ZEROS up to a multiple of 64
+ * values (w_stride is at least that, and the view w_bytes reaches the last row's).  Rows of x, gate, residual and y
+ * are x_stride, ... values apart, at any value's address; x's are read as they lie where k_in is a multiple of 64,
+ * x on 16 bytes and x_stride a multiple of 8 (x_aligned in the workspace's query: 1 for that, 0 for any), else through
+ * a copy in the workspace.  residual or gate may be y itself (address, stride and type); y overlaps no operand
+ * otherwise.  At most SYN_HALF_MAX_ROWS rows and 2^24 - 1 weight rows.  ws: 256-byte aligned. */
+#define SYN_ACT_NONE 0
+#define SYN_ACT_RELU 1
+#define SYN_ACT_SILU 2
+#define SYN_ACT_GELU 3
+#define SYN_ACT_GELU_TANH 4
+#define SYN_HALF_MAX_K (1 << 20)
+#define SYN_HALF_MAX_ROWS 2097120
+int syn_half_gemv_workspace_bytes(uint32_t n_out, uint32_t k_in, uint32_t rows, int32_t x_aligned, uint64_t* bytes);
+int syn_half_gemv(int32_t wtype, const void* w, uint64_t w_bytes, uint64_t w_stride, const float* bias, uint32_t n_out,
+                  uint32_t k_in, const void* x, uint64_t x_stride, uint32_t rows, int32_t act, int32_t gtype,
+                  const void* gate, uint64_t gate_stride, int32_t rtype, const void* residual, uint64_t r_stride,
+                  int32_t ytype, void* y, uint64_t y_stride, void* ws, uint64_t ws_bytes, void* stream);
+
+/* ---- The norms between two blocks ------------------------------------------------------------------
+ * For each of `rows` rows of n values (1 to SYN_BLOCK_NORM_MAX_COLS), rms(v; g) = v g / sqrt(mean v^2 + eps):
+ *   a = rms(branch; post), or branch where post is NULL
+ *   h = x + scale gate a                     (gate NULL: 1)
+ *   y = rms(h; g)                            (g NULL: none)
+ * in F32, each of h and y rounded once (y's norm takes the h that is not rounded).  x and h, the residual stream, are of
+ * xtype; branch and gate of btype; y of ytype (F32, F16 or BF16 each); post and g F32 [n].  gate has a row a row, or
+ * with gate_stride 0 one for all.  With branch NULL h is x and not written.  Rows are *_stride values apart, at any
+ * value's address.  h may be x itself (address and stride); h and y overlap no operand otherwise.  Fewer than 2^24
+ * rows.  syn_rms_norm is the norm in the reference's order of sums; this has no counterpart there. */
+#define SYN_BLOCK_NORM_MAX_COLS 32768
+int syn_block_norm(int32_t xtype, const void* x, uint64_t x_stride, int32_t btype, const void* branch, uint64_t b_stride,
+                   const float* post, const void* gate, uint64_t gate_stride, float scale, const float* g, float eps,
+                   uint32_t rows, uint32_t n, void* h, uint64_t h_stride, int32_t ytype, void* y, uint64_t y_stride,
+                   void* stream);
+
+/* ---- Sampling ------------------------------------------------------------------------------------
+ * A token of each row of logits x [rows, vocab] (F32, F16 or BF16, rows x_stride values apart; -infinity hides a
+ * token) by a temperature T, top-k, top-p, min-p and a number u [rows] F32 in [0, 1).  A row's visible logits stand
+ * in order (descending, the lower index first among equals), w = exp((x - max x) / T), a real number:
+ *   top-k: the first k (0: all);
+ *   top-p: of those the least number whose sum of w reaches p times the sum of them (1: all);
+ *   min-p: of those the ones with w >= min_p (0: all).
+ * Of the n that are left, W the sum of their w, the token is the first whose running sum passes u W.
+ *   token [rows] I32; logprob [rows] F32: log(w / W) of it; kept [rows] I32: n.
+ * T = 0 takes the greatest logit (top-k 1).  A setting is a number for all rows, or, where its pointer is not NULL, a
+ * value a row: temperatures F32 (0, or 2^-64 to 2^64), top_ks I32, top_ps F32 (above 0), min_ps F32 (0 to 1).  As
+ * numbers others are refused; a row's top_k below 0 counts as 0, top_p above 1 as 1 and not above 0 as the
+ * least above it, min_p below 0 as 0 and above 1 as 1; u outside [0, 1) as the nearest in it.  A row with a NaN or
+ * +infinity among its logits, with no visible logit, or with a NaN setting, u, or a temperature that is none of the
+ * above has the token -1, kept 0 and logprob NaN.
+ * Sums are held to about 2^-62 vocab of a weight, in an order that does not matter: equal calls give equal tokens.
+ * Weights below 2^-64 of the greatest count as 0.  Fewer than 2^24 rows of at most SYN_SAMPLE_MAX_VOCAB logits.
+ * ws: 256-byte aligned, syn_sample_tokens_workspace_bytes (0: may be NULL).  No counterpart in the reference. */
+#define SYN_SAMPLE_MAX_VOCAB (1 << 24)
+int syn_sample_tokens_workspace_bytes(int32_t xtype, uint32_t rows, uint32_t vocab, uint64_t* bytes);
+int syn_sample_tokens(int32_t xtype, const void* x, uint64_t x_stride, uint32_t rows, uint32_t vocab, const float* u,
+                      const float* temperatures, const int32_t* top_ks, const float* top_ps, const float* min_ps,
+                      float temperature, int32_t top_k, float top_p, float min_p, int32_t* token, float* logprob,
+                      int32_t* kept, void* ws, uint64_t ws_bytes, void* stream);
+
 /* ---- Prefill GEMM ---------------------------------------------------------------------------
  * Q4_K weights times many activation rows on the matrix cores, each output bit-identical to
  * syn_gemv (which takes this path itself for Q4_K calls of 32 rows or more).  The reference

@@ -79,6 +79,14 @@ def lib():
         "syn_i8_logits": [vp, u64, u64, vp, u32, u32, vp, C.c_float, vp, u32, vp, vp, u64, vp],
         "syn_token_logprobs_workspace_bytes": [i32, u32, u32, u32, C.POINTER(C.c_uint64)],
         "syn_token_logprobs": [i32, vp, u64, u32, u32, vp, u32, C.c_float, u32, vp, vp, vp, vp, vp, vp, u64, vp],
+        "syn_half_gemv_workspace_bytes": [u32, u32, u32, i32, C.POINTER(C.c_uint64)],
+        "syn_half_gemv": [i32, vp, u64, u64, vp, u32, u32, vp, u64, u32, i32, i32, vp, u64, i32, vp, u64, i32, vp, u64, vp, u64,
+                          vp],
+        "syn_block_norm": [i32, vp, u64, i32, vp, u64, vp, vp, u64, C.c_float, vp, C.c_float, u32, u32, vp, u64, i32, vp, u64,
+                           vp],
+        "syn_sample_tokens_workspace_bytes": [i32, u32, u32, C.POINTER(C.c_uint64)],
+        "syn_sample_tokens": [i32, vp, u64, u32, u32, vp, vp, vp, vp, vp, C.c_float, i32, C.c_float, C.c_float, vp, vp, vp, vp, u64,
+                              vp],
         "syn_moe_route": [vp, vp, u32, u32, u32, u32, i32, vp, vp, vp, vp],
         "syn_moe_pack": [vp, u32, u32, u32, vp, vp, vp, vp],
         "syn_moe_grouped_workspace_bytes": [i32, u32, u32, u32, u32, u32, C.POINTER(C.c_uint64)],

@@ -9,6 +9,7 @@
 
 #include "../../include/syntropy_hip.h"
 #include "capi_rows.hpp"
+#include "half.hpp"
 #include "int8.hpp"
 #include "kernels.hpp"
 
@@ -1270,6 +1271,162 @@ SYN_EXPORT int syn_token_logprobs(int32_t xtype, const void* x, uint64_t x_strid
     const syn::LogprobArgs a{x, x_stride, xtype, (int)rows, (int)vocab, tokens, token_bytes == 8, scale, (int)top,
                              logprob, rank, entropy, top_ids, top_logprobs, (uint8_t*)ws};
     syn::launch_logprobs(a, (hipStream_t)stream);
+    return check_launch(W);
+}
+
+// ---- half-precision products with an epilogue, the norms between blocks, sampling ---------------------
+
+namespace {
+
+int check_half_shape(const char* W, uint32_t n_out, uint32_t k, uint32_t rows) {
+    if (k == 0 || k > SYN_HALF_MAX_K) return fail(SYN_E_UNSUPPORTED, "%s: rows of %u values (1 to %d)", W, k, SYN_HALF_MAX_K);
+    if (n_out >= 1u << 24 || rows > SYN_HALF_MAX_ROWS)  // what a launch's grid holds
+        return fail(SYN_E_UNSUPPORTED, "%s: %u weight rows (below 2^24), %u rows (at most %d)", W, n_out, rows, SYN_HALF_MAX_ROWS);
+    return SYN_OK;
+}
+static_assert(SYN_HALF_MAX_K == syn::HALF_MAX_K, "the header's limit");
+static_assert(SYN_BLOCK_NORM_MAX_COLS == syn::BLOCK_NORM_MAX_COLS, "the header's limit");
+
+// Whether the rows of x are whole 128-byte lines on 16 bytes, as the product's kernels read them.
+bool half_lines(const void* x, uint64_t stride, uint32_t rows, uint32_t k) {
+    return k % syn::HALF_LINE == 0 && aligned(x, 16) && (rows <= 1 || stride % 8 == 0);
+}
+
+}  // namespace
+
+SYN_EXPORT int syn_half_gemv_workspace_bytes(uint32_t n_out, uint32_t k_in, uint32_t rows, int32_t x_aligned, uint64_t* bytes) {
+    const char* W = "syn_half_gemv_workspace_bytes";
+    if (!bytes) return fail(SYN_E_INVALID, "%s: null output", W);
+    if (int rc = check_half_shape(W, n_out, k_in, rows)) return rc;
+    *bytes = rows && n_out ? syn::half_ws_bytes((int)n_out, (int)k_in, (int)rows, x_aligned && k_in % syn::HALF_LINE == 0) : 0;
+    return SYN_OK;
+}
+
+SYN_EXPORT int syn_half_gemv(int32_t wtype, const void* w, uint64_t w_bytes, uint64_t w_stride, const float* bias, uint32_t n_out,
+                             uint32_t k_in, const void* x, uint64_t x_stride, uint32_t rows, int32_t act, int32_t gtype,
+                             const void* gate, uint64_t gate_stride, int32_t rtype, const void* residual, uint64_t r_stride,
+                             int32_t ytype, void* y, uint64_t y_stride, void* ws, uint64_t ws_bytes, void* stream) {
+    const char* W = "syn_half_gemv";
+    if (!float_type(wtype)) return fail(SYN_E_UNSUPPORTED, "%s: weights of type %d are not F16 or BF16", W, wtype);
+    if (int rc = check_half_shape(W, n_out, k_in, rows)) return rc;
+    if (act < SYN_ACT_NONE || act > SYN_ACT_GELU_TANH) return fail(SYN_E_UNSUPPORTED, "%s: activation %d", W, act);
+    if (rows == 0 || n_out == 0) return SYN_OK;
+    if (!w || !aligned(w, 16) || w_stride % 8)
+        return fail(SYN_E_INVALID, "%s: the weight rows must be on 16 bytes (stride %llu)", W, (unsigned long long)w_stride);
+    const uint64_t row = syn::half_padded(k_in);
+    if (w_stride < row || w_stride > (1ull << 30))
+        return fail(SYN_E_INVALID, "%s: weight rows of %llu values, zeros included, %llu apart", W, (unsigned long long)row,
+                    (unsigned long long)w_stride);
+    if (w_bytes < 2 * ((n_out - 1) * w_stride + row))
+        return fail(SYN_E_INVALID, "%s: the weight view holds %llu bytes, the matrix %llu", W, (unsigned long long)w_bytes,
+                    (unsigned long long)(2 * ((n_out - 1) * w_stride + row)));
+    if (bias && !aligned(bias, 4)) return fail(SYN_E_INVALID, "%s: the bias must be 4-byte aligned", W);
+    if (int rc = check_values(W, "x", wtype, x, x_stride, rows, k_in)) return rc;
+    if (gate)
+        if (int rc = check_values(W, "gate", gtype, gate, gate_stride, rows, n_out)) return rc;
+    if (residual)
+        if (int rc = check_values(W, "residual", rtype, residual, r_stride, rows, n_out)) return rc;
+    if (int rc = check_values(W, "y", ytype, y, y_stride, rows, n_out)) return rc;
+    const bool lines = half_lines(x, x_stride, rows, k_in);
+    const uint64_t need = syn::half_ws_bytes((int)n_out, (int)k_in, (int)rows, lines);
+    if (need)
+        if (int rc = check_ws(W, ws, ws_bytes, need)) return rc;
+    syn::HalfArgs a{};
+    a.wtype = wtype;
+    a.w = (const uint16_t*)w;
+    a.ldw = w_stride;
+    a.bias = bias;
+    a.n_out = (int)n_out;
+    a.k = (int)k_in;
+    a.x = (const uint16_t*)x;
+    a.ldx = x_stride;
+    a.T = (int)rows;
+    a.act = act;
+    a.gate = gate;
+    a.ldg = gate_stride;
+    a.gtype = gtype;
+    a.res = residual;
+    a.ldr = r_stride;
+    a.rtype = rtype;
+    a.y = y;
+    a.ldy = y_stride;
+    a.ytype = ytype;
+    syn::launch_half_gemv(a, lines, (uint8_t*)ws, (hipStream_t)stream);
+    return check_launch(W);
+}
+
+SYN_EXPORT int syn_block_norm(int32_t xtype, const void* x, uint64_t x_stride, int32_t btype, const void* branch, uint64_t b_stride,
+                              const float* post, const void* gate, uint64_t gate_stride, float scale, const float* g, float eps,
+                              uint32_t rows, uint32_t n, void* h, uint64_t h_stride, int32_t ytype, void* y, uint64_t y_stride,
+                              void* stream) {
+    const char* W = "syn_block_norm";
+    if (n == 0 || n > SYN_BLOCK_NORM_MAX_COLS)
+        return fail(SYN_E_UNSUPPORTED, "%s: rows of %u values (1 to %d)", W, n, SYN_BLOCK_NORM_MAX_COLS);
+    if (rows >= 1u << 24) return fail(SYN_E_UNSUPPORTED, "%s: %u rows (below 2^24)", W, rows);
+    if (rows == 0) return SYN_OK;
+    if (int rc = check_values(W, "x", xtype, x, x_stride, rows, n)) return rc;
+    if (branch) {
+        if (int rc = check_values(W, "branch", btype, branch, b_stride, rows, n)) return rc;
+        if (gate)
+            if (int rc = check_values(W, "gate", btype, gate, gate_stride, gate_stride ? rows : 1, n)) return rc;
+        if (int rc = check_values(W, "h", xtype, h, h_stride, rows, n)) return rc;
+        if (post && !aligned(post, 4)) return fail(SYN_E_INVALID, "%s: the weights must be 4-byte aligned", W);
+    } else {
+        if (post || gate) return fail(SYN_E_INVALID, "%s: a weight or a gate of no branch", W);
+        if (!g) return fail(SYN_E_INVALID, "%s: neither a branch nor a norm", W);
+        btype = SYN_F32;
+    }
+    if (g) {
+        if (!aligned(g, 4)) return fail(SYN_E_INVALID, "%s: the weights must be 4-byte aligned", W);
+        if (int rc = check_values(W, "y", ytype, y, y_stride, rows, n)) return rc;
+    }
+    const syn::BlockNormArgs a{xtype, x, x_stride, btype, branch, b_stride, post, gate, gate_stride, scale, g, eps,
+                               (int)rows, (int)n, h, h_stride, ytype, y, y_stride};
+    syn::launch_block_norm(a, (hipStream_t)stream);
+    return check_launch(W);
+}
+
+namespace {
+int check_sample(const char* W, int32_t xtype, uint32_t rows, uint32_t vocab) {
+    if (xtype != SYN_F32 && !float_type(xtype)) return fail(SYN_E_UNSUPPORTED, "%s: logits of type %d are not F32, F16 or BF16", W, xtype);
+    if (vocab == 0) return fail(SYN_E_INVALID, "%s: rows of no logits", W);
+    if (vocab > SYN_SAMPLE_MAX_VOCAB || rows >= 1u << 24)
+        return fail(SYN_E_UNSUPPORTED, "%s: %u rows (below 2^24) of %u logits (at most %d)", W, rows, vocab, SYN_SAMPLE_MAX_VOCAB);
+    return SYN_OK;
+}
+}  // namespace
+
+SYN_EXPORT int syn_sample_tokens_workspace_bytes(int32_t xtype, uint32_t rows, uint32_t vocab, uint64_t* bytes) {
+    const char* W = "syn_sample_tokens_workspace_bytes";
+    if (!bytes) return fail(SYN_E_INVALID, "%s: null output", W);
+    if (int rc = check_sample(W, xtype, rows, vocab)) return rc;
+    *bytes = rows ? syn::sample_ws_bytes((int)rows, (int)vocab) : 0;
+    return SYN_OK;
+}
+
+SYN_EXPORT int syn_sample_tokens(int32_t xtype, const void* x, uint64_t x_stride, uint32_t rows, uint32_t vocab, const float* u,
+                                 const float* temperatures, const int32_t* top_ks, const float* top_ps, const float* min_ps,
+                                 float temperature, int32_t top_k, float top_p, float min_p, int32_t* token, float* logprob,
+                                 int32_t* kept, void* ws, uint64_t ws_bytes, void* stream) {
+    const char* W = "syn_sample_tokens";
+    if (int rc = check_sample(W, xtype, rows, vocab)) return rc;
+    if (!temperatures && !(temperature == 0.0f || (temperature >= 0x1p-64f && temperature <= 0x1p64f)))
+        return fail(SYN_E_INVALID, "%s: the temperature %g is neither 0 nor from 2^-64 to 2^64", W, temperature);
+    if (!top_ks && top_k < 0) return fail(SYN_E_INVALID, "%s: top_k %d", W, top_k);
+    if (!top_ps && !(top_p > 0.0f && top_p <= 1.0f)) return fail(SYN_E_INVALID, "%s: top_p %g (above 0, at most 1)", W, top_p);
+    if (!min_ps && !(min_p >= 0.0f && min_p <= 1.0f)) return fail(SYN_E_INVALID, "%s: min_p %g (0 to 1)", W, min_p);
+    if (rows == 0) return SYN_OK;
+    if (int rc = check_values(W, "x", xtype, x, x_stride, rows, vocab)) return rc;
+    if (!u || !token || !logprob || !kept) return fail(SYN_E_INVALID, "%s: null operand", W);
+    if (!aligned(u, 4) || !aligned(temperatures, 4) || !aligned(top_ks, 4) || !aligned(top_ps, 4) || !aligned(min_ps, 4) ||
+        !aligned(token, 4) || !aligned(logprob, 4) || !aligned(kept, 4))
+        return fail(SYN_E_INVALID, "%s: operands must be aligned to their values", W);
+    const uint64_t need = syn::sample_ws_bytes((int)rows, (int)vocab);
+    if (need)
+        if (int rc = check_ws(W, ws, ws_bytes, need)) return rc;
+    const syn::SampleArgs a{x, x_stride, xtype, (int)rows, (int)vocab, u, temperatures, top_ks, top_ps, min_ps,
+                            temperature, top_k, top_p, min_p, token, logprob, kept, (uint8_t*)ws};
+    syn::launch_sample(a, (hipStream_t)stream);
     return check_launch(W);
 }
 

@@ -143,15 +143,17 @@ SYN_DEV float i8_value(int sum, float sx, float sw) { return ((float)sum * sx) *
 // result, and a quotient that is one rounds once.  Below -111 the power is infinite and the quotient 0 (a value
 // below 2^-150).  An infinite or NaN g is met in the product with g.  (14336 x 4096 gated at 1024 tokens 138.7 us;
 // 137.2 with neither the rest of log2(e) nor the values below -88.)
-SYN_DEV float i8_silu(float g) {
+// i8_times_sigmoid(v, z, rest) is v / (1 + exp(-z - rest)), rest far below z; silu(g) with both g.
+SYN_DEV float i8_times_sigmoid(float v, float z, float rest) {
     constexpr float LOG2E = 1.44269504088896340736f, LOG2E_REST = (float)(1.44269504088896340736 - (double)LOG2E);
-    const bool far = g < -80.0f;
-    const float gc = __builtin_amdgcn_fmed3f(g, -180.0f, 100.0f);
+    const bool far = z < -80.0f;
+    const float gc = __builtin_amdgcn_fmed3f(z, -180.0f, 100.0f);
     const float t = gc * -LOG2E;
-    const float r = __builtin_fmaf(gc, -LOG2E_REST, __builtin_fmaf(gc, -LOG2E, -t));
+    const float r = __builtin_fmaf(gc, -LOG2E_REST, __builtin_fmaf(gc, -LOG2E, -t)) - rest;
     const float e = __builtin_amdgcn_exp2f(t + (far ? -32.0f : 0.0f)) * __builtin_fmaf(r, 0.69314718055994530942f, 1.0f);
-    return g * __builtin_amdgcn_rcpf(1.0f + e) * (far ? 0x1p-32f : 1.0f);
+    return v * __builtin_amdgcn_rcpf(1.0f + e) * (far ? 0x1p-32f : 1.0f);
 }
+SYN_DEV float i8_silu(float g) { return i8_times_sigmoid(g, g, 0.0f); }
 
 // Workgroups go to the 8 XCDs in turn.  Each XCD takes a run of neighbouring tiles, token tiles first within
 // groups of 8, so that what runs on it at once shares its weight rows and tokens in its L2.

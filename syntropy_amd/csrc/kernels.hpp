@@ -213,4 +213,49 @@ struct LogprobArgs {
 uint64_t logprob_ws_bytes(int rows, int vocab, int top);
 void launch_logprobs(const LogprobArgs& a, hipStream_t stream);
 
+// block_norm.hip: a block's output into the residual stream and the norm before the next block
+constexpr int BLOCK_NORM_MAX_COLS = 32768;
+struct BlockNormArgs {
+    int xtype;             // of x and h
+    const void* x;         // [rows][n], rows ldx values apart
+    uint64_t ldx;
+    int btype;             // of branch and gate
+    const void* branch;    // [rows][n] or null: h is x, and not written
+    uint64_t ldb;
+    const float* post;     // [n] or null
+    const void* gate;      // [rows][n], rows ldg values apart (0: one for all), or null
+    uint64_t ldg;
+    float scale;
+    const float* g;        // [n] or null: y is not written
+    float eps;
+    int rows, n;
+    void* h;
+    uint64_t ldh;
+    int ytype;
+    void* y;
+    uint64_t ldy;
+};
+void launch_block_norm(const BlockNormArgs& a, hipStream_t stream);
+
+// sample.hip: a token of each row of logits
+struct SampleArgs {
+    const void* x;  // [rows][vocab] of xtype, rows ldx values apart
+    uint64_t ldx;
+    int xtype, rows, vocab;
+    const float* u;              // [rows]
+    const float* temperature;    // [rows], or null: the number below for every row
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    float temperature0;
+    int32_t top_k0;
+    float top_p0, min_p0;
+    int32_t* token;
+    float* logprob;
+    int32_t* kept;
+    uint8_t* ws;
+};
+uint64_t sample_ws_bytes(int rows, int vocab);
+void launch_sample(const SampleArgs& a, hipStream_t stream);
+
 }  // namespace syn

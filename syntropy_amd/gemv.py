@@ -264,6 +264,13 @@ def _ptr_rows(t: torch.Tensor, rows: int, n: int, what: str, device=None) -> int
     return n
 
 
+def _ptr_width(t: torch.Tensor, rows: int, n: int, what: str, device=None) -> int:
+    """_ptr_rows of a tensor whose rows, where it has two dimensions, are n values wide."""
+    if t.dim() == 2 and t.shape[1] != n:
+        raise GemvError("Len", f"`{what}` has rows of {t.shape[1]} values, not {n}")
+    return _ptr_rows(t, rows, n, what, device)
+
+
 _current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
@@ -337,6 +344,134 @@ def _logprobs(logits, ty, stride, rows, vocab, tokens, top, scale, handle) -> To
          top, at, at + 4 * (2 * rows + n), at + 4 * rows, at + 4 * (3 * rows + n), at + 4 * 2 * rows,
          ws.data_ptr() if need else None, need, handle)
     return TokenLogprobs(lp, rank, entropy, ids, lps)
+
+
+class BlockNorm(NamedTuple):
+    """What block_norm gives: the residual stream behind the block, and its norm (None where none is asked for)."""
+
+    h: torch.Tensor
+    y: torch.Tensor | None
+
+
+def _f32_values(t: torch.Tensor, n: int, what: str, device: int) -> int:
+    if t.get_device() != device or t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != n:
+        raise GemvError("Len", f"`{what}` must be a contiguous F32 tensor of {n} values beside the rows")
+    return t.data_ptr()
+
+
+def block_norm(x: torch.Tensor, branch: torch.Tensor | None, g: torch.Tensor | None, eps: float, rows: int,
+               post: torch.Tensor | None = None, gate: torch.Tensor | None = None, scale: float = 1.0,
+               h: torch.Tensor | None = None, y: torch.Tensor | None = None, dtype: torch.dtype | None = None,
+               stream=None) -> BlockNorm:
+    """The end of a block and the beginning of the next over the first `rows` rows: with rms(v; g) = v g /
+    sqrt(mean v^2 + eps),
+
+        h = x + scale * gate * a,  a = rms(branch; post) (branch itself without `post`);  y = rms(h; g)
+
+    in F32, each rounded once, y from the h that is not rounded.  x [., n], the residual stream, and h are of one type,
+    branch and gate of one, y of y's, `dtype` or branch's (F32, F16 or BF16 each); g and post are F32 [n]; gate is
+    [n], [1, n] or rows as x.  Rows may be strided; h may be x itself, and no other output lies in an operand.  Without
+    a branch h is x; without g there is no y.  (rms_norm has the reference's order of sums.)"""
+    if g is None and x.dim() != 2:
+        raise GemvError("Len", "x must be rows of values where no norm's weights say how many")
+    n = g.numel() if g is not None else x.shape[1]
+    ty, xs = _value_type(x, "x"), _ptr_width(x, rows, n, "x")
+    device = x.get_device()
+    bty = bs = gs = 0
+    if branch is not None:
+        bty, bs = _value_type(branch, "branch"), _ptr_width(branch, rows, n, "branch", device)
+        if gate is not None:
+            if gate.dtype != branch.dtype:
+                raise GemvError("Activations", f"the gate is of {gate.dtype}, the branch of {branch.dtype}")
+            if gate.dim() == 1 or (gate.shape == (1, n) and rows != 1):
+                _ptr_width(gate, 1, n, "gate", device)
+                if gate.numel() != n:
+                    raise GemvError("Len", f"a gate of {gate.numel()} values for rows of {n}")
+            else:
+                gs = _ptr_width(gate, rows, n, "gate", device)
+    elif post is not None or gate is not None:
+        raise GemvError("Activations", "post and gate belong to a branch")
+    elif g is None:
+        raise GemvError("Activations", "neither a branch nor a norm")
+    pp = None if post is None else _f32_values(post, n, "post", device)
+    gp = None if g is None else _f32_values(g, n, "g", device)
+    if h is not None and h.dtype != x.dtype:
+        raise GemvError("Len", f"`h` is of {h.dtype}, not {x.dtype}")
+    if y is not None and dtype is not None and dtype != y.dtype:
+        raise GemvError("Len", f"`y` is of {y.dtype}, not {dtype}")
+
+    def launch(handle):
+        ho = x if branch is None else torch.empty(rows, n, dtype=x.dtype, device=x.device) if h is None else h
+        hs = _ptr_width(ho, rows, n, "h", device)
+        yo, yty, ys = None, 0, 0
+        if g is not None:
+            yo = y
+            if y is None:
+                yo = torch.empty(rows, n, dtype=dtype or (x if branch is None else branch).dtype, device=x.device)
+            yty, ys = _value_type(yo, "y"), _ptr_width(yo, rows, n, "y", device)
+        call("syn_block_norm", ty, x.data_ptr(), xs, bty, None if branch is None else branch.data_ptr(), bs, pp,
+             None if gate is None else gate.data_ptr(), gs, scale, gp, eps, rows, n, ho.data_ptr(), hs, yty,
+             None if yo is None else yo.data_ptr(), ys, handle)
+        return BlockNorm(ho, yo)
+    return _on_stream(x, stream, launch)
+
+
+class Sampled(NamedTuple):
+    """What sample_tokens gives, a row each: the token I32, its log probability F32 among those that were kept, and
+    how many were kept I32; all of one allocation."""
+
+    token: torch.Tensor
+    logprob: torch.Tensor
+    kept: torch.Tensor
+
+
+def _setting(v, dtype, rows: int, what: str, device: int):
+    """(address, number) of a setting: a tensor of a value a row, or a number for all."""
+    if not torch.is_tensor(v):
+        return None, v
+    if v.get_device() != device or v.dtype != dtype or not v.is_contiguous() or v.shape != (rows,):
+        raise GemvError("Len", f"`{what}` must be a number or a contiguous {dtype} tensor of {rows} values beside the logits")
+    return v.data_ptr(), 0
+
+
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                  stream=None) -> Sampled:
+    """A token of each row of logits [rows, vocab] (F32, F16 or BF16; strided rows; -infinity hides a token) from a
+    uniform random number u [rows] F32 in [0, 1).  A row's visible logits stand in order (descending, the lower index
+    first among equals), w = exp((x - max x) / temperature): top_k keeps the first k (0: all), top_p of those the least
+    number whose sum of w reaches p times the sum of them (1: all), min_p of those the ones with w >= min_p (0:
+    all).  The token is the first whose running sum of w passes u times the kept ones' sum; a temperature of 0 takes
+    the greatest logit.  Each setting is a number or a tensor of a value a row (F32, top_k int32).
+
+    As numbers: temperature 0 or 2^-64 to 2^64, top_k from 0, top_p above 0 to 1, min_p 0 to 1.  In a tensor values
+    outside top_k's, top_p's and min_p's ranges count as the nearest in them, as u does outside its own.  A row with a
+    NaN or +infinity, without a visible logit, or with a NaN setting or a temperature outside its range has the token
+    -1, the logprob NaN and kept 0.  Equal calls give equal tokens."""
+    shape = logits.shape
+    if len(shape) != 2 or u.shape != shape[:1]:
+        raise GemvError("Len", "logits must be rows of values, with a random number each")
+    rows, vocab = shape
+    device = logits.get_device()
+    if u.dtype != torch.float32 or not u.is_contiguous() or u.get_device() != device:
+        raise GemvError("Len", "u must be contiguous float32 values beside the logits")
+    ty, xs = _value_type(logits, "logits"), _ptr_rows(logits, rows, vocab, "logits")
+    f32 = torch.float32
+    tp, t = _setting(temperature, f32, rows, "temperature", device)
+    kp, k = _setting(top_k, torch.int32, rows, "top_k", device)
+    pp, p = _setting(top_p, f32, rows, "top_p", device)
+    mp, m = _setting(min_p, f32, rows, "min_p", device)
+    if not 0 <= k < 1 << 31:
+        raise GemvError("Len", f"top_k {k}")
+
+    def launch(handle):
+        lp, token, kept = torch.split_with_sizes(torch.empty(3 * rows, dtype=f32, device=logits.device), (rows, rows, rows))
+        need = _need("syn_sample_tokens_workspace_bytes", ty, rows, vocab)
+        ws = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
+        at = lp.data_ptr()
+        call("syn_sample_tokens", ty, logits.data_ptr(), xs, rows, vocab, u.data_ptr(), tp, kp, pp, mp, t, k, p, m,
+             at + 4 * rows, at, at + 8 * rows, ws.data_ptr() if need else None, need, handle)
+        return Sampled(token.view(torch.int32), lp, kept.view(torch.int32))
+    return _on_stream(logits, stream, launch)
 
 
 class GemvBatch:
@@ -440,4 +575,5 @@ def dequantize(ty: WeightType, src: torch.Tensor, stream=None) -> torch.Tensor:
 __all__ = ["WeightType", "Weights", "GemvError", "SynError", "GemvBatch", "workspace_bytes", "quantize_into",
            "repack", "LAYOUT_SOURCE", "LAYOUT_X8", "LAYOUT_SPLIT",
            "gemv_quantized", "gemv", "quantize", "dequantize", "new_workspace", "gemm_workspace",
-           "gemm_quantize_into", "gemm_quantized", "gate_up_act", "token_logprobs", "TokenLogprobs", "lib"]
+           "gemm_quantize_into", "gemm_quantized", "gate_up_act", "token_logprobs", "TokenLogprobs", "block_norm", "BlockNorm",
+           "sample_tokens", "Sampled", "lib"]
