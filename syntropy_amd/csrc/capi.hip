@@ -1287,9 +1287,9 @@ int check_half_shape(const char* W, uint32_t n_out, uint32_t k, uint32_t rows) {
 static_assert(SYN_HALF_MAX_K == syn::HALF_MAX_K, "the header's limit");
 static_assert(SYN_BLOCK_NORM_MAX_COLS == syn::BLOCK_NORM_MAX_COLS, "the header's limit");
 
-// Whether the rows of x are whole 128-byte lines on 16 bytes, as the product's kernels read them.
+// Whether the rows of x are whole pairs of 128-byte lines on 16 bytes, as the product's kernels read them.
 bool half_lines(const void* x, uint64_t stride, uint32_t rows, uint32_t k) {
-    return k % syn::HALF_LINE == 0 && aligned(x, 16) && (rows <= 1 || stride % 8 == 0);
+    return k % syn::HALF_PAIR == 0 && aligned(x, 16) && (rows <= 1 || stride % 8 == 0);
 }
 
 }  // namespace
@@ -1298,7 +1298,7 @@ SYN_EXPORT int syn_half_gemv_workspace_bytes(uint32_t n_out, uint32_t k_in, uint
     const char* W = "syn_half_gemv_workspace_bytes";
     if (!bytes) return fail(SYN_E_INVALID, "%s: null output", W);
     if (int rc = check_half_shape(W, n_out, k_in, rows)) return rc;
-    *bytes = rows && n_out ? syn::half_ws_bytes((int)n_out, (int)k_in, (int)rows, x_aligned && k_in % syn::HALF_LINE == 0) : 0;
+    *bytes = rows && n_out ? syn::half_ws_bytes((int)n_out, (int)k_in, (int)rows, x_aligned && k_in % syn::HALF_PAIR == 0) : 0;
     return SYN_OK;
 }
 

@@ -1,57 +1,95 @@
-// y = act(x W^T + bias) gate + residual over F16 or BF16 weights.
-// The simple form: a wavefront takes a weight row against up to four tokens, 64 values of K a step, in F32.
+// y = act(x W^T + bias) gate + residual over F16 or BF16 weights: the copy of x's rows to whole lines, the fold of a
+// split K, and the choice of the kernels.
 #include "half.hpp"
 #include "kernels.hpp"
 
 namespace syn {
 
-constexpr int DOT_TOKENS = 4;
-
-template <int WTY>
-__global__ __launch_bounds__(256) void k_half_dot(HalfArgs g) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int n = (int)blockIdx.x * 4 + wave, t0 = (int)blockIdx.y * DOT_TOKENS;
-    if (n >= g.n_out) return;
-    const int nt = g.T - t0 < DOT_TOKENS ? g.T - t0 : DOT_TOKENS;
-    const uint16_t* w = g.w + (uint64_t)n * g.ldw;
-    float acc[DOT_TOKENS] = {};
-    for (int k = lane; k < g.k; k += 64) {
-        const float wv = half_at(w, WTY, k);
+// ---- rows of x that are no whole lines, once, zeros behind them ---------------------------------------------
+// Eight values a thread.
+__global__ __launch_bounds__(256) void k_half_rows(const uint16_t* x, uint64_t ldx, int rows, int k, int kp, uint16_t* out) {
+    const int pieces = kp / 8;
+    const uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint64_t t = id / (uint32_t)pieces;
+    const int i = 8 * (int)(id % (uint32_t)pieces);
+    if (t >= (uint64_t)rows) return;
+    const uint16_t* from = x + t * ldx + i;
+    uint32_t h[4] = {};
+    if (i + 8 <= k) {
+        __builtin_memcpy(h, from, 16);
+    } else {
 #pragma unroll
-        for (int j = 0; j < DOT_TOKENS; ++j)
-            if (j < nt) acc[j] = __builtin_fmaf(wv, half_at(g.x + (uint64_t)(t0 + j) * g.ldx, WTY, k), acc[j]);
+        for (int e = 0; e < 8; ++e)
+            if (i + e < k) h[e / 2] |= (uint32_t)from[e] << (16 * (e & 1));
+    }
+    *reinterpret_cast<uint4*>(out + t * (uint32_t)kp + i) = uint4{h[0], h[1], h[2], h[3]};
+}
+
+// ---- the fold of a split K ----------------------------------------------------------------------------
+// Four outputs a thread: their parts added in order, then the epilogue.
+__global__ __launch_bounds__(256) void k_half_fold(HalfArgs g) {
+    const int n = 4 * ((int)blockIdx.x * 256 + (int)threadIdx.x), t = blockIdx.y;
+    if (n >= g.n_out) return;
+    const int in = g.n_out - n < 4 ? g.n_out - n : 4;
+    const uint64_t part = (uint64_t)g.T * g.n_out;
+    const float* p = g.partial + (uint64_t)t * g.n_out + n;
+    float sum[4] = {}, bias[4], gate[4], res[4];
+    if (g.bias) half_load<4>(g.bias, T_F32, n, in, bias);
+    if (g.gate) half_load<4>(g.gate, g.gtype, (uint64_t)t * g.ldg + n, in, gate);
+    if (g.res) half_load<4>(g.res, g.rtype, (uint64_t)t * g.ldr + n, in, res);
+    for (int z = 0; z < g.splits; ++z) {
+        float v[4];
+        half_load<4>(p + z * part, T_F32, 0, in, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += v[e];
     }
 #pragma unroll
-    for (int j = 0; j < DOT_TOKENS; ++j)
-        for (int d = 32; d >= 1; d /= 2) acc[j] += __shfl_xor(acc[j], d);
-    if (lane < nt) {
-        float v = acc[0];
-#pragma unroll
-        for (int j = 1; j < DOT_TOKENS; ++j) v = lane == j ? acc[j] : v;
-        half_emit(g, t0 + lane, n, v);
+    for (int e = 0; e < 4; ++e) {
+        if (e >= in) break;
+        float v = sum[e];
+        if (g.bias) v = v + bias[e];
+        v = half_act(g.act, v);
+        if (g.gate) v = v * gate[e];
+        if (g.res) v = v + res[e];
+        i8_store(g.y, g.ytype, (uint64_t)t * g.ldy + n + e, v);
     }
 }
 
-uint64_t half_ws_bytes(int, int, int, bool) { return 0; }
+// ---- the choice ----------------------------------------------------------------------------------------
+// A workspace: the rows of x, then the parts' sums.
+static uint64_t rows_bytes(int k, int T, bool lines) { return lines ? 0 : align_up(2 * half_padded(k) * (uint64_t)T, 256); }
 
-void launch_half_gemv(const HalfArgs& a, bool, uint8_t*, hipStream_t stream) {
-    constexpr int MOST = 65535 * DOT_TOKENS;
-    for (int t = 0; t < a.T; t += MOST) {  // (what a grid holds)
-        HalfArgs g = a;
-        auto at = [&](const void* p, int ty, uint64_t ld) {
-            return p ? (const uint8_t*)p + (uint64_t)t * ld * (ty == T_F32 ? 4 : 2) : nullptr;
-        };
-        g.T = a.T - t < MOST ? a.T - t : MOST;
-        g.x = a.x + (uint64_t)t * a.ldx;
-        g.gate = at(a.gate, a.gtype, a.ldg);
-        g.res = at(a.res, a.rtype, a.ldr);
-        g.y = (void*)at(a.y, a.ytype, a.ldy);
-        const dim3 grid((g.n_out + 3) / 4, (g.T + DOT_TOKENS - 1) / DOT_TOKENS);
-        if (a.wtype == T_F16)
-            hipLaunchKernelGGL(k_half_dot<T_F16>, grid, dim3(256), 0, stream, g);
-        else
-            hipLaunchKernelGGL(k_half_dot<T_BF16>, grid, dim3(256), 0, stream, g);
+uint64_t half_ws_bytes(int n_out, int k, int T, bool lines) {
+    if (half_few_fits(n_out, T)) return 0;
+    const uint64_t splits = (uint64_t)half_gemm_pick(n_out, k, T).splits;
+    return rows_bytes(k, T, lines) + (splits > 1 ? align_up(4 * splits * (uint64_t)T * (uint64_t)n_out, 256) : 0);
+}
+
+void launch_half_gemv(const HalfArgs& in, bool lines, uint8_t* ws, hipStream_t stream) {
+    HalfArgs a = in;
+    if (half_few_fits(a.n_out, a.T)) {
+        launch_half_few(a, stream);
+        return;
     }
+    const HalfPick p = half_gemm_pick(a.n_out, a.k, a.T);
+    if (!lines) {
+        const int kp = (int)half_padded(a.k);
+        const uint64_t pieces = (uint64_t)a.T * (uint64_t)(kp / 8);
+        hipLaunchKernelGGL(k_half_rows, dim3((uint32_t)((pieces + 255) / 256)), dim3(256), 0, stream, a.x, a.ldx, a.T, a.k, kp,
+                           (uint16_t*)ws);
+        a.x = (const uint16_t*)ws;
+        a.ldx = (uint64_t)kp;
+    }
+    // (rows may be so far apart that a tile's offsets pass 32 bits)
+    if (!half_gemm_reaches(p.tile, a)) {
+        launch_half_few(a, stream);
+        return;
+    }
+    a.splits = p.splits;
+    a.partial = p.splits > 1 ? (float*)(ws + rows_bytes(a.k, a.T, lines)) : nullptr;
+    launch_half_gemm(p.tile, a, stream);
+    if (p.splits > 1)  // (never more rows than a grid holds: K is split where the tiles are few)
+        hipLaunchKernelGGL(k_half_fold, dim3((a.n_out + 1023) / 1024, a.T), dim3(256), 0, stream, a);
 }
 
 }  // namespace syn

@@ -7,9 +7,9 @@ namespace syn {
 
 enum HalfAct { HALF_NONE = 0, HALF_RELU, HALF_SILU, HALF_GELU, HALF_GELU_TANH };
 
-// Rows of weights are followed by zeros up to whole 128-byte lines.
-constexpr int HALF_LINE = 64;  // values
-SYN_HD inline uint64_t half_padded(uint64_t k) { return align_up(k, HALF_LINE); }
+// Rows of weights are followed by zeros up to whole pairs of 128-byte lines, and so are those of a copy of x.
+constexpr int HALF_PAIR = 128;  // values
+SYN_HD inline uint64_t half_padded(uint64_t k) { return align_up(k, HALF_PAIR); }
 constexpr uint32_t HALF_MAX_K = 1 << 20;
 
 struct HalfArgs {
@@ -72,6 +72,47 @@ SYN_DEV float half_at(const void* p, int ty, uint64_t i) {
     return ty == T_F16 ? f16_to_f32(h) : u2f(h << 16);
 }
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+// Eight values of each of 32 (16) rows and columns a lane.
+template <int WTY>
+SYN_DEV f32x16 half_mfma32(i8x16 a, i8x16 b, f32x16 c) {
+    if constexpr (WTY == T_F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <int WTY>
+SYN_DEV f32x4 half_mfma16(i8x16 a, i8x16 b, f32x4 c) {
+    if constexpr (WTY == T_F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// N (4 or 8) values from value i on, the first `in` of them there (the rest 0), at any value's address.
+template <int N>
+SYN_DEV void half_load(const void* p, int ty, uint64_t i, int in, float (&v)[N]) {
+    if (in >= N) {
+        if (ty == T_F32) {
+            __builtin_memcpy(v, (const float*)p + i, 4 * N);
+        } else {
+            uint32_t h[N / 2];
+            __builtin_memcpy(h, (const uint16_t*)p + i, 2 * N);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const uint32_t b = h[j / 2] >> (16 * (j & 1)) & 0xFFFFu;
+                v[j] = ty == T_F16 ? f16_to_f32(b) : u2f(b << 16);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = j < in ? half_at(p, ty, i + j) : 0.0f;
+    }
+}
+
 // One output from its sum: y = act(sum + bias) gate + residual, in F32, rounded once.
 SYN_DEV void half_emit(const HalfArgs& g, int t, int n, float v) {
     if (g.bias) v = v + g.bias[n];
@@ -81,8 +122,19 @@ SYN_DEV void half_emit(const HalfArgs& g, int t, int n, float v) {
     i8_store(g.y, g.ytype, (uint64_t)t * g.ldy + n, v);
 }
 
-uint64_t half_ws_bytes(int n_out, int k, int T, bool x_lines);
-// lines: x's rows are whole lines on 16 bytes; else they are copied into the workspace first.
+// half_few.hip: up to 16 tokens, weights straight to registers; x at any address
+bool half_few_fits(int n_out, int T);
+void launch_half_few(const HalfArgs& a, hipStream_t stream);
+// half_gemm.hip: tiles through LDS, K in one part or several; x's rows are whole pairs of lines on 16 bytes
+struct HalfPick {
+    int tile, splits;
+};
+HalfPick half_gemm_pick(int n_out, int k, int T);
+bool half_gemm_reaches(int tile, const HalfArgs& a);
+void launch_half_gemm(int tile, const HalfArgs& a, hipStream_t stream);
+// half.hip
+// lines: x's rows are whole pairs of lines on 16 bytes; else they are copied into the workspace where they have to be.
+uint64_t half_ws_bytes(int n_out, int k, int T, bool lines);
 void launch_half_gemv(const HalfArgs& a, bool lines, uint8_t* ws, hipStream_t stream);
 
 }  // namespace syn

@@ -1,0 +1,162 @@
+// The half-precision product at few tokens (one to 16): bound by reading the weights once from HBM.
+//
+// v_mfma_f32_16x16x32 multiplies 16 rows by 16 columns over 32 values, four lanes a row of 8 values each.  Its rows
+// are taken as 8 weight rows x the two halves of a 128-byte line and its columns as 8 tokens x the same halves: where
+// a row's half is a column's, the product is one that is wanted (the other quarters are not looked at).  So a lane
+// loads 16 bytes of a weight row straight to the registers that the instruction reads, and an instruction loads
+// whole lines of 8 rows.  No other wavefront reads them, so LDS would only be a detour.
+// The eight wavefronts of a workgroup share 8 RT rows and take turns at K, U lines at a time, two turns in flight;
+// their sums meet in LDS, always in the same order.  The tokens' values of a turn are loaded with its weights (loads
+// return in order), what the epilogue reads before them all.
+#include "half.hpp"
+#include "kernels.hpp"
+
+namespace syn {
+
+// LINES: x's rows are whole pairs of lines on 16 bytes.
+template <int WTY, int RT, int TG, int U, int NW, int LINES>
+__global__ __launch_bounds__(64 * NW, TG > 1 || U * RT > 4 ? 4 : 6) void k_half_few(HalfArgs g) {
+    static_assert(RT * TG <= 4, "the outputs of one wavefront");
+    __shared__ f32x4 red[NW][RT][TG][64];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 7;                                       // weight row, and token, of 8
+    const int piece = 8 * (4 * ((lane >> 3) & 1) + (lane >> 4));  // of a line, in values
+    const int lines = (int)half_padded(g.k) / 64;
+    const int t0 = (int)blockIdx.y * 8 * TG;
+    const int nt = g.T - t0 < 8 * TG ? g.T - t0 : 8 * TG;
+    const int64_t n0 = (int64_t)blockIdx.x * 8 * RT;
+    const uint16_t* wr[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const int64_t n = n0 + 8 * i + c;
+        wr[i] = g.w + (uint64_t)(n < g.n_out ? n : g.n_out - 1) * g.ldw + piece;
+    }
+    const uint16_t* xr = g.x + (uint64_t)(t0 + c) * g.ldx;
+    constexpr int TURN = U * NW;  // lines
+    struct Turn {
+        i8x16 w[U][RT], x[U][TG];
+    };
+    auto load = [&](int s, Turn& to) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (s + u >= lines) break;  // uniform
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+                to.w[u][i] = __builtin_nontemporal_load(reinterpret_cast<const i8x16*>(wr[i] + 64 * (s + u)));
+#pragma unroll
+            for (int j = 0; j < TG; ++j) {
+                to.x[u][j] = i8x16{0, 0, 0, 0};
+                if (8 * j + c >= nt) continue;
+                const int at = 64 * (s + u) + piece;
+                const uint16_t* from = xr + (uint64_t)(8 * j) * g.ldx + at;
+                if constexpr (LINES) {
+                    to.x[u][j] = *reinterpret_cast<const i8x16*>(from);
+                } else if (at + 8 <= g.k) {
+                    __builtin_memcpy(&to.x[u][j], from, 16);
+                } else if (at < g.k) {
+                    uint32_t h[4] = {};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (at + e < g.k) h[e / 2] |= (uint32_t)from[e] << (16 * (e & 1));
+                    to.x[u][j] = i8x16{(int)h[0], (int)h[1], (int)h[2], (int)h[3]};
+                }
+            }
+        }
+    };
+    // the outputs of lane: tile l / 16 of the RT x TG, rows 4 (l / 8 & 1) .. + 3, token l & 7; by the first wavefront
+    const int tile = lane >> 4, half = (lane >> 3) & 1, oi = tile / TG, oj = tile % TG, t = 8 * oj + c;
+    const int64_t n = n0 + 8 * oi + 4 * half;
+    const int in = wave == 0 && tile < RT * TG && t < nt ? (g.n_out - n < 4 ? (int)(g.n_out - n) : 4) : 0;
+    float bias[4] = {}, gate[4] = {}, res[4] = {};
+    if (in > 0) {
+        if (g.bias) half_load<4>(g.bias, T_F32, (uint64_t)n, in, bias);
+        if (g.gate) half_load<4>(g.gate, g.gtype, (uint64_t)(t0 + t) * g.ldg + n, in, gate);
+        if (g.res) half_load<4>(g.res, g.rtype, (uint64_t)(t0 + t) * g.ldr + n, in, res);
+    }
+    Turn cur, nxt;
+    int s = wave * U;
+    load(s, cur);
+    load(s + TURN, nxt);
+    f32x4 acc[RT][TG] = {};
+    auto product = [&](int s, const Turn& o) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (s + u >= lines) break;  // uniform
+#pragma unroll
+            for (int j = 0; j < TG; ++j)
+#pragma unroll
+                for (int i = 0; i < RT; ++i) acc[i][j] = half_mfma16<WTY>(o.w[u][i], o.x[u][j], acc[i][j]);
+        }
+    };
+    while (s < lines) {  // uniform
+        product(s, cur);
+        load(s + 2 * TURN, cur);
+        s += TURN;
+        product(s, nxt);
+        load(s + 2 * TURN, nxt);
+        s += TURN;
+    }
+
+    // The wavefronts' sums.  Lane l holds columns l & 15, rows 4 (l >> 4) .. + 3 of 16: those of the first half
+    // by the first (lanes 0..7 and 16..23) and of the second by the second (40..47 and 56..63).
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < TG; ++j) red[wave][i][j][lane] = acc[i][j];
+    __syncthreads();
+    if (in <= 0) return;
+    f32x4 sum = {};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) sum += red[w][oi][oj][16 * half + c] + red[w][oi][oj][16 * half + 40 + c];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (e >= in) break;
+        float v = sum[e];
+        if (g.bias) v = v + bias[e];
+        v = half_act(g.act, v);
+        if (g.gate) v = v * gate[e];
+        if (g.res) v = v + res[e];
+        i8_store(g.y, g.ytype, (uint64_t)(t0 + t) * g.ldy + n + e, v);
+    }
+}
+
+bool half_few_fits(int n_out, int T) { return T <= 16; }
+
+template <int WTY, int RT, int TG, int U, int NW>
+static void launch_few(const HalfArgs& a, hipStream_t stream) {
+    const dim3 grid((a.n_out + 8 * RT - 1) / (8 * RT), (a.T + 8 * TG - 1) / (8 * TG));
+    const bool lines = a.k % HALF_PAIR == 0 && (uintptr_t)a.x % 16 == 0 && (a.T <= 1 || a.ldx % 8 == 0);
+    if (lines)
+        hipLaunchKernelGGL((k_half_few<WTY, RT, TG, U, NW, 1>), grid, dim3(64 * NW), 0, stream, a);
+    else
+        hipLaunchKernelGGL((k_half_few<WTY, RT, TG, U, NW, 0>), grid, dim3(64 * NW), 0, stream, a);
+}
+template <int WTY>
+static void launch_some(const HalfArgs& a, hipStream_t stream) {
+    if (a.T > 8)
+        launch_few<WTY, 2, 2, 2, 8>(a, stream);
+    else if (a.T > 2)
+        launch_few<WTY, 2, 1, 2, 8>(a, stream);
+    else
+        launch_few<WTY, 1, 1, 2, 8>(a, stream);
+}
+
+// (any number of tokens, for rows that a tile's offsets do not reach: as many a launch as a grid holds)
+void launch_half_few(const HalfArgs& a, hipStream_t stream) {
+    constexpr int MOST = 1 << 18;
+    auto at = [](const void* p, int ty, uint64_t ld, int t) {
+        return p ? (const uint8_t*)p + (uint64_t)t * ld * (ty == T_F32 ? 4 : 2) : nullptr;
+    };
+    for (int t = 0; t < a.T; t += MOST) {
+        HalfArgs g = a;
+        g.T = a.T - t < MOST ? a.T - t : MOST;
+        g.x = a.x + (uint64_t)t * a.ldx;
+        g.gate = at(a.gate, a.gtype, a.ldg, t);
+        g.res = at(a.res, a.rtype, a.ldr, t);
+        g.y = (void*)at(a.y, a.ytype, a.ldy, t);
+        a.wtype == T_F16 ? launch_some<T_F16>(g, stream) : launch_some<T_BF16>(g, stream);
+    }
+}
+
+}  // namespace syn

@@ -103,6 +103,14 @@ SYN_DEV void i8_store(void* y, int ty, uint64_t i, float v) {
         ((uint16_t*)y)[i] = (uint16_t)bf16_bits(v);
 }
 
+template <int N, class F, int I = 0>
+SYN_DEV void static_for(F&& f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        static_for<N, F, I + 1>(static_cast<F&&>(f));
+    }
+}
+
 // A token's scale and the factor of its codes from its largest magnitude's bits: s = a / 127, codes
 // rint(x / s) by the rounded inverse (0 where s or the inverse says nothing); a NaN or an infinity in the
 // row gives the scale NaN and codes 0, so that every output of the row is NaN.

@@ -24,14 +24,6 @@
 
 namespace syn {
 
-template <int N, class F, int I = 0>
-SYN_DEV void static_for(F&& f) {
-    if constexpr (I < N) {
-        f(std::integral_constant<int, I>{});
-        static_for<N, F, I + 1>(static_cast<F&&>(f));
-    }
-}
-
 template <int WM_, int WN_, int WK_, int MT_, int NT_, int RING_>
 struct I8Tile {
     static constexpr int WM = WM_, WN = WN_, WK = WK_, MT = MT_, NT = NT_, RING = RING_;

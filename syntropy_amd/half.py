@@ -20,14 +20,14 @@ from .gemv import GemvError, _current_device, _current_stream, _need, _on_stream
 
 MAX_K = 1 << 20
 ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
-_LINE = 64  # values of a 128-byte line
+_PAIR = 128  # values of two 128-byte lines
 
 
 @dataclass(frozen=True, eq=False)
 class Weights:
     """`matrix` F16 or BF16 [n_out, k_in] with an optional F32 `bias` [n_out], device tensors.  A matrix whose rows are
-    whole 128-byte lines (k_in a multiple of 64) on 16 bytes is kept as it is; any other is copied once, here, into
-    rows of whole lines with zeros behind the values."""
+    whole pairs of 128-byte lines (k_in a multiple of 128) on 16 bytes is kept as it is; any other is copied once, here,
+    into such rows with zeros behind the values."""
 
     matrix: torch.Tensor
     bias: torch.Tensor | None = None
@@ -41,11 +41,11 @@ class Weights:
             raise GemvError("RowLength", f"rows of {k_in} values (1 to {MAX_K})")
         if b is not None and (b.device != w.device or b.dtype != torch.float32 or not b.is_contiguous() or b.shape != (n_out,)):
             raise GemvError("Len", f"bias must be a contiguous F32 tensor of {n_out} values beside the matrix")
-        if k_in % _LINE or w.stride(1) != 1 or w.stride(0) < k_in or w.stride(0) % 8 or w.data_ptr() % 16:
-            rows = torch.zeros(n_out, -(-k_in // _LINE) * _LINE, dtype=w.dtype, device=w.device)[:, :k_in]
+        if k_in % _PAIR or w.stride(1) != 1 or w.stride(0) < k_in or w.stride(0) % 8 or w.data_ptr() % 16:
+            rows = torch.zeros(n_out, -(-k_in // _PAIR) * _PAIR, dtype=w.dtype, device=w.device)[:, :k_in]
             w = rows.copy_(w)
         stride = w.stride(0)
-        row = -(-k_in // _LINE) * _LINE
+        row = -(-k_in // _PAIR) * _PAIR
         # the C ABI's arguments: type, the matrix's view (address, bytes, stride), bias
         view = (_value_type(w, "matrix"), w.data_ptr(), 2 * ((n_out - 1) * stride + row) if n_out else 0, stride,
                 0 if b is None else b.data_ptr())
@@ -55,7 +55,7 @@ class Weights:
 
 def workspace_bytes(n_out: int, k_in: int, rows: int, x_aligned: bool = False) -> int:
     """Scratch bytes of a call: partial sums where K is split, and a copy of x's rows unless they can be read as they
-    lie (`x_aligned`: on 16 bytes, a stride of a multiple of 8 values, and k_in a multiple of 64)."""
+    lie (`x_aligned`: on 16 bytes, a stride of a multiple of 8 values, and k_in a multiple of 128)."""
     return _need("syn_half_gemv_workspace_bytes", n_out, k_in, rows, 1 if x_aligned else 0)
 
 
