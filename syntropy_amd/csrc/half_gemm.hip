@@ -204,98 +204,84 @@ __global__ __launch_bounds__(64 * C::NW, C::MT* C::NT >= 16 ? 1 : 2) void k_half
                 wave_lds_sync();
             }
         }
-        // piece p of the tile: token p / PIECES, outputs p % PIECES * PER ..  At most four at a time: gate and residual
-        // are read before the first of them is written (y may be either).
-        constexpr int GROUP = TURNS < 4 ? TURNS : 4;
-        static_for<TURNS / GROUP>([&](auto gc) {
-            constexpr int p0 = decltype(gc)::value * GROUP * 64;
-            float gate[GROUP][PER], res[GROUP][PER];
-            auto place_of = [&](int q, int& t, int& n, int& in) {
-                const int p = p0 + 64 * q + lane;
-                t = p / PIECES;
-                n = nb + p % PIECES * PER;
-                in = tb + t < g.T ? (g.n_out - n < PER ? g.n_out - n : PER) : 0;
-                in = in < 0 ? 0 : in;
-            };
-            if constexpr (OT != OUT_PART) {
-                if (g.gate) {
-#pragma unroll
-                    for (int q = 0; q < GROUP; ++q) {
-                        int t, n, in;
-                        place_of(q, t, n, in);
-                        if (in > 0) half_load<PER>(g.gate, g.gtype, (uint64_t)(tb + t) * g.ldg + n, in, gate[q]);
-                    }
-                }
-                if (g.res) {
-#pragma unroll
-                    for (int q = 0; q < GROUP; ++q) {
-                        int t, n, in;
-                        place_of(q, t, n, in);
-                        if (in > 0) half_load<PER>(g.res, g.rtype, (uint64_t)(tb + t) * g.ldr + n, in, res[q]);
-                    }
+        const float* staged = reinterpret_cast<const float*>(mine);
+        if (nb + OC > g.n_out) {  // uniform: behind the last output, value by value
+#pragma unroll 1
+            for (int p = lane; p < 32 * OC; p += 64) {
+                const int t = p / OC, n = nb + p % OC;
+                if (tb + t >= g.T || n >= g.n_out) continue;
+                float v = staged[t * (PITCH / 4) + n - nb];
+                if constexpr (OT == OUT_PART) {
+                    g.partial[((uint64_t)z * g.T + tb + t) * (uint64_t)g.n_out + n] = v;
+                } else {
+                    if (g.gate) v = v * half_at(g.gate, g.gtype, (uint64_t)(tb + t) * g.ldg + n);
+                    if (g.res) v = v + half_at(g.res, g.rtype, (uint64_t)(tb + t) * g.ldr + n);
+                    i8_store(g.y, g.ytype, (uint64_t)(tb + t) * g.ldy + n, v);
                 }
             }
-#pragma unroll
-            for (int q = 0; q < GROUP; ++q) {
-                int t, n, in;
-                place_of(q, t, n, in);
-                if (in <= 0) continue;
-                float v[PER];
-                const float* from = reinterpret_cast<const float*>(mine + t * PITCH) + (n - nb);
-#pragma unroll
-                for (int e = 0; e < PER; e += 4) {
-                    const float4 f = *reinterpret_cast<const float4*>(from + e);
-                    v[e] = f.x, v[e + 1] = f.y, v[e + 2] = f.z, v[e + 3] = f.w;
-                }
-                if constexpr (OT == OUT_PART) {
-                    float* out = g.partial + ((uint64_t)z * g.T + tb + t) * (uint64_t)g.n_out + n;
-                    if (in == PER) {
-                        __builtin_memcpy(out, v, 16);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < PER; ++e)
-                            if (e < in) out[e] = v[e];
-                    }
-                } else {
+        } else {
+            // piece p of the tile: token p / PIECES, outputs p % PIECES * PER ..  At most four at a time: gate and residual
+            // are read before the first of them is written (y may be either).
+            constexpr int GROUP = TURNS < 4 ? TURNS : 4;
+            static_for<TURNS / GROUP>([&](auto gc) {
+                constexpr int p0 = decltype(gc)::value * GROUP * 64;
+                float gate[GROUP][PER], res[GROUP][PER];
+                auto token = [&](int q) { return (p0 + 64 * q + lane) / PIECES; };
+                const int o = lane % PIECES * PER, n = nb + o;  // (64 is whole tokens' pieces)
+                static_assert(64 % PIECES == 0, "the same outputs each turn");
+                if constexpr (OT != OUT_PART) {
                     if (g.gate) {
 #pragma unroll
-                        for (int e = 0; e < PER; ++e) v[e] = v[e] * gate[q][e];
+                        for (int q = 0; q < GROUP; ++q)
+                            if (tb + token(q) < g.T)
+                                half_load<PER>(g.gate, g.gtype, (uint64_t)(tb + token(q)) * g.ldg + n, PER, gate[q]);
                     }
                     if (g.res) {
 #pragma unroll
-                        for (int e = 0; e < PER; ++e) v[e] = v[e] + res[q][e];
+                        for (int q = 0; q < GROUP; ++q)
+                            if (tb + token(q) < g.T)
+                                half_load<PER>(g.res, g.rtype, (uint64_t)(tb + token(q)) * g.ldr + n, PER, res[q]);
                     }
-                    const uint64_t to = (uint64_t)(tb + t) * g.ldy + n;
-                    if constexpr (OT == OUT_F32) {
-                        float* out = (float*)g.y + to;
-                        if (in == PER) {
-                            __builtin_memcpy(out, v, 16);
-                        } else {
+                }
 #pragma unroll
-                            for (int e = 0; e < PER; ++e)
-                                if (e < in) out[e] = v[e];
-                        }
+                for (int q = 0; q < GROUP; ++q) {
+                    const int t = token(q);
+                    if (tb + t >= g.T) continue;
+                    float v[PER];
+#pragma unroll
+                    for (int e = 0; e < PER; e += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(staged + t * (PITCH / 4) + o + e);
+                        v[e] = f.x, v[e + 1] = f.y, v[e + 2] = f.z, v[e + 3] = f.w;
+                    }
+                    if constexpr (OT == OUT_PART) {
+                        __builtin_memcpy(g.partial + ((uint64_t)z * g.T + tb + t) * (uint64_t)g.n_out + n, v, 16);
                     } else {
-                        uint32_t w[4];
-                        if (g.ytype == T_F16) {
+                        if (g.gate) {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) w[e] = i8_half2<T_F16>(v[2 * e], v[2 * e + 1]);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) w[e] = i8_half2<T_BF16>(v[2 * e], v[2 * e + 1]);
+                            for (int e = 0; e < PER; ++e) v[e] = v[e] * gate[q][e];
                         }
-                        uint16_t* out = (uint16_t*)g.y + to;
-                        if (in == PER) {
-                            __builtin_memcpy(out, w, 16);
-                        } else {
+                        if (g.res) {
 #pragma unroll
-                            for (int e = 0; e < PER; ++e)
-                                if (e < in) out[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+                            for (int e = 0; e < PER; ++e) v[e] = v[e] + res[q][e];
+                        }
+                        const uint64_t to = (uint64_t)(tb + t) * g.ldy + n;
+                        if constexpr (OT == OUT_F32) {
+                            __builtin_memcpy((float*)g.y + to, v, 16);
+                        } else {
+                            uint32_t w[4];
+                            if (g.ytype == T_F16) {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) w[e] = i8_half2<T_F16>(v[2 * e], v[2 * e + 1]);
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) w[e] = i8_half2<T_BF16>(v[2 * e], v[2 * e + 1]);
+                            }
+                            __builtin_memcpy((uint16_t*)g.y + to, w, 16);
                         }
                     }
                 }
-            }
-        });
+            });
+        }
         wave_lds_sync();
         __builtin_amdgcn_sched_barrier(0);  // (the sums of one token tile at a time in vector registers)
     };
