@@ -33,26 +33,15 @@ __global__ __launch_bounds__(256) void k_half_fold(HalfArgs g) {
     const int in = g.n_out - n < 4 ? g.n_out - n : 4;
     const uint64_t part = (uint64_t)g.T * g.n_out;
     const float* p = g.partial + (uint64_t)t * g.n_out + n;
-    float sum[4] = {}, bias[4], gate[4], res[4];
-    if (g.bias) half_load<4>(g.bias, T_F32, n, in, bias);
-    if (g.gate) half_load<4>(g.gate, g.gtype, (uint64_t)t * g.ldg + n, in, gate);
-    if (g.res) half_load<4>(g.res, g.rtype, (uint64_t)t * g.ldr + n, in, res);
+    const HalfRest rest = half_rest(g, t, n, in);
+    float sum[4] = {};
     for (int z = 0; z < g.splits; ++z) {
         float v[4];
         half_load<4>(p + z * part, T_F32, 0, in, v);
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum[e] += v[e];
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if (e >= in) break;
-        float v = sum[e];
-        if (g.bias) v = v + bias[e];
-        v = half_act(g.act, v);
-        if (g.gate) v = v * gate[e];
-        if (g.res) v = v + res[e];
-        i8_store(g.y, g.ytype, (uint64_t)t * g.ldy + n + e, v);
-    }
+    half_emit(g, t, n, in, sum, rest);
 }
 
 // ---- the choice ----------------------------------------------------------------------------------------

@@ -37,14 +37,30 @@ struct HalfArgs {
 
 // The activation of an F32 sum, each within about 2^-20 of its value where that is no subnormal: the argument of
 // each exponential is carried in two parts, since its rounding (2^-24 of up to 80) would be the result's error.
-// gelu is v Phi(v) = v erfc(-v / sqrt 2) / 2, which keeps its relative accuracy where v is far below 0 and
-// 1 + erf would cancel; d erfc(a) is about -2 a erfc(a) there.  The tanh form of it is v / (1 + exp(-2 z)), the
-// value of v (1 + tanh z) / 2 without its cancellation, 2 z = v (c1 + c2 v^2).
+// gelu is v Phi(v) with Phi(-x) = erfc(x / sqrt 2) / 2, which keeps its relative accuracy where v is far below 0 and
+// 1 + erf would cancel.  With t = 1 / (1 + 0.4 x / sqrt 2) the logarithm of erfc(x / sqrt 2) exp(x^2 / 2) / t is
+// smooth in t: a polynomial of degree 8, a minimax fit over x from 0 to 17 (9.1e-8; in F32 4.3e-7 of the result, no
+// branches).  (With the library's erfc, some 150 instructions on both sides of a branch, 5003 x 2011 at 333 tokens took
+// 9 us more than without an activation.)
 SYN_DEV float half_gelu(float v) {
-    constexpr double C = -0.70710678118654752440;
+    constexpr double C = -0.72134752044448170368;  // -log2(e) / 2
     constexpr float HI = (float)C, LO = (float)(C - (double)HI);
-    const float a = v * HI, rest = __builtin_fmaf(v, LO, __builtin_fmaf(v, HI, -a));
-    return 0.5f * v * (erfcf(a) * (a > 1.0f && a < 12.0f ? __builtin_fmaf(-2.0f * a, rest, 1.0f) : 1.0f));
+    const float x = fminf(__builtin_fabsf(v), 20.0f);
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(x, 0.28284271247461900976f, 1.0f));
+    float q = -0.30159053206443787f;
+    q = __builtin_fmaf(q, t, 1.345345377922058f);
+    q = __builtin_fmaf(q, t, -2.168454647064209f);
+    q = __builtin_fmaf(q, t, 1.4710724353790283f);
+    q = __builtin_fmaf(q, t, -0.6613202691078186f);
+    q = __builtin_fmaf(q, t, 0.44308316707611084f);
+    q = __builtin_fmaf(q, t, 0.5741007924079895f);
+    q = __builtin_fmaf(q, t, 1.4455450773239136f);
+    q = __builtin_fmaf(q, t, -2.1477816104888916f);
+    const float s = x * x, sr = __builtin_fmaf(x, x, -s);
+    const float e = s * HI, er = __builtin_fmaf(sr, HI, __builtin_fmaf(s, LO, __builtin_fmaf(s, HI, -e)));
+    const float n = __builtin_rintf(e);
+    const float tail = __builtin_ldexpf(0.5f * x * t * __builtin_amdgcn_exp2f((e - n) + (q + er)), (int)n);
+    return v < 0.0f ? (v - v) - tail : v - tail;  // (a NaN at -infinity, as the formula)
 }
 SYN_DEV float half_gelu_tanh(float v) {
     constexpr double C1 = 1.5957691216057307117, C2 = C1 * 0.044715;
@@ -56,13 +72,23 @@ SYN_DEV float half_gelu_tanh(float v) {
     const float z = v * p, zr = __builtin_fmaf(v, pr, __builtin_fmaf(v, p, -z));
     return i8_times_sigmoid(v, z, zr * 1.44269504088896340736f);
 }
-SYN_DEV float half_act(int act, float v) {
+template <int ACT>
+SYN_DEV float half_act(float v) {
+    if constexpr (ACT == HALF_RELU) return v < 0.0f ? 0.0f : v;  // (a NaN stays one)
+    if constexpr (ACT == HALF_SILU) return i8_silu(v);
+    if constexpr (ACT == HALF_GELU) return half_gelu(v);
+    if constexpr (ACT == HALF_GELU_TANH) return half_gelu_tanh(v);
+    return v;
+}
+// f(the activation's constant) of a uniform `act`.
+template <class F>
+SYN_DEV void half_act_of(int act, F&& f) {
     switch (act) {
-        case HALF_RELU: return v < 0.0f ? 0.0f : v;  // (a NaN stays one)
-        case HALF_SILU: return i8_silu(v);
-        case HALF_GELU: return half_gelu(v);
-        case HALF_GELU_TANH: return half_gelu_tanh(v);
-        default: return v;
+        case HALF_RELU: return f(std::integral_constant<int, HALF_RELU>{});
+        case HALF_SILU: return f(std::integral_constant<int, HALF_SILU>{});
+        case HALF_GELU: return f(std::integral_constant<int, HALF_GELU>{});
+        case HALF_GELU_TANH: return f(std::integral_constant<int, HALF_GELU_TANH>{});
+        default: return;
     }
 }
 
@@ -113,13 +139,51 @@ SYN_DEV void half_load(const void* p, int ty, uint64_t i, int in, float (&v)[N])
     }
 }
 
-// One output from its sum: y = act(sum + bias) gate + residual, in F32, rounded once.
-SYN_DEV void half_emit(const HalfArgs& g, int t, int n, float v) {
-    if (g.bias) v = v + g.bias[n];
-    v = half_act(g.act, v);
-    if (g.gate) v = v * half_at(g.gate, g.gtype, (uint64_t)t * g.ldg + n);
-    if (g.res) v = v + half_at(g.res, g.rtype, (uint64_t)t * g.ldr + n);
-    i8_store(g.y, g.ytype, (uint64_t)t * g.ldy + n, v);
+// The same as they lie in memory, to be unpacked when they are used: N (4 or 8) values that are all there.
+template <int N>
+SYN_DEV void half_fetch(const void* p, int ty, uint64_t i, uint32_t (&raw)[N]) {
+    if (ty == T_F32)
+        __builtin_memcpy(raw, (const float*)p + i, 4 * N);
+    else
+        __builtin_memcpy(raw, (const uint16_t*)p + i, 2 * N);
+}
+template <int N>
+SYN_DEV void half_unpack(int ty, const uint32_t (&raw)[N], float (&v)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const uint32_t b = raw[j / 2] >> (16 * (j & 1)) & 0xFFFFu;
+        v[j] = ty == T_F32 ? u2f(raw[j]) : ty == T_F16 ? f16_to_f32(b) : u2f(b << 16);
+    }
+}
+
+// Four outputs (the first `in` of them) of token t from their sums, with what the epilogue reads:
+// y = act(sum + bias) gate + residual in F32, rounded once.
+struct HalfRest {
+    float bias[4], gate[4], res[4];
+};
+SYN_DEV HalfRest half_rest(const HalfArgs& g, int t, int64_t n, int in) {
+    HalfRest r{};
+    if (g.bias) half_load<4>(g.bias, T_F32, (uint64_t)n, in, r.bias);
+    if (g.gate) half_load<4>(g.gate, g.gtype, (uint64_t)t * g.ldg + n, in, r.gate);
+    if (g.res) half_load<4>(g.res, g.rtype, (uint64_t)t * g.ldr + n, in, r.res);
+    return r;
+}
+SYN_DEV void half_emit(const HalfArgs& g, int t, int64_t n, int in, float (&v)[4], const HalfRest& r) {
+    if (g.bias) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = v[e] + r.bias[e];
+    }
+    half_act_of(g.act, [&](auto act) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = half_act<decltype(act)::value>(v[e]);
+    });
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (e >= in) break;
+        if (g.gate) v[e] = v[e] * r.gate[e];
+        if (g.res) v[e] = v[e] + r.res[e];
+        i8_store(g.y, g.ytype, (uint64_t)t * g.ldy + n + e, v[e]);
+    }
 }
 
 // half_few.hip: up to 16 tokens, weights straight to registers; x at any address

@@ -68,12 +68,8 @@ __global__ __launch_bounds__(64 * NW, TG > 1 || U * RT > 4 ? 4 : 6) void k_half_
     const int tile = lane >> 4, half = (lane >> 3) & 1, oi = tile / TG, oj = tile % TG, t = 8 * oj + c;
     const int64_t n = n0 + 8 * oi + 4 * half;
     const int in = wave == 0 && tile < RT * TG && t < nt ? (g.n_out - n < 4 ? (int)(g.n_out - n) : 4) : 0;
-    float bias[4] = {}, gate[4] = {}, res[4] = {};
-    if (in > 0) {
-        if (g.bias) half_load<4>(g.bias, T_F32, (uint64_t)n, in, bias);
-        if (g.gate) half_load<4>(g.gate, g.gtype, (uint64_t)(t0 + t) * g.ldg + n, in, gate);
-        if (g.res) half_load<4>(g.res, g.rtype, (uint64_t)(t0 + t) * g.ldr + n, in, res);
-    }
+    HalfRest rest{};
+    if (in > 0) rest = half_rest(g, t0 + t, n, in);
     Turn cur, nxt;
     int s = wave * U;
     load(s, cur);
@@ -109,16 +105,8 @@ __global__ __launch_bounds__(64 * NW, TG > 1 || U * RT > 4 ? 4 : 6) void k_half_
     f32x4 sum = {};
 #pragma unroll
     for (int w = 0; w < NW; ++w) sum += red[w][oi][oj][16 * half + c] + red[w][oi][oj][16 * half + 40 + c];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if (e >= in) break;
-        float v = sum[e];
-        if (g.bias) v = v + bias[e];
-        v = half_act(g.act, v);
-        if (g.gate) v = v * gate[e];
-        if (g.res) v = v + res[e];
-        i8_store(g.y, g.ytype, (uint64_t)(t0 + t) * g.ldy + n + e, v);
-    }
+    float v[4] = {sum[0], sum[1], sum[2], sum[3]};
+    half_emit(g, t0 + t, n, in, v, rest);
 }
 
 bool half_few_fits(int n_out, int T) { return T <= 16; }

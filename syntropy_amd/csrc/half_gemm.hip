@@ -136,6 +136,36 @@ __global__ __launch_bounds__(64 * C::NW, C::MT* C::NT >= 16 ? 1 : 2) void k_half
         });
     };
 
+    // What the epilogue reads of one operand (the gate, else the residual) is fetched a unit of it ahead, the first
+    // unit before all else: a unit waits for memory otherwise, with nothing beside it.
+    constexpr int IC = WK > 1 ? 1 : MT;                           // row tiles of an emission
+    constexpr int OC = 32 * IC, PITCH = OC * 4 + 16;
+    constexpr int PER = OT == OUT_16 ? 8 : 4, ROW = OC / PER;     // values of 16 bytes, pieces a token
+    constexpr int TURNS = 32 * ROW / 64, GROUP = TURNS < 4 ? TURNS : 4, GROUPS = TURNS / GROUP;
+    static_assert(64 % ROW == 0, "the same outputs each turn");
+    uint32_t ahead[2][GROUP][PER];
+    const void* const op = g.gate ? g.gate : g.res;
+    const int otype = g.gate ? g.gtype : g.rtype;
+    const uint64_t ldo = g.gate ? g.ldg : g.ldr;
+    const int lo = lane % ROW * PER;                              // of the emission's outputs
+    auto fetch = [&](int i0, int j, int gi, uint32_t (&to)[GROUP][PER]) {
+        if constexpr (OT != OUT_PART) {
+            const int tb = t0 + (wn * NT + j) * 32, nb = n0 + wm * 32 * MT + 32 * i0;
+            if (!op || nb + OC > g.n_out) return;  // uniform
+#pragma unroll
+            for (int q = 0; q < GROUP; ++q) {
+                const int t = tb + (64 * (GROUP * gi + q) + lane) / ROW;
+                if (t < g.T) half_fetch<PER>(op, otype, (uint64_t)t * ldo + nb + lo, to[q]);
+            }
+        }
+    };
+    if constexpr (WK == 1) {
+        fetch(0, 0, 0, ahead[0]);
+    } else {
+        static_assert(MT * NT % WK == 0 || MT * NT < WK, "as many tiles a part");
+        if (wk < MT * NT) fetch(wk / NT, wk % NT, 0, ahead[0]);
+    }
+
     static_for<RING - 1>([&](auto sc) {
         const Where v = where(s0 + decltype(sc)::value, decltype(sc)::value);
         static_for<C::CPW>([&](auto i) { copy(v, decltype(i)::value); });
@@ -168,11 +198,9 @@ __global__ __launch_bounds__(64 * C::NW, C::MT* C::NT >= 16 ? 1 : 2) void k_half
             wave_lds_sync();
         }
     }
-    // the outputs of token tile j, row tiles i0 .. i0 + IC - 1
-    auto emit = [&](auto jc, auto i0c, auto icc) {
-        constexpr int j = decltype(jc)::value, i0 = decltype(i0c)::value, IC = decltype(icc)::value;
-        constexpr int OC = 32 * IC, PITCH = OC * 4 + 16;
-        constexpr int PER = OT == OUT_16 ? 8 : 4, PIECES = OC / PER, TURNS = 32 * PIECES / 64;  // of 16 bytes
+    // The outputs of token tile j, row tiles i0 .. i0 + IC - 1; unit: how many units were before; (in, jn): the next ones.
+    auto emit = [&](auto jc, auto i0c, auto unitc, int in, int jn) {
+        constexpr int j = decltype(jc)::value, i0 = decltype(i0c)::value;
         const int tb = t0 + (wn * NT + j) * 32, nb = n0 + wm * WR + 32 * i0;
         static_for<IC>([&](auto ic) {
             constexpr int i = i0 + decltype(ic)::value;
@@ -193,19 +221,23 @@ __global__ __launch_bounds__(64 * C::NW, C::MT* C::NT >= 16 ? 1 : 2) void k_half
         });
         wave_lds_sync();
         if constexpr (OT != OUT_PART) {
-            if (g.act != HALF_NONE) {  // in place and in a loop: the four activations' code once
+            // in place and in a loop, eight values at a time: each activation's code once
+            half_act_of(g.act, [&](auto act) {
+                constexpr int ACT = decltype(act)::value;
 #pragma unroll 1
-                for (int p = lane; p < 32 * OC / 4; p += 64) {
-                    float4* at = reinterpret_cast<float4*>(mine + p / (OC / 4) * PITCH) + p % (OC / 4);
-                    float4 v = *at;
-                    v.x = half_act(g.act, v.x), v.y = half_act(g.act, v.y), v.z = half_act(g.act, v.z), v.w = half_act(g.act, v.w);
-                    *at = v;
+                for (int p = lane; p < 32 * OC / 4; p += 128) {
+                    float4* a0 = reinterpret_cast<float4*>(mine + p / (OC / 4) * PITCH) + p % (OC / 4);
+                    float4* a1 = a0 + 64 / (OC / 4) * (PITCH / 16);
+                    float4 v = *a0, w = *a1;
+                    v.x = half_act<ACT>(v.x), v.y = half_act<ACT>(v.y), v.z = half_act<ACT>(v.z), v.w = half_act<ACT>(v.w);
+                    w.x = half_act<ACT>(w.x), w.y = half_act<ACT>(w.y), w.z = half_act<ACT>(w.z), w.w = half_act<ACT>(w.w);
+                    *a0 = v, *a1 = w;
                 }
                 wave_lds_sync();
-            }
+            });
         }
         const float* staged = reinterpret_cast<const float*>(mine);
-        if (nb + OC > g.n_out) {  // uniform: behind the last output, value by value
+        if (nb + OC > g.n_out) {  // uniform: the last outputs, value by value
 #pragma unroll 1
             for (int p = lane; p < 32 * OC; p += 64) {
                 const int t = p / OC, n = nb + p % OC;
@@ -219,24 +251,22 @@ __global__ __launch_bounds__(64 * C::NW, C::MT* C::NT >= 16 ? 1 : 2) void k_half
                     i8_store(g.y, g.ytype, (uint64_t)(tb + t) * g.ldy + n, v);
                 }
             }
+            // (tiles beside it may not be the last ones)
+            if constexpr (WK > 1) fetch(in, jn, 0, ahead[(decltype(unitc)::value + GROUPS) & 1]);
         } else {
-            // piece p of the tile: token p / PIECES, outputs p % PIECES * PER ..  At most four at a time: gate and residual
-            // are read before the first of them is written (y may be either).
-            constexpr int GROUP = TURNS < 4 ? TURNS : 4;
-            static_for<TURNS / GROUP>([&](auto gc) {
-                constexpr int p0 = decltype(gc)::value * GROUP * 64;
-                float gate[GROUP][PER], res[GROUP][PER];
-                auto token = [&](int q) { return (p0 + 64 * q + lane) / PIECES; };
-                const int o = lane % PIECES * PER, n = nb + o;  // (64 is whole tokens' pieces)
-                static_assert(64 % PIECES == 0, "the same outputs each turn");
+            // Piece p of the tile: token p / ROW, outputs p % ROW * PER ..  A group's gate and residual are read before the
+            // first of its outputs is written (y may be either, and no other group's).
+            const int n = nb + lo;
+            static_for<GROUPS>([&](auto gc) {
+                constexpr int gi = decltype(gc)::value, now = (decltype(unitc)::value + gi) & 1;
+                if constexpr (gi + 1 < GROUPS)
+                    fetch(i0, j, gi + 1, ahead[1 - now]);
+                else
+                    fetch(in, jn, 0, ahead[1 - now]);
+                float res[GROUP][PER];
+                auto token = [&](int q) { return (64 * (GROUP * gi + q) + lane) / ROW; };
                 if constexpr (OT != OUT_PART) {
-                    if (g.gate) {
-#pragma unroll
-                        for (int q = 0; q < GROUP; ++q)
-                            if (tb + token(q) < g.T)
-                                half_load<PER>(g.gate, g.gtype, (uint64_t)(tb + token(q)) * g.ldg + n, PER, gate[q]);
-                    }
-                    if (g.res) {
+                    if (g.gate && g.res) {
 #pragma unroll
                         for (int q = 0; q < GROUP; ++q)
                             if (tb + token(q) < g.T)
@@ -250,19 +280,26 @@ __global__ __launch_bounds__(64 * C::NW, C::MT* C::NT >= 16 ? 1 : 2) void k_half
                     float v[PER];
 #pragma unroll
                     for (int e = 0; e < PER; e += 4) {
-                        const float4 f = *reinterpret_cast<const float4*>(staged + t * (PITCH / 4) + o + e);
+                        const float4 f = *reinterpret_cast<const float4*>(staged + t * (PITCH / 4) + lo + e);
                         v[e] = f.x, v[e + 1] = f.y, v[e + 2] = f.z, v[e + 3] = f.w;
                     }
                     if constexpr (OT == OUT_PART) {
                         __builtin_memcpy(g.partial + ((uint64_t)z * g.T + tb + t) * (uint64_t)g.n_out + n, v, 16);
                     } else {
-                        if (g.gate) {
+                        if (op) {
+                            float o[PER];
+                            half_unpack<PER>(otype, ahead[now][q], o);
+                            if (g.gate) {
 #pragma unroll
-                            for (int e = 0; e < PER; ++e) v[e] = v[e] * gate[q][e];
-                        }
-                        if (g.res) {
+                                for (int e = 0; e < PER; ++e) v[e] = v[e] * o[e];
+                                if (g.res) {
 #pragma unroll
-                            for (int e = 0; e < PER; ++e) v[e] = v[e] + res[q][e];
+                                    for (int e = 0; e < PER; ++e) v[e] = v[e] + res[q][e];
+                                }
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < PER; ++e) v[e] = v[e] + o[e];
+                            }
                         }
                         const uint64_t to = (uint64_t)(tb + t) * g.ldy + n;
                         if constexpr (OT == OUT_F32) {
@@ -286,7 +323,10 @@ __global__ __launch_bounds__(64 * C::NW, C::MT* C::NT >= 16 ? 1 : 2) void k_half
         __builtin_amdgcn_sched_barrier(0);  // (the sums of one token tile at a time in vector registers)
     };
     if constexpr (WK == 1) {
-        static_for<NT>([&](auto jc) { emit(jc, std::integral_constant<int, 0>{}, std::integral_constant<int, MT>{}); });
+        static_for<NT>([&](auto jc) {
+            constexpr int j = decltype(jc)::value;
+            emit(jc, std::integral_constant<int, 0>{}, std::integral_constant<int, j * GROUPS>{}, 0, j + 1 < NT ? j + 1 : j);
+        });
     } else {
         // output tile u goes to the wavefront of part u % WK: the others' sums of it through LDS, added in the
         // parts' order from its own on
@@ -312,7 +352,9 @@ __global__ __launch_bounds__(64 * C::NW, C::MT* C::NT >= 16 ? 1 : 2) void k_half
 #pragma unroll
                     for (int m = 0; m < 4; ++m) acc[i][j][4 * e + m] += v[m];
                 }
-            emit(std::integral_constant<int, j>{}, std::integral_constant<int, i>{}, std::integral_constant<int, 1>{});
+            constexpr int next = u + WK < MT * NT ? u + WK : u;
+            emit(std::integral_constant<int, j>{}, std::integral_constant<int, i>{}, std::integral_constant<int, u / WK * GROUPS>{},
+                 next / NT, next % NT);
         });
     }
 }
