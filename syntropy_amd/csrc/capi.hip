@@ -1400,7 +1400,7 @@ SYN_EXPORT int syn_sample_tokens_workspace_bytes(int32_t xtype, uint32_t rows, u
     const char* W = "syn_sample_tokens_workspace_bytes";
     if (!bytes) return fail(SYN_E_INVALID, "%s: null output", W);
     if (int rc = check_sample(W, xtype, rows, vocab)) return rc;
-    *bytes = rows ? syn::sample_ws_bytes((int)rows, (int)vocab) : 0;
+    *bytes = rows ? syn::sample_ws_bytes(xtype, (int)rows, (int)vocab) : 0;
     return SYN_OK;
 }
 
@@ -1421,7 +1421,7 @@ SYN_EXPORT int syn_sample_tokens(int32_t xtype, const void* x, uint64_t x_stride
     if (!aligned(u, 4) || !aligned(temperatures, 4) || !aligned(top_ks, 4) || !aligned(top_ps, 4) || !aligned(min_ps, 4) ||
         !aligned(token, 4) || !aligned(logprob, 4) || !aligned(kept, 4))
         return fail(SYN_E_INVALID, "%s: operands must be aligned to their values", W);
-    const uint64_t need = syn::sample_ws_bytes((int)rows, (int)vocab);
+    const uint64_t need = syn::sample_ws_bytes(xtype, (int)rows, (int)vocab);
     if (need)
         if (int rc = check_ws(W, ws, ws_bytes, need)) return rc;
     const syn::SampleArgs a{x, x_stride, xtype, (int)rows, (int)vocab, u, temperatures, top_ks, top_ps, min_ps,

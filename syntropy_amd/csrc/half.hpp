@@ -196,6 +196,8 @@ struct HalfPick {
 HalfPick half_gemm_pick(int n_out, int k, int T);
 bool half_gemm_reaches(int tile, const HalfArgs& a);
 void launch_half_gemm(int tile, const HalfArgs& a, hipStream_t stream);
+void launch_half_gemm_f16(int tile, const HalfArgs& a, hipStream_t stream);
+void launch_half_gemm_bf16(int tile, const HalfArgs& a, hipStream_t stream);
 // half.hip
 // lines: x's rows are whole pairs of lines on 16 bytes; else they are copied into the workspace where they have to be.
 uint64_t half_ws_bytes(int n_out, int k, int T, bool lines);

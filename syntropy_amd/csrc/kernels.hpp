@@ -255,7 +255,7 @@ struct SampleArgs {
     int32_t* kept;
     uint8_t* ws;
 };
-uint64_t sample_ws_bytes(int rows, int vocab);
+uint64_t sample_ws_bytes(int xtype, int rows, int vocab);
 void launch_sample(const SampleArgs& a, hipStream_t stream);
 
 }  // namespace syn

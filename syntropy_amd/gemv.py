@@ -374,46 +374,64 @@ def block_norm(x: torch.Tensor, branch: torch.Tensor | None, g: torch.Tensor | N
     a branch h is x; without g there is no y.  (rms_norm has the reference's order of sums.)"""
     if g is None and x.dim() != 2:
         raise GemvError("Len", "x must be rows of values where no norm's weights say how many")
+    device = x.get_device()
+    if stream is None and device == _current_device():
+        return _block_norm(x, branch, g, eps, rows, post, gate, scale, h, y, dtype, device, _current_stream(device))
+    return _on_stream(x, stream, lambda handle: _block_norm(x, branch, g, eps, rows, post, gate, scale, h, y, dtype, device, handle))
+
+
+def _block_norm(x, branch, g, eps, rows, post, gate, scale, h, y, dtype, device, handle) -> BlockNorm:
     n = g.numel() if g is not None else x.shape[1]
     ty, xs = _value_type(x, "x"), _ptr_width(x, rows, n, "x")
-    device = x.get_device()
-    bty = bs = gs = 0
+    like, whole = x, x.shape == (rows, n)  # y's type; whether empty_like gives the outputs' shape (less host time)
+    bty = bs = gs = bp = sp = pp = gp = None
     if branch is not None:
-        bty, bs = _value_type(branch, "branch"), _ptr_width(branch, rows, n, "branch", device)
+        like, bp = branch, branch.data_ptr()
+        bty, bs = ty if branch.dtype is x.dtype else _value_type(branch, "branch"), _ptr_width(branch, rows, n, "branch", device)
+        if post is not None:
+            pp = _f32_values(post, n, "post", device)
         if gate is not None:
             if gate.dtype != branch.dtype:
                 raise GemvError("Activations", f"the gate is of {gate.dtype}, the branch of {branch.dtype}")
+            sp = gate.data_ptr()
             if gate.dim() == 1 or (gate.shape == (1, n) and rows != 1):
-                _ptr_width(gate, 1, n, "gate", device)
+                _ptr_rows(gate, 1, n, "gate", device)
                 if gate.numel() != n:
                     raise GemvError("Len", f"a gate of {gate.numel()} values for rows of {n}")
             else:
                 gs = _ptr_width(gate, rows, n, "gate", device)
-    elif post is not None or gate is not None:
-        raise GemvError("Activations", "post and gate belong to a branch")
-    elif g is None:
-        raise GemvError("Activations", "neither a branch nor a norm")
-    pp = None if post is None else _f32_values(post, n, "post", device)
-    gp = None if g is None else _f32_values(g, n, "g", device)
-    if h is not None and h.dtype != x.dtype:
-        raise GemvError("Len", f"`h` is of {h.dtype}, not {x.dtype}")
-    if y is not None and dtype is not None and dtype != y.dtype:
-        raise GemvError("Len", f"`y` is of {y.dtype}, not {dtype}")
-
-    def launch(handle):
-        ho = x if branch is None else torch.empty(rows, n, dtype=x.dtype, device=x.device) if h is None else h
-        hs = _ptr_width(ho, rows, n, "h", device)
-        yo, yty, ys = None, 0, 0
-        if g is not None:
-            yo = y
-            if y is None:
-                yo = torch.empty(rows, n, dtype=dtype or (x if branch is None else branch).dtype, device=x.device)
-            yty, ys = _value_type(yo, "y"), _ptr_width(yo, rows, n, "y", device)
-        call("syn_block_norm", ty, x.data_ptr(), xs, bty, None if branch is None else branch.data_ptr(), bs, pp,
-             None if gate is None else gate.data_ptr(), gs, scale, gp, eps, rows, n, ho.data_ptr(), hs, yty,
-             None if yo is None else yo.data_ptr(), ys, handle)
-        return BlockNorm(ho, yo)
-    return _on_stream(x, stream, launch)
+        if h is None:
+            h = torch.empty_like(x) if whole and x.is_contiguous() else torch.empty(rows, n, dtype=x.dtype, device=x.device)
+            hs = n
+        else:
+            if h.dtype != x.dtype:
+                raise GemvError("Len", f"`h` is of {h.dtype}, not {x.dtype}")
+            hs = _ptr_width(h, rows, n, "h", device)
+    else:
+        if post is not None or gate is not None:
+            raise GemvError("Activations", "post and gate belong to a branch")
+        if g is None:
+            raise GemvError("Activations", "neither a branch nor a norm")
+        h, hs = x, xs
+    yp, yty, ys = None, 0, 0
+    if g is not None:
+        gp = _f32_values(g, n, "g", device)
+        if y is None:
+            if whole and like.shape == (rows, n) and (dtype is None or dtype is like.dtype) and like.is_contiguous():
+                y = torch.empty_like(like)
+            else:
+                y = torch.empty(rows, n, dtype=dtype or like.dtype, device=x.device)
+            ys = n
+        else:
+            if dtype is not None and dtype != y.dtype:
+                raise GemvError("Len", f"`y` is of {y.dtype}, not {dtype}")
+            ys = _ptr_width(y, rows, n, "y", device)
+        yp, yty = y.data_ptr(), _value_type(y, "y")
+    else:
+        y = None
+    call("syn_block_norm", ty, x.data_ptr(), xs, bty or 0, bp, bs or 0, pp, sp, gs or 0, scale, gp, eps, rows, n, h.data_ptr(), hs,
+         yty, yp, ys, handle)
+    return BlockNorm(h, y)
 
 
 class Sampled(NamedTuple):
@@ -463,15 +481,20 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     if not 0 <= k < 1 << 31:
         raise GemvError("Len", f"top_k {k}")
 
-    def launch(handle):
-        lp, token, kept = torch.split_with_sizes(torch.empty(3 * rows, dtype=f32, device=logits.device), (rows, rows, rows))
-        need = _need("syn_sample_tokens_workspace_bytes", ty, rows, vocab)
-        ws = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
-        at = lp.data_ptr()
-        call("syn_sample_tokens", ty, logits.data_ptr(), xs, rows, vocab, u.data_ptr(), tp, kp, pp, mp, t, k, p, m,
-             at + 4 * rows, at, at + 8 * rows, ws.data_ptr() if need else None, need, handle)
-        return Sampled(token.view(torch.int32), lp, kept.view(torch.int32))
-    return _on_stream(logits, stream, launch)
+    if stream is None and device == _current_device():
+        return _sample(logits, ty, xs, rows, vocab, u, (tp, kp, pp, mp, t, k, p, m), _current_stream(device))
+    return _on_stream(logits, stream, lambda handle: _sample(logits, ty, xs, rows, vocab, u, (tp, kp, pp, mp, t, k, p, m), handle))
+
+
+def _sample(logits, ty, xs, rows, vocab, u, settings, handle) -> Sampled:
+    need = _need("syn_sample_tokens_workspace_bytes", ty, rows, vocab)
+    out = torch.empty(3, rows, dtype=torch.float32, device=logits.device)
+    ws = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
+    at = out.data_ptr()
+    call("syn_sample_tokens", ty, logits.data_ptr(), xs, rows, vocab, u.data_ptr(), *settings, at + 4 * rows, at, at + 8 * rows,
+         ws.data_ptr() if need else None, need, handle)
+    lp, token, kept = out.unbind()
+    return Sampled(token.view(torch.int32), lp, kept.view(torch.int32))
 
 
 class GemvBatch:
