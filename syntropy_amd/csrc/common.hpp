@@ -355,6 +355,22 @@ SYN_DEV void q8k_block_wave(const float* __restrict__ xb, int8_t* __restrict__ c
     if (lane == 0) *dout = r.d;
 }
 
+// The greatest number that at least n of a wavefront's values (four a lane) reach, but for its last 14 bits
+// (which let a few more values pass).  Two bits a turn: a turn is the wait for the counts.
+SYN_DEV uint32_t reached_by(const uint32_t (&v)[4], int n) {
+    uint32_t r = 0;
+#pragma unroll 1
+    for (int at = 30; at >= 14; at -= 2) {
+        int c[3] = {0, 0, 0};
+#pragma unroll
+        for (uint32_t b = 1; b < 4; ++b)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) c[b - 1] += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[j] >= (r | b << at)));
+        r |= (c[2] >= n ? 3u : c[1] >= n ? 2u : c[0] >= n ? 1u : 0u) << at;
+    }
+    return r;
+}
+
 // ---- LDS staging helpers of the matrix-core kernels ----------------------------------------
 
 // s_waitcnt that waits for vector memory only: vmcnt n, expcnt and lgkmcnt left at their maxima.

@@ -42,22 +42,6 @@ SYN_DEV float lp_value(uint32_t k) { return u2f(k >> 31 ? k ^ 0x80000000u : ~k);
 SYN_DEV uint64_t lp_key(float v, int i) { return (uint64_t)lp_order(v) << 32 | (0x7FFFFFFFu - (uint32_t)i); }
 SYN_DEV int lp_index(uint64_t k) { return (int)(0x7FFFFFFFu - (uint32_t)k); }
 
-// The greatest number that at least n of a wavefront's values (four a lane) reach, but for its last 14 bits
-// (which let a few more values pass).  Two bits a turn: a turn is the wait for the counts.
-SYN_DEV uint32_t reached_by(const uint32_t (&v)[4], int n) {
-    uint32_t r = 0;
-#pragma unroll 1
-    for (int at = 30; at >= 14; at -= 2) {
-        int c[3] = {0, 0, 0};
-#pragma unroll
-        for (uint32_t b = 1; b < 4; ++b)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) c[b - 1] += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[j] >= (r | b << at)));
-        r |= (c[2] >= n ? 3u : c[1] >= n ? 2u : c[0] >= n ? 1u : 0u) << at;
-    }
-    return r;
-}
-
 constexpr int LP_ROOM = 512;
 // The greatest keys so far of a workgroup of W wavefronts, in LDS.
 template <int W>
