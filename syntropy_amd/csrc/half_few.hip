@@ -109,7 +109,11 @@ __global__ __launch_bounds__(64 * NW, TG > 1 || U * RT > 4 ? 4 : 6) void k_half_
     half_emit(g, t0 + t, n, in, v, rest);
 }
 
-bool half_few_fits(int n_out, int T) { return T <= 16; }
+// Against the tiles that split K (BF16, us, at 8 rows): 4096 x 4096 9.2 and 12.3, 14336 x 4096 25.0 and 23.9, 4096 x 14336 24.1
+// and 25.4, 6144 x 4096 14.5 and 15.1, 32000 x 4096 46.9 and 54.7.  At 16 rows the tokens' values weigh as much as
+// the weights here, and the tiles' LDS pays but for small matrices: 10.6 and 12.6, 32.0 and 24.0, 29.0 and 25.5, 18.1 and
+// 15.2, 60.7 and 55.5; 1024 x 1024 4.6 and 4.8, 2048 x 8192 13.9 and 14.0.
+bool half_few_fits(int n_out, int k, int T) { return T <= 8 || (T <= 16 && n_out * half_padded(k) <= 1 << 24); }
 
 template <int WTY, int RT, int TG, int U, int NW>
 static void launch_few(const HalfArgs& a, hipStream_t stream) {
@@ -120,14 +124,17 @@ static void launch_few(const HalfArgs& a, hipStream_t stream) {
     else
         hipLaunchKernelGGL((k_half_few<WTY, RT, TG, U, NW, 0>), grid, dim3(64 * NW), 0, stream, a);
 }
+// 16 weight rows a workgroup read each token's values for twice as many products as 8, and leave half as many workgroups:
+// taken from three tokens on where their last round over the 256 CUs is full enough (4096 x 4096 at 8 tokens 9.2 us and
+// 10.5, 32000 x 4096 46.9 and 59.6; 6144 x 4096 at 4, one round and a half, 14.0 and 12.5, 2048 x 8192 12.3 and 9.5).
 template <int WTY>
 static void launch_some(const HalfArgs& a, hipStream_t stream) {
+    const int64_t wgs = ((int64_t)a.n_out + 15) / 16, rounds = (wgs + 255) / 256;
+    const bool two = a.T > 2 && 5 * wgs >= 4 * 256 * rounds;
     if (a.T > 8)
-        launch_few<WTY, 2, 2, 2, 8>(a, stream);
-    else if (a.T > 2)
-        launch_few<WTY, 2, 1, 2, 8>(a, stream);
+        two ? launch_few<WTY, 2, 2, 1, 8>(a, stream) : launch_few<WTY, 1, 2, 2, 8>(a, stream);
     else
-        launch_few<WTY, 1, 1, 2, 8>(a, stream);
+        two ? launch_few<WTY, 2, 1, 1, 8>(a, stream) : launch_few<WTY, 1, 1, 2, 8>(a, stream);
 }
 
 // (any number of tokens, for rows that a tile's offsets do not reach: as many a launch as a grid holds)

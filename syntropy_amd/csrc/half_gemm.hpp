@@ -2,13 +2,15 @@
 //
 // A workgroup takes a tile of 32 MT WM weight rows x 32 NT WN tokens; WM x WN x WK wavefronts take 32 MT x 32 NT
 // of it each, and a WK-th of K: 32 values of every row a stage and wavefront.  The stages' lines are copied into
-// a ring in LDS by global_load_lds, RING - 1 stages ahead.  Piece p (16 bytes) of line r lies at p ^ (r & 7) (p
+// a ring in LDS by global_load_lds, RING - 1 stages ahead (RING 0: whole lines of 128 bytes, two stages and a half
+// ahead, below).  Piece p (16 bytes) of line r lies at p ^ (r & 7) (p
 // ^ (r / 2 & 3) for lines of 64 bytes), so that eight neighbouring lines' same pieces are on eight different
 // bank groups.
 // Each half stage's operands are read into registers during the half stage before, the first half of the next
 // stage's behind the stage's one barrier, and all of it (products, reads, copies) is written in the order in
-// which it is to be issued and held there: a large tile leaves two wavefronts a SIMD, of which each has to cover
-// its own reads.
+// which it is to be issued and held there: a large tile leaves one or two wavefronts a SIMD, of which each has to cover
+// its own reads.  Bound by the matrix cores at many tokens: 8192^3 takes 790 us (1390 TFLOP/s; the library's product
+// 767), 14336 x 4096 at 2048 tokens 200 (1200 TFLOP/s; 203), where 448 tiles are two rounds over 256 CUs for 1.75.
 // The weight rows are the instruction's A rows, the tokens its columns: a lane holds four neighbouring outputs
 // of a token at a time, which go, with the bias, through LDS to whole pieces of y's rows, where the activation is
 // applied and gate and residual are read as such pieces too.
@@ -43,7 +45,7 @@ struct HalfTile {
     static_assert(BM % (RPC * NW) == 0 && BN % (RPC * NW) == 0, "every wavefront copies as many lines");
     static_assert(PIECES < 8 || NW % 2 == 0 || WIDE, "a wavefront's copies begin at rows of one parity");
     static_assert(WIDE || (RING >= 3 && CPW * (RING - 2) < 64), "vmcnt");
-    static_assert(!WIDE || (WK == 1 && BM == BN && MT * NT == 16 && WPW == 8 && XPW == 8), "copies beside products");
+    static_assert(!WIDE || (WK == 1 && BM == BN && XPW == WPW && WPW <= MT * NT && MT + NT <= MT * NT), "copies and reads beside products");
     static_assert(MT * NT >= 2, "reads beside one product, copies beside another");
     static_assert(LDS <= 160 * 1024, "LDS");
     static_assert(2 * HALF_PAIR % LINE == 0, "a row is whole stages");
@@ -186,8 +188,8 @@ __global__ __launch_bounds__(64 * C::NW, C::MT* C::NT >= 16 ? 1 : 2) void k_half
             const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(p >> 32));
             return (const uint8_t*)(uintptr_t)((uint64_t)hi << 32 | lo);
         };
-        // copy i of a unit's eight into its place
-        auto copy5 = [&](const uint8_t* base, const uint32_t (&offsets)[8], int slot, int i) {
+        // copy i of a unit's into its place
+        auto copy5 = [&](const uint8_t* base, const uint32_t (&offsets)[C::WPW], int slot, int i) {
             lds_dma16(offsets[i], base, ring + (uint32_t)slot * C::UNIT + 1024u * (uint32_t)(wave + C::NW * i));
         };
         const uint8_t* aw = lds + (wm * WR + c) * LINE;
@@ -210,11 +212,11 @@ __global__ __launch_bounds__(64 * C::NW, C::MT* C::NT >= 16 ? 1 : 2) void k_half
                 __builtin_amdgcn_sched_barrier(0);
             });
         };
-        static_for<8>([&](auto i) { copy5(from(wb, s0), wo, 0, decltype(i)::value); });
-        static_for<8>([&](auto i) { copy5(from(xb, s0), xo, 1, decltype(i)::value); });
-        static_for<8>([&](auto i) { copy5(from(wb, s0 + 1), wo, 2, decltype(i)::value); });
-        static_for<8>([&](auto i) { copy5(from(xb, s0 + 1), xo, 3, decltype(i)::value); });
-        wait_vm<16>();
+        static_for<C::WPW>([&](auto i) { copy5(from(wb, s0), wo, 0, decltype(i)::value); });
+        static_for<C::WPW>([&](auto i) { copy5(from(xb, s0), xo, 1, decltype(i)::value); });
+        static_for<C::WPW>([&](auto i) { copy5(from(wb, s0 + 1), wo, 2, decltype(i)::value); });
+        static_for<C::WPW>([&](auto i) { copy5(from(xb, s0 + 1), xo, 3, decltype(i)::value); });
+        wait_vm<2 * C::WPW>();
         lds_barrier();
         static_for<MT + NT>([&](auto r) { operand(0, 0, decltype(r)::value); });
         int slot = 0;
@@ -222,14 +224,14 @@ __global__ __launch_bounds__(64 * C::NW, C::MT* C::NT >= 16 ? 1 : 2) void k_half
             const int spare = place5(slot + 4), next = place5(slot + 2);
             const uint8_t *w2 = from(wb, s + 2), *x2 = from(xb, s + 2);
             quarter(std::integral_constant<int, 0>{}, slot, [&](int m) {
-                if (m >= 8) copy5(w2, wo, spare, m - 8);
+                if (m >= MT * NT - C::WPW) copy5(w2, wo, spare, m - (MT * NT - C::WPW));
             });
             quarter(std::integral_constant<int, 1>{}, slot, [](int) {});
             quarter(std::integral_constant<int, 2>{}, slot, [](int) {});
-            wait_vm<8>();  // stage s + 1 is there
+            wait_vm<C::WPW>();  // stage s + 1 is there
             lds_barrier();
             quarter(std::integral_constant<int, 3>{}, next, [&](int m) {
-                if (m < 8) copy5(x2, xo, slot, m);
+                if (m < C::WPW) copy5(x2, xo, slot, m);
             });
             slot = next;
         }
@@ -428,18 +430,15 @@ __global__ __launch_bounds__(64 * C::NW, C::MT* C::NT >= 16 ? 1 : 2) void k_half
     }
 }
 
-// The tiles: wavefronts over weight rows, tokens and K, each one's 32-row and 32-token tiles, the ring's stages;
-// then what a workgroup that has a CU to itself takes beside K and a 1024 values of K, in tenths of a microsecond.
+// The tiles: wavefronts over weight rows, tokens and K, each one's 32-row and 32-token tiles, the ring's stages (0: WIDE);
+// then what a workgroup that has a CU to itself takes beside K and a 1024 values of K, in tenths of a microsecond
+// (BF16, 4096 x 4096, 14336 x 4096 and 4096 x 14336 matrices at 32 to 2048 tokens).
 #define SYN_HALF_TILES(X)             \
-    X(0, 4, 2, 1, 2, 4, 4, 50, 270)   \
-    X(1, 4, 2, 1, 2, 2, 4, 27, 200)   \
-    X(2, 2, 4, 1, 2, 2, 4, 30, 174)   \
-    X(3, 2, 4, 1, 2, 1, 6, 5, 120)    \
-    X(4, 2, 1, 2, 2, 4, 3, 56, 96)    \
-    X(5, 1, 2, 2, 2, 2, 4, 2, 64)     \
-    X(6, 1, 1, 4, 2, 2, 4, 4, 40)     \
-    X(7, 1, 1, 4, 2, 1, 4, 1, 30)    \
-    X(8, 2, 2, 1, 4, 4, 0, 250, 240)
+    X(0, 4, 2, 1, 2, 4, 0, 77, 191)   \
+    X(1, 2, 2, 1, 2, 2, 0, 28, 77)    \
+    X(2, 1, 2, 2, 2, 2, 4, 19, 58)    \
+    X(3, 1, 1, 4, 2, 2, 4, 19, 36)    \
+    X(4, 1, 1, 4, 2, 1, 4, 19, 26)
 
 template <class C, int WTY, int OT>
 static void launch_as(const HalfArgs& a, hipStream_t stream) {
