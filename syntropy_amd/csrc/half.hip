@@ -49,14 +49,14 @@ __global__ __launch_bounds__(256) void k_half_fold(HalfArgs g) {
 static uint64_t rows_bytes(int k, int T, bool lines) { return lines ? 0 : align_up(2 * half_padded(k) * (uint64_t)T, 256); }
 
 uint64_t half_ws_bytes(int n_out, int k, int T, bool lines) {
-    if (half_few_fits(n_out, k, T)) return 0;
+    if (half_few_fits(T)) return 0;
     const uint64_t splits = (uint64_t)half_gemm_pick(n_out, k, T).splits;
     return rows_bytes(k, T, lines) + (splits > 1 ? align_up(4 * splits * (uint64_t)T * (uint64_t)n_out, 256) : 0);
 }
 
 void launch_half_gemv(const HalfArgs& in, bool lines, uint8_t* ws, hipStream_t stream) {
     HalfArgs a = in;
-    if (half_few_fits(a.n_out, a.k, a.T)) {
+    if (half_few_fits(a.T)) {
         launch_half_few(a, stream);
         return;
     }

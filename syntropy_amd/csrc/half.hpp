@@ -186,8 +186,8 @@ SYN_DEV void half_emit(const HalfArgs& g, int t, int64_t n, int in, float (&v)[4
     }
 }
 
-// half_few.hip: up to 16 tokens, weights straight to registers; x at any address
-bool half_few_fits(int n_out, int k, int T);
+// half_few.hip: up to 8 tokens, weights straight to registers; x at any address
+bool half_few_fits(int T);
 void launch_half_few(const HalfArgs& a, hipStream_t stream);
 // half_gemm.hip: tiles through LDS, K in one part or several; x's rows are whole pairs of lines on 16 bytes
 struct HalfPick {

@@ -1,4 +1,4 @@
-// The half-precision product at few tokens (one to 16): bound by reading the weights once from HBM.
+// The half-precision product at few tokens (one to eight): bound by reading the weights once from HBM.
 //
 // v_mfma_f32_16x16x32 multiplies 16 rows by 16 columns over 32 values, four lanes a row of 8 values each.  Its rows
 // are taken as 8 weight rows x the two halves of a 128-byte line and its columns as 8 tokens x the same halves: where
@@ -14,17 +14,17 @@
 namespace syn {
 
 // LINES: x's rows are whole pairs of lines on 16 bytes.
-template <int WTY, int RT, int TG, int U, int NW, int LINES>
-__global__ __launch_bounds__(64 * NW, TG > 1 || U * RT > 4 ? 4 : 6) void k_half_few(HalfArgs g) {
-    static_assert(RT * TG <= 4, "the outputs of one wavefront");
-    __shared__ f32x4 red[NW][RT][TG][64];
+template <int WTY, int RT, int U, int NW, int LINES>
+__global__ __launch_bounds__(64 * NW, 6) void k_half_few(HalfArgs g) {
+    static_assert(RT <= 4, "the outputs of one wavefront");
+    __shared__ f32x4 red[NW][RT][64];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 7;                                       // weight row, and token, of 8
     const int piece = 8 * (4 * ((lane >> 3) & 1) + (lane >> 4));  // of a line, in values
     const int lines = (int)half_padded(g.k) / 64;
-    const int t0 = (int)blockIdx.y * 8 * TG;
-    const int nt = g.T - t0 < 8 * TG ? g.T - t0 : 8 * TG;
+    const int t0 = (int)blockIdx.y * 8;
+    const int nt = g.T - t0 < 8 ? g.T - t0 : 8;
     const int64_t n0 = (int64_t)blockIdx.x * 8 * RT;
     const uint16_t* wr[RT];
 #pragma unroll
@@ -35,7 +35,7 @@ __global__ __launch_bounds__(64 * NW, TG > 1 || U * RT > 4 ? 4 : 6) void k_half_
     const uint16_t* xr = g.x + (uint64_t)(t0 + c) * g.ldx;
     constexpr int TURN = U * NW;  // lines
     struct Turn {
-        i8x16 w[U][RT], x[U][TG];
+        i8x16 w[U][RT], x[U];
     };
     auto load = [&](int s, Turn& to) {
 #pragma unroll
@@ -44,45 +44,40 @@ __global__ __launch_bounds__(64 * NW, TG > 1 || U * RT > 4 ? 4 : 6) void k_half_
 #pragma unroll
             for (int i = 0; i < RT; ++i)
                 to.w[u][i] = __builtin_nontemporal_load(reinterpret_cast<const i8x16*>(wr[i] + 64 * (s + u)));
+            to.x[u] = i8x16{0, 0, 0, 0};
+            if (c >= nt) continue;
+            const int at = 64 * (s + u) + piece;
+            const uint16_t* from = xr + at;
+            if constexpr (LINES) {
+                to.x[u] = *reinterpret_cast<const i8x16*>(from);
+            } else if (at + 8 <= g.k) {
+                __builtin_memcpy(&to.x[u], from, 16);
+            } else if (at < g.k) {
+                uint32_t h[4] = {};
 #pragma unroll
-            for (int j = 0; j < TG; ++j) {
-                to.x[u][j] = i8x16{0, 0, 0, 0};
-                if (8 * j + c >= nt) continue;
-                const int at = 64 * (s + u) + piece;
-                const uint16_t* from = xr + (uint64_t)(8 * j) * g.ldx + at;
-                if constexpr (LINES) {
-                    to.x[u][j] = *reinterpret_cast<const i8x16*>(from);
-                } else if (at + 8 <= g.k) {
-                    __builtin_memcpy(&to.x[u][j], from, 16);
-                } else if (at < g.k) {
-                    uint32_t h[4] = {};
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (at + e < g.k) h[e / 2] |= (uint32_t)from[e] << (16 * (e & 1));
-                    to.x[u][j] = i8x16{(int)h[0], (int)h[1], (int)h[2], (int)h[3]};
-                }
+                for (int e = 0; e < 8; ++e)
+                    if (at + e < g.k) h[e / 2] |= (uint32_t)from[e] << (16 * (e & 1));
+                to.x[u] = i8x16{(int)h[0], (int)h[1], (int)h[2], (int)h[3]};
             }
         }
     };
-    // the outputs of lane: tile l / 16 of the RT x TG, rows 4 (l / 8 & 1) .. + 3, token l & 7; by the first wavefront
-    const int tile = lane >> 4, half = (lane >> 3) & 1, oi = tile / TG, oj = tile % TG, t = 8 * oj + c;
-    const int64_t n = n0 + 8 * oi + 4 * half;
-    const int in = wave == 0 && tile < RT * TG && t < nt ? (g.n_out - n < 4 ? (int)(g.n_out - n) : 4) : 0;
+    // the outputs of lane l: tile l / 16, rows 4 (l / 8 & 1) .. + 3, token l & 7; by the first wavefront
+    const int tile = lane >> 4, half = (lane >> 3) & 1;
+    const int64_t n = n0 + 8 * tile + 4 * half;
+    const int in = wave == 0 && tile < RT && c < nt ? (g.n_out - n < 4 ? (int)(g.n_out - n) : 4) : 0;
     HalfRest rest{};
-    if (in > 0) rest = half_rest(g, t0 + t, n, in);
+    if (in > 0) rest = half_rest(g, t0 + c, n, in);
     Turn cur, nxt;
     int s = wave * U;
     load(s, cur);
     load(s + TURN, nxt);
-    f32x4 acc[RT][TG] = {};
+    f32x4 acc[RT] = {};
     auto product = [&](int s, const Turn& o) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (s + u >= lines) break;  // uniform
 #pragma unroll
-            for (int j = 0; j < TG; ++j)
-#pragma unroll
-                for (int i = 0; i < RT; ++i) acc[i][j] = half_mfma16<WTY>(o.w[u][i], o.x[u][j], acc[i][j]);
+            for (int i = 0; i < RT; ++i) acc[i] = half_mfma16<WTY>(o.w[u][i], o.x[u], acc[i]);
         }
     };
     while (s < lines) {  // uniform
@@ -97,32 +92,29 @@ __global__ __launch_bounds__(64 * NW, TG > 1 || U * RT > 4 ? 4 : 6) void k_half_
     // The wavefronts' sums.  Lane l holds columns l & 15, rows 4 (l >> 4) .. + 3 of 16: those of the first half
     // by the first (lanes 0..7 and 16..23) and of the second by the second (40..47 and 56..63).
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int j = 0; j < TG; ++j) red[wave][i][j][lane] = acc[i][j];
+    for (int i = 0; i < RT; ++i) red[wave][i][lane] = acc[i];
     __syncthreads();
     if (in <= 0) return;
     f32x4 sum = {};
 #pragma unroll
-    for (int w = 0; w < NW; ++w) sum += red[w][oi][oj][16 * half + c] + red[w][oi][oj][16 * half + 40 + c];
+    for (int w = 0; w < NW; ++w) sum += red[w][tile][16 * half + c] + red[w][tile][16 * half + 40 + c];
     float v[4] = {sum[0], sum[1], sum[2], sum[3]};
-    half_emit(g, t0 + t, n, in, v, rest);
+    half_emit(g, t0 + c, n, in, v, rest);
 }
 
-// Against the tiles that split K (BF16, us, at 8 rows): 4096 x 4096 9.2 and 12.3, 14336 x 4096 25.0 and 23.9, 4096 x 14336 24.1
-// and 25.4, 6144 x 4096 14.5 and 15.1, 32000 x 4096 46.9 and 54.7.  At 16 rows the tokens' values weigh as much as
-// the weights here, and the tiles' LDS pays but for small matrices: 10.6 and 12.6, 32.0 and 24.0, 29.0 and 25.5, 18.1 and
-// 15.2, 60.7 and 55.5; 1024 x 1024 4.6 and 4.8, 2048 x 8192 13.9 and 14.0.
-bool half_few_fits(int n_out, int k, int T) { return T <= 8 || (T <= 16 && n_out * half_padded(k) <= 1 << 24); }
+// Against the tiles (BF16, us, at 8 rows): 4096 x 4096 9.2 and 10.5, 14336 x 4096 25.0 and 23.9, 4096 x 14336 24.1 and 25.4,
+// 32000 x 4096 46.9 and 54.7, 1024 x 1024 4.1 and 4.2.  At 16 rows the tokens' values weigh as much as the weights here,
+// and the tiles' LDS pays: 10.6 and 10.7, 32.0 and 24.0, 29.0 and 25.5, 60.7 and 55.5, 4.6 and 4.2.
+bool half_few_fits(int T) { return T <= 8; }
 
-template <int WTY, int RT, int TG, int U, int NW>
+template <int WTY, int RT, int U, int NW>
 static void launch_few(const HalfArgs& a, hipStream_t stream) {
-    const dim3 grid((a.n_out + 8 * RT - 1) / (8 * RT), (a.T + 8 * TG - 1) / (8 * TG));
+    const dim3 grid((a.n_out + 8 * RT - 1) / (8 * RT), (a.T + 7) / 8);
     const bool lines = a.k % HALF_PAIR == 0 && (uintptr_t)a.x % 16 == 0 && (a.T <= 1 || a.ldx % 8 == 0);
     if (lines)
-        hipLaunchKernelGGL((k_half_few<WTY, RT, TG, U, NW, 1>), grid, dim3(64 * NW), 0, stream, a);
+        hipLaunchKernelGGL((k_half_few<WTY, RT, U, NW, 1>), grid, dim3(64 * NW), 0, stream, a);
     else
-        hipLaunchKernelGGL((k_half_few<WTY, RT, TG, U, NW, 0>), grid, dim3(64 * NW), 0, stream, a);
+        hipLaunchKernelGGL((k_half_few<WTY, RT, U, NW, 0>), grid, dim3(64 * NW), 0, stream, a);
 }
 // 16 weight rows a workgroup read each token's values for twice as many products as 8, and leave half as many workgroups:
 // taken from three tokens on where their last round over the 256 CUs is full enough (4096 x 4096 at 8 tokens 9.2 us and
@@ -130,11 +122,10 @@ static void launch_few(const HalfArgs& a, hipStream_t stream) {
 template <int WTY>
 static void launch_some(const HalfArgs& a, hipStream_t stream) {
     const int64_t wgs = ((int64_t)a.n_out + 15) / 16, rounds = (wgs + 255) / 256;
-    const bool two = a.T > 2 && 5 * wgs >= 4 * 256 * rounds;
-    if (a.T > 8)
-        two ? launch_few<WTY, 2, 2, 1, 8>(a, stream) : launch_few<WTY, 1, 2, 2, 8>(a, stream);
+    if (a.T > 2 && 5 * wgs >= 4 * 256 * rounds)
+        launch_few<WTY, 2, 1, 8>(a, stream);
     else
-        two ? launch_few<WTY, 2, 1, 1, 8>(a, stream) : launch_few<WTY, 1, 1, 2, 8>(a, stream);
+        launch_few<WTY, 1, 2, 8>(a, stream);
 }
 
 // (any number of tokens, for rows that a tile's offsets do not reach: as many a launch as a grid holds)

@@ -12,15 +12,16 @@ static const TileOf TILES[] = {SYN_HALF_TILES(SYN_HALF_TILE)};
 #undef SYN_HALF_TILE
 
 // The tile and the parts of K that are estimated to take least: rounds of 256 workgroups, the last one's faster the fewer
-// there are in it, beside what the weights take from HBM (6.0 TB/s at most, 48 GB/s a workgroup, and part of a reading
+// there are in it, beside what the weights take from HBM (5.6 TB/s at most, 92 GB/s a workgroup, and part of a reading
 // more for every further tile of tokens): the longer of the two and a quarter of the other; K in parts costs the
-// fold's launch and its partial sums' writing and reading.  The constants are a fit to 200 measured calls; of 29
-// matrices and row counts 24 run on the fastest choice, three within 8 % of it, two at 11 and 12.  Large tiles read less from L2
+// fold's launch and its partial sums' writing and reading.  The constants are a fit to 500 measured calls; of 51 matrices
+// and row counts 43 run on the fastest choice, 6 within 8 % of it, two at 11 and 14.  Large tiles read less from L2
 // for an output, small ones fill the chip: 4096 x 4096 at 512 tokens takes 27 us in 256 tiles of 64 x 128 and 37 in
-// 128 of 128 x 128, 14336 x 4096 at 2048 tokens 202 in 448 of 256 x 256 and 232 in 1792 of 128 x 128.
+// 128 of 128 x 128, at 32 tokens 11.5 in 128 of 32 x 32 and 12.7 in 64 of 64 x 32 by four parts of K; 14336 x 4096 at 2048
+// tokens 202 in 448 of 256 x 256 and 232 in 1792 of 128 x 128.
 HalfPick half_gemm_pick(int n_out, int k, int T) {
-    constexpr float LAUNCH = 2.0f, FOLD = 2.2f;                     // us
-    constexpr float HBM = 6.0e6f, EACH = 4.85e4f, SUMS = 4.5e6f;    // bytes a us
+    constexpr float LAUNCH = 2.3f, FOLD = 3.0f;                     // us
+    constexpr float HBM = 5.6e6f, EACH = 9.2e4f, SUMS = 5.4e6f;     // bytes a us
     const int kp = (int)half_padded(k);
     HalfPick best{0, 1};
     float least = 0.0f;
@@ -31,7 +32,7 @@ HalfPick half_gemm_pick(int n_out, int k, int T) {
         for (int s = 1; s <= 8; s = s < 4 ? s + 1 : s + 2) {
             const int64_t wgs = tw * tt * s, rounds = (wgs + 255) / 256;
             if (s > 1 && (kp < 512 * s || wgs > 256)) break;  // (a part has four stages and more)
-            const float last = (float)(wgs - 256 * (rounds - 1)) / 256.0f, turns = (float)rounds - 0.43f + 0.43f * last;
+            const float last = (float)(wgs - 256 * (rounds - 1)) / 256.0f, turns = (float)rounds - 0.26f + 0.26f * last;
             const float work = (float)rounds * t.base + turns * t.per_k * (float)kp / (float)s;
             const float rate = EACH * (float)wgs < HBM ? EACH * (float)wgs : HBM;
             const float read = bytes / rate;

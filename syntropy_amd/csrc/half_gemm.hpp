@@ -46,7 +46,6 @@ struct HalfTile {
     static_assert(PIECES < 8 || NW % 2 == 0 || WIDE, "a wavefront's copies begin at rows of one parity");
     static_assert(WIDE || (RING >= 3 && CPW * (RING - 2) < 64), "vmcnt");
     static_assert(!WIDE || (WK == 1 && BM == BN && XPW == WPW && WPW <= MT * NT && MT + NT <= MT * NT), "copies and reads beside products");
-    static_assert(MT * NT >= 2, "reads beside one product, copies beside another");
     static_assert(LDS <= 160 * 1024, "LDS");
     static_assert(2 * HALF_PAIR % LINE == 0, "a row is whole stages");
 };
@@ -135,10 +134,11 @@ __global__ __launch_bounds__(64 * C::NW, C::MT* C::NT >= 16 ? 1 : 2) void k_half
             constexpr int m = decltype(mc)::value, i = m / NT, j = m % NT;
             acc[i][j] = half_mfma32<WTY>(a[kk][i], b[kk][j], acc[i][j]);
             // reads in the first half of the products (one or more a product), copies in the second
-            constexpr int H = M / 2;
+            constexpr int H = M > 1 ? M / 2 : 1;
             constexpr int r0 = m < H ? m * R / H : R, r1 = m < H ? (m + 1) * R / H : R;
             if constexpr (r1 > r0) static_for<r1 - r0>([&](auto rc) { read(rs, 1 - kk, r0 + decltype(rc)::value); });
-            constexpr int c0 = m >= H ? (m - H) * CP / (M - H) : 0, c1 = m >= H ? (m - H + 1) * CP / (M - H) : 0;
+            constexpr int L = M > 1 ? M - H : 1, l = M > 1 ? m - H : 0;
+            constexpr int c0 = l >= 0 ? l * CP / L : 0, c1 = l >= 0 ? (l + 1) * CP / L : 0;
             if constexpr (c1 > c0) static_for<c1 - c0>([&](auto cc) { copy(v, first + c0 + decltype(cc)::value); });
             __builtin_amdgcn_sched_barrier(0);
         });
@@ -431,14 +431,14 @@ __global__ __launch_bounds__(64 * C::NW, C::MT* C::NT >= 16 ? 1 : 2) void k_half
 }
 
 // The tiles: wavefronts over weight rows, tokens and K, each one's 32-row and 32-token tiles, the ring's stages (0: WIDE);
-// then what a workgroup that has a CU to itself takes beside K and a 1024 values of K, in tenths of a microsecond
-// (BF16, 4096 x 4096, 14336 x 4096 and 4096 x 14336 matrices at 32 to 2048 tokens).
+// then what a workgroup takes beside K and a 1024 values of K, in tenths of a microsecond (a fit, half_gemm.hip).
 #define SYN_HALF_TILES(X)             \
-    X(0, 4, 2, 1, 2, 4, 0, 77, 191)   \
-    X(1, 2, 2, 1, 2, 2, 0, 28, 77)    \
-    X(2, 1, 2, 2, 2, 2, 4, 19, 58)    \
-    X(3, 1, 1, 4, 2, 2, 4, 19, 36)    \
-    X(4, 1, 1, 4, 2, 1, 4, 19, 26)
+    X(0, 4, 2, 1, 2, 4, 0, 45, 213)   \
+    X(1, 2, 2, 1, 2, 2, 0, 24, 80)    \
+    X(2, 1, 2, 2, 2, 2, 4, 17, 58)    \
+    X(3, 1, 1, 4, 2, 2, 4, 20, 33)    \
+    X(4, 1, 1, 4, 2, 1, 4, 15, 24)    \
+    X(5, 1, 1, 4, 1, 1, 4, 9, 18)
 
 template <class C, int WTY, int OT>
 static void launch_as(const HalfArgs& a, hipStream_t stream) {
