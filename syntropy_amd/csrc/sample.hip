@@ -83,8 +83,9 @@ struct Scale {
         uint64_t whole;
     };
     static SYN_DEV int bin(double s) { return (int)__builtin_rint(__builtin_fmin(s, (double)(SB - 1))); }
-    SYN_DEV Part part(double s) const {
-        const double t = __builtin_fmin(s, (double)(SB - 1)), n = __builtin_rint(t), y = t - n;
+    SYN_DEV Part part(double s) const { return inside(__builtin_fmin(s, (double)(SB - 1))); }
+    SYN_DEV Part inside(double s) const {
+        const double n = __builtin_rint(s), y = s - n;
         // exp(L y) one, whose 1 one is added with 2^52: the sum's last bits are the whole number
         double p = __builtin_fma(y, EXPS[4], EXPS[3]);
         p = __builtin_fma(p, y, EXPS[2]);
@@ -107,6 +108,7 @@ struct Wanted {
     int a0, a1, b;   // (b: none where negative)
     int cut;         // BINS: the bin of the border (none: -1)
     bool by_p, by_min_p;
+    bool only;       // BINS: only the border's bin, for the list holds not all; the token's after it
     uint32_t n;      // how many values that is (0: not known), or more than LIST: no list
     float lo, hi, lo2, hi2;  // the values from lo to below hi and from lo2 to below hi2
     // The list: its first n0 values are a0's to a1's, which `sum0` stands before, the others b's, which `sum1` does; the
@@ -306,15 +308,33 @@ struct Sampler : Reader<TY> {
     }
 
     // ---- the bins -------------------------------------------------------------------------------------------
+    SYN_DEV float s32(float v) const { return ((float)sc.m - v) * (float)sc.c; }
     SYN_DEV int bin32(float v) const {
-        const float s = ((float)sc.m - v) * (float)sc.c;
+        const float s = s32(v);
         return s < (float)(SB - 1) ? (int)s : SB - 1;
     }
-    SYN_DEV void add_to_bin(float v) {
-        if (v == -__builtin_inff()) return;
-        const Scale::Part p = sc.part(sc.s(v));
-        atomicAdd(&r.counts[p.bin], 1u);
-        atomicAdd((unsigned long long*)&r.masses[p.bin], (unsigned long long)p.whole);
+    // (what is beyond the last bin is counted by each thread: of a cold row it is most, and a bin's sums are added one lane
+    // after the other.  A row of 128256 BF16 with a third there 171 us, 60 so)
+    SYN_DEV void add_to_bin(float v, uint32_t& beyond) {
+        const double s = sc.s(v);
+        if (s < (double)(SB - 1)) {
+            const Scale::Part p = sc.inside(s);
+            atomicAdd(&r.counts[p.bin], 1u);
+            atomicAdd((unsigned long long*)&r.masses[p.bin], (unsigned long long)p.whole);
+        } else {
+            beyond += v > -__builtin_inff() ? 1 : 0;
+        }
+    }
+    // (every thread) each of the weight 2^-64 at most
+    SYN_DEV void add_beyond(uint32_t beyond) {
+#pragma unroll
+        for (int d = 32; d > 0; d /= 2) beyond += __shfl_xor(beyond, d);
+        if ((threadIdx.x & 63) == 0 && beyond) {
+            const Scale::Part p = sc.part((double)(SB - 1));
+            atomicAdd(&r.counts[SB - 1], beyond);
+            atomicAdd((unsigned long long*)&r.masses[SB - 1], (unsigned long long)(p.whole * beyond));
+        }
+        __syncthreads();
     }
     SYN_DEV void no_bins() {
         for (int i = threadIdx.x; i < SB; i += ST) r.counts[i] = 0, r.masses[i] = 0;
@@ -323,13 +343,18 @@ struct Sampler : Reader<TY> {
     // The counts (and sums) of the bins over this workgroup's values.
     SYN_DEV void bins(Mode mode) {
         no_bins();
+        uint32_t beyond = 0;
         if (mode == LIST_K)
             each([&](float v, int) {
-                if (v != -__builtin_inff()) atomicAdd(&r.counts[bin32(v)], 1u);
+                const float s = s32(v);
+                if (s < (float)(SB - 1))
+                    atomicAdd(&r.counts[(int)s], 1u);
+                else
+                    beyond += v > -__builtin_inff() ? 1 : 0;
             });
         else
-            each([&](float v, int) { add_to_bin(v); });
-        __syncthreads();
+            each([&](float v, int) { add_to_bin(v, beyond); });
+        add_beyond(beyond);
     }
     // (every thread) The counts and sums of the bins before each, in place.  (Whole numbers: a sum grows exactly where a bin
     // holds something.)
@@ -375,8 +400,8 @@ struct Sampler : Reader<TY> {
     }
 
     // ---- what to gather -------------------------------------------------------------------------------------
-    // (every thread gets it) LIST_TOP: from 1024 numbers in r.run's place, each the greatest of a part of the row.
-    SYN_DEV Wanted want_top() {
+    // Into r.want.  LIST_TOP: from 1024 numbers in r.run's place, each the greatest of a part of the row.
+    SYN_DEV void want_top() {
         if (threadIdx.x < 64) {
             const uint32_t* tops = reinterpret_cast<const uint32_t*>(r.run);
             uint32_t of[4];
@@ -397,10 +422,9 @@ struct Sampler : Reader<TY> {
             if (threadIdx.x == 0) r.want = w;
         }
         __syncthreads();
-        return r.want;
     }
-    // (every thread gets it) Of the other modes, from the bins (which are prefixes behind it).
-    SYN_DEV Wanted want(Mode mode) {
+    // Of the other modes, from the bins (which are prefixes behind it).
+    SYN_DEV void want(Mode mode) {
         if (mode != LIST_MIN_P) prefix();
         if (threadIdx.x < 64) {
             Wanted w = wanted(mode);
@@ -408,7 +432,6 @@ struct Sampler : Reader<TY> {
             if (threadIdx.x == 0) r.want = w;
         }
         __syncthreads();
-        return r.want;
     }
     // (one wavefront) The least values of the bins from a1, a0 - 1, b and b - 1 up, the wanted ones' edges: by 16 numbers at
     // a time between one that is below and one that is not, 16 lanes an edge.
@@ -474,11 +497,18 @@ struct Sampler : Reader<TY> {
             w.i0 = w.b >= 0 ? w.n0 : (int)(r.counts[w.cut] - r.counts[w.a0]);
             w.end = w.i0 + (int)r.in(w.cut);
             w.before = r.counts[w.cut], w.under = base(w.cut);
+            if (w.n > (uint32_t)LIST && r.in(w.cut) <= (uint32_t)LIST) {
+                w.only = true;
+                w.a0 = w.a1 = w.cut, w.b = -1;
+                w.i0 = 0, w.end = w.n0 = (int)r.in(w.cut), w.n = r.in(w.cut);
+                w.sum0 = w.under;
+            }
         }
         return w;
     }
     // The keys of the wanted among this workgroup's values into r.keys, those that find room; r.n: how many there are.
-    SYN_DEV void pick(Mode mode, const Wanted& w) {
+    SYN_DEV void pick(Mode mode) {
+        const Wanted& w = r.want;
         if (threadIdx.x == 0) r.n = 0;
         __syncthreads();
         auto put = [&](float v, int i) {
@@ -666,21 +696,39 @@ struct Sampler : Reader<TY> {
     static SYN_DEV void write_none(const SampleArgs& g, uint64_t row) {
         if (threadIdx.x == 0) g.token[row] = -1, g.logprob[row] = __builtin_nanf(""), g.kept[row] = 0;
     }
-    // The row's results from the n wanted values in r.keys (where they are no more than LIST), by one wavefront; else from
-    // the bins and the row, all of which this workgroup then reads.
-    SYN_DEV void finish(const SampleArgs& g, uint64_t row, Mode mode, const Wanted& w, uint32_t n) {
-        if (n > (uint32_t)LIST) {
-            seldom(g, row, mode);
-            return;
+    // The row's results from the n wanted values, which this workgroup gathers now or which are in r.keys; the sums by one
+    // wavefront.  Where they are more than LIST, from the bins and the row.
+    SYN_DEV void finish(const SampleArgs& g, uint64_t row, Mode mode, uint32_t n, bool there) {
+#pragma unroll 1
+        for (;;) {
+            if (!there && n <= (uint32_t)LIST) {
+                pick(mode);
+                n = r.n;
+            }
+            if (n > (uint32_t)LIST) {
+                seldom(g, row, mode);
+                return;
+            }
+            if (mode == BINS) {  // (bin b after a1: nothing between them)
+                const int a1 = r.want.a1, b = r.want.b;
+                order((int)n, (double)r.want.a0 - 0.5, b >= 0 ? (double)(b - a1 - 1) : 0.0, (double)a1 + (b >= 0 ? 1.5 : 0.5));
+            } else {
+                order((int)n, 0.0, 0.0, mode == LIST_MIN_P ? last : (double)r.want.a1 + 1.0);
+            }
+            const bool only = r.want.only;
+            if (only) __syncthreads();
+            if (threadIdx.x < 64) results(g, row, mode, n);
+            if (!only) return;
+            __syncthreads();
+            if (!r.at) return;
+            n = r.want.n, there = false;
         }
-        if (mode == BINS) {  // (bin b after a1: nothing between them)
-            const double gap = w.b >= 0 ? (double)(w.b - w.a1 - 1) : 0.0, end = (double)w.a1 + (w.b >= 0 ? 1.5 : 0.5);
-            order((int)n, (double)w.a0 - 0.5, gap, end);
-        } else {
-            order((int)n, 0.0, 0.0, mode == LIST_MIN_P ? last : (double)w.a1 + 1.0);
-        }
-        if (threadIdx.x >= 64) return;
+    }
+    // (one wavefront) From the list; of `only` the border's bin, the token too if it lies there, else what holds it is wanted
+    // next (r.at).
+    SYN_DEV void results(const SampleArgs& g, uint64_t row, Mode mode, uint32_t n) {
         run_up((int)n);
+        const Wanted& w = r.want;
         const bool bins = mode == BINS, cut = !bins || w.cut >= 0;
         const int n0 = bins ? w.n0 : (int)n, i0 = w.i0;
         int end = bins ? w.end : k < n ? (int)k : (int)n;
@@ -697,6 +745,21 @@ struct Sampler : Reader<TY> {
         const double all = !cut ? w.all : end > i0 ? run(end - 1) : w.under;
         // (where nothing of the cut's own bin is kept, the token lies in the first range)
         const double pass = (double)u * all;
+        if (w.only) {
+            const bool next = pass < w.under;
+            if (threadIdx.x == 0) r.at = next;
+            if (next) {
+                Wanted t{};
+                t.b = t.cut = -1;
+                t.a0 = t.a1 = bin_of(SUM_PASSES, 0, pass);
+                t.n = r.in(t.a0), t.n0 = t.end = (int)t.n;
+                t.sum0 = base(t.a0);
+                t.total = kept, t.all = all;
+                edges(mode, t);
+                if (threadIdx.x == 0) r.want = t;
+                return;
+            }
+        }
         const int stop = end > 0 ? end : 1, at = first((int)n, 0, stop, [&](int i) { return run(i) > pass; });
         write(g, row, kept, all, r.keys[at < stop ? at : stop - 1]);
     }
@@ -775,8 +838,9 @@ struct Sampler : Reader<TY> {
     SYN_DEV void seldom(const SampleArgs& g, uint64_t row, Mode mode) {
         if (mode != BINS) {
             no_bins();
-            every([&](float v, int) { add_to_bin(v); });
-            __syncthreads();
+            uint32_t beyond = 0;
+            every([&](float v, int) { add_to_bin(v, beyond); });
+            add_beyond(beyond);
             prefix();
         }
         Place cut{r.counts[SB], base(SB), 0};
@@ -830,13 +894,11 @@ __global__ __launch_bounds__(ST) void k_sample(SampleArgs g) {
     }
     const Mode mode = sp.mode();
     if (mode == LIST_K || mode == BINS) sp.bins(mode);
-    const Wanted w = mode == LIST_TOP ? sp.want_top() : sp.want(mode);
-    uint32_t n = w.n;
-    if (n <= (uint32_t)LIST) {
-        sp.pick(mode, w);
-        n = r.n;
-    }
-    sp.finish(g, row, mode, w, n);
+    if (mode == LIST_TOP)
+        sp.want_top();
+    else
+        sp.want(mode);
+    sp.finish(g, row, mode, r.want.n, false);
 }
 
 // ---- few long rows: a row's parts, a launch a step ------------------------------------------------------------
@@ -898,13 +960,16 @@ __global__ __launch_bounds__(ST) void k_sample_bins(SampleArgs g, int parts) {
 }
 // What to gather, from the row's bins or tops.
 template <class S>
-SYN_DEV Wanted want_shared(S& sp, const Shared& s, Row& r, Mode mode) {
-    if (mode == LIST_TOP) return sp.want_top();
+SYN_DEV void want_shared(S& sp, const Shared& s, Row& r, Mode mode) {
+    if (mode == LIST_TOP) {
+        sp.want_top();
+        return;
+    }
     if (mode != LIST_MIN_P) {
         for (int i = threadIdx.x; i < SB; i += ST) r.counts[i] = s.counts[i], r.masses[i] = s.masses[i];
         __syncthreads();
     }
-    return sp.want(mode);
+    sp.want(mode);
 }
 template <int TY>
 __global__ __launch_bounds__(ST) void k_sample_pick(SampleArgs g, int parts) {
@@ -914,11 +979,11 @@ __global__ __launch_bounds__(ST) void k_sample_pick(SampleArgs g, int parts) {
     Shared& s = ((Shared*)g.ws)[row];
     if (!sp.settle(gather_tops(sp, r, s, parts))) return;
     const Mode mode = sp.mode();
-    const Wanted w = want_shared(sp, s, r, mode);
+    want_shared(sp, s, r, mode);
     if (blockIdx.x % (uint32_t)parts == 0 && threadIdx.x < sizeof(Wanted) / 4)
         reinterpret_cast<uint32_t*>(&s.want)[threadIdx.x] = reinterpret_cast<const uint32_t*>(&r.want)[threadIdx.x];
-    if (w.n > (uint32_t)LIST) return;
-    sp.pick(mode, w);
+    if (r.want.n > (uint32_t)LIST) return;
+    sp.pick(mode);
     // (a place for all of this workgroup's at once: one by one, 24 rows' lists took 7 us more)
     const uint32_t n = r.n;
     if (threadIdx.x == 0) r.at = n ? atomicAdd(&s.n, n) : 0;
@@ -938,17 +1003,19 @@ __global__ __launch_bounds__(ST) void k_sample_end(SampleArgs g, int parts) {
         return;
     }
     const Mode mode = sp.mode();
-    const Wanted w = s.want;
-    const uint32_t n = w.n <= (uint32_t)LIST ? s.n : w.n;
-    if (n <= (uint32_t)LIST) {
+    if (threadIdx.x < sizeof(Wanted) / 4)
+        reinterpret_cast<uint32_t*>(&r.want)[threadIdx.x] = reinterpret_cast<const uint32_t*>(&s.want)[threadIdx.x];
+    __syncthreads();
+    const uint32_t n = r.want.n <= (uint32_t)LIST ? s.n : r.want.n;
+    if (n <= (uint32_t)LIST)
         for (int i = threadIdx.x; i < (int)n; i += ST) r.keys[i] = s.keys[i];
-    } else if (mode == BINS) {
+    if (mode == BINS && (n > (uint32_t)LIST || r.want.only)) {
         for (int i = threadIdx.x; i < SB; i += ST) r.counts[i] = s.counts[i], r.masses[i] = s.masses[i];
         __syncthreads();
         sp.prefix();
     }
     __syncthreads();
-    sp.finish(g, row, mode, w, n);
+    sp.finish(g, row, mode, n, true);
 }
 
 // How many workgroups share a row: as many as fill the chip twice, of 8192 values at least.

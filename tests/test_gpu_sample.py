@@ -53,7 +53,9 @@ def one(z, u, temperature, top_k, top_p, min_p):
     return int(order[at]), np.log(w[at] / run[-1]), n, gap
 
 
-def check(S, x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, near=1e-11, what=""):
+def check(S, x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, near=1e-11, what="", ends=0):
+    """ends: rows whose u is the greatest.  What is behind it, 2^-24 of the sum, may be thousands of values of less than
+    `near` each: such a row's token is one whose share of [0, 1) reaches to within `near` of u."""
     r = S.sample_tokens(x, u, temperature, top_k, top_p, min_p)
     rows = x.shape[0]
     z, us = x.double().cpu().numpy(), u.double().cpu().numpy()
@@ -67,10 +69,15 @@ def check(S, x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, near=1e-11, w
         tok, lp, n, gap = one(z[i], us[i], at(temperature, i), at(top_k, i), at(top_p, i), at(min_p, i))
         if gap < near:  # (the 64-bit sums of the test are not exact either)
             skipped += 1
+            if ends and us[i] == 1 - 2.0 ** -24:
+                order = np.argsort(-z[i], kind="stable")[:got[2][i]]
+                run = np.cumsum(np.exp((z[i][order] - z[i][order[0]]) / at(temperature, i)))
+                place = int(np.nonzero(order == got[0][i])[0][0])
+                assert run[place] / run[-1] > us[i] - near and (run[place - 1] if place else 0.0) / run[-1] < us[i] + near
             continue
         assert (got[0][i], got[2][i]) == (tok, n), f"{what} row {i}: token {got[0][i]}, kept {got[2][i]}, not {tok}, {n}"
         assert abs(got[1][i] - lp) <= 2.0 ** -24 * abs(lp) + 1e-9, f"{what} row {i}: logprob {got[1][i]}, not {lp}"
-    assert skipped <= rows // 20, f"{skipped} rows next to a border"
+    assert skipped <= rows // 20 + ends, f"{skipped} rows next to a border"
 
 
 FILTERS = [dict(), dict(top_k=1), dict(top_k=7), dict(top_k=300), dict(top_p=0.9), dict(top_p=0.01), dict(top_p=0.9999), dict(min_p=0.1),
@@ -228,3 +235,92 @@ def test_strided_rows_streams_and_graphs(S):
 def test_no_rows(S):
     r = S.sample_tokens(torch.zeros(0, 50, device="cuda"), torch.zeros(0, device="cuda"))
     assert [t.shape for t in r] == [(0,)] * 3
+
+
+def spread(rows):
+    """How often rows are repeated to be more than are shared out between workgroups."""
+    return -(-200 // rows)
+
+
+@pytest.mark.parametrize("ty", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("temperature", [0.5, 1.4, 3.0, 5.0, 30.0])
+def test_flat_rows(S, ty, temperature):
+    """Bins of hundreds and of thousands of values: border and token in one list, in two, and past a list."""
+    rows, vocab = 6, 128256
+    x = (2 * real(7, rows, vocab)).to(ty)
+    u = uniform(8, rows)
+    u[0], u[1] = 0.0, 1 - 2.0 ** -24
+    for kw in (dict(), dict(top_p=0.93), dict(top_p=0.4), dict(min_p=0.2), dict(top_p=0.8, min_p=0.05), dict(top_p=0.6, top_k=60000)):
+        announce(f"sample flat {ty} {temperature} {kw}")
+        check(S, x, u, temperature, what=f"{kw}", ends=1, **kw)
+        n = spread(rows)
+        few, many = S.sample_tokens(x, u, temperature, **kw), S.sample_tokens(x.repeat(n, 1), u.repeat(n), temperature, **kw)
+        for a, b in zip(few, many):
+            assert torch.equal(a.repeat(n), b), kw
+
+
+@pytest.mark.parametrize("ty", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,vocab", [(4, 9000), (4, 131071), (130, 70001)])
+def test_most_of_a_row_far_below(S, rows, vocab, ty):
+    """Weights below 2^-64 beside a few that count: they are counted, and never the token."""
+    x = real(3, rows, vocab) - 300
+    x.scatter_(1, torch.randint(vocab, (rows, 150), generator=torch.Generator(device="cuda").manual_seed(4), device="cuda"),
+               2 * real(5, rows, 150))
+    x = x.to(ty)
+    u = uniform(6, rows)
+    u[0], u[-1] = 1 - 2.0 ** -24, 0.0
+    for kw in (dict(), dict(top_k=400), dict(top_k=60), dict(top_k=5000), dict(top_p=0.99), dict(min_p=1e-4), dict(top_p=0.5, min_p=0.3)):
+        announce(f"sample far {rows} {vocab} {ty} {kw}")
+        check(S, x[:4], u[:4], what=f"{kw}", ends=1, **kw)
+        many, few = S.sample_tokens(x, u, **kw), S.sample_tokens(x[:4], u[:4], **kw)
+        assert all(torch.equal(a[:4], b) for a, b in zip(many, few))
+
+
+@pytest.mark.parametrize("ty", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+def test_long_rows_shared_by_workgroups(S, ty):
+    """Each way to a row's list, in rows that several workgroups read, each row with its own settings."""
+    rows, vocab = 14, 100003
+    x = 2 * real(11, rows, vocab)
+    x.scatter_(1, torch.randint(vocab, (rows, 9), generator=torch.Generator(device="cuda").manual_seed(12), device="cuda"),
+               11 + 2 * real(13, rows, 9))
+    x[5:7] = x[5:7].bfloat16().float()
+    x = x.to(ty)
+    none = torch.tensor([0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 1, 1, 1], dtype=torch.bool)
+    x[11], x[12, 99999], x[13, 7] = -float("inf"), float("nan"), float("inf")
+    t = torch.tensor([1, .7, 0, 1.2, .9, 1, 1.1, 2, .5, 1, .8, 1, 1, 1], device="cuda")
+    k = torch.tensor([0, 7, 0, 64, 65, 700, 1984, 1985, 30000, 0, 0, 3, 0, 900], dtype=torch.int32, device="cuda")
+    p = torch.tensor([1, .9, 1, 1, .95, 1, .99, .8, .9, .9, 1, .9, 1, 1], device="cuda")
+    mp = torch.tensor([0, 0, 0, 0, .001, 0, 0, 0, .0001, .01, .02, 0, 0, .1], device="cuda")
+    for seed in range(3):
+        u = uniform(20 + seed, rows)
+        check(S, x[:11], u[:11], t[:11], k[:11], p[:11], mp[:11])
+        r = S.sample_tokens(x, u, t, k, p, mp)
+        assert r.token.cpu()[none].tolist() == [-1] * 3 and r.kept.cpu()[none].tolist() == [0] * 3
+        assert bool(torch.isnan(r.logprob.cpu()[none]).all())
+        n = spread(rows)
+        many = S.sample_tokens(x.repeat(n, 1), u.repeat(n), t.repeat(n), k.repeat(n), p.repeat(n), mp.repeat(n))
+        for a, b in zip(r, many):
+            assert torch.equal(torch.nan_to_num(a.float(), -9.0).repeat(n), torch.nan_to_num(b.float(), -9.0))
+
+
+def test_two_calls_at_once(S):
+    """On two streams, each with its own workspace, and a call that is replayed between them."""
+    xs, us = [2 * real(i, 5, 128256) for i in range(3)], [uniform(9 + i, 5) for i in range(3)]
+    want = [S.sample_tokens(x, u, top_p=0.95) for x, u in zip(xs, us)]
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        kept = S.sample_tokens(xs[2], us[2], top_p=0.95)
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in sides:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(6):
+        for i, s in enumerate(sides):
+            got[i].append(S.sample_tokens(xs[i], us[i], top_p=0.95, stream=s))
+        g.replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
+    assert all(torch.equal(a, b) for a, b in zip(kept, want[2]))
