@@ -322,7 +322,7 @@ int syn_block_norm(int32_t xtype, const void* x, uint64_t x_stride, int32_t btyp
  * +infinity among its logits, with no visible logit, or with a NaN setting, u, or a temperature that is none of the
  * above has the token -1, kept 0 and logprob NaN.
  * Sums are held to about 2^-62 vocab of a weight, in an order that does not matter: equal calls give equal tokens.
- * Weights below 2^-64 of the greatest count as 0.  Fewer than 2^24 rows of at most SYN_SAMPLE_MAX_VOCAB logits.
+ * Weights below 2^-64 of the greatest count as that at most.  Fewer than 2^24 rows of at most SYN_SAMPLE_MAX_VOCAB logits.
  * ws: 256-byte aligned, syn_sample_tokens_workspace_bytes (0: may be NULL).  No counterpart in the reference. */
 #define SYN_SAMPLE_MAX_VOCAB (1 << 24)
 int syn_sample_tokens_workspace_bytes(int32_t xtype, uint32_t rows, uint32_t vocab, uint64_t* bytes);

@@ -129,8 +129,20 @@ __global__ __launch_bounds__(64 * (WAVES > 1 ? WAVES : BN_ROWS)) void k_block_no
 
 template <int TX, int TB, int WAVES, int P>
 static void launch_as(const BlockNormArgs& a, hipStream_t stream) {
-    constexpr int ROWS = WAVES > 1 ? 1 : BN_ROWS;
-    hipLaunchKernelGGL((k_block_norm<TX, TB, WAVES, P>), dim3((a.rows + ROWS - 1) / ROWS), dim3(64 * WAVES * ROWS), 0, stream, a);
+    constexpr int ROWS = WAVES > 1 ? 1 : BN_ROWS, MOST = 1 << 20;  // (a launch's threads are counted in 32 bits)
+    auto at = [](const void* p, int ty, uint64_t ld, int t) {
+        return p ? (const uint8_t*)p + (uint64_t)t * ld * (ty == T_F32 ? 4 : 2) : nullptr;
+    };
+    for (int t = 0; t < a.rows; t += MOST) {
+        BlockNormArgs g = a;
+        g.rows = a.rows - t < MOST ? a.rows - t : MOST;
+        g.x = at(a.x, TX, a.ldx, t);
+        g.branch = at(a.branch, TB, a.ldb, t);
+        g.gate = at(a.gate, TB, a.ldg, t);  // (ldg 0: one for all)
+        g.h = (void*)at(a.h, TX, a.ldh, t);
+        g.y = (void*)at(a.y, a.ytype, a.ldy, t);
+        hipLaunchKernelGGL((k_block_norm<TX, TB, WAVES, P>), dim3((g.rows + ROWS - 1) / ROWS), dim3(64 * WAVES * ROWS), 0, stream, g);
+    }
 }
 // As many wavefronts as hold a row in one or two pieces a lane: more rows are in flight than with more pieces or with more
 // wavefronts (2048 rows of 8192 on 16 wavefronts 44 us, on 8 31; 32768 of 512 on four 89, on one 26).

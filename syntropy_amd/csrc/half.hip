@@ -62,10 +62,13 @@ void launch_half_gemv(const HalfArgs& in, bool lines, uint8_t* ws, hipStream_t s
     }
     const HalfPick p = half_gemm_pick(a.n_out, a.k, a.T);
     if (!lines) {
-        const int kp = (int)half_padded(a.k);
-        const uint64_t pieces = (uint64_t)a.T * (uint64_t)(kp / 8);
-        hipLaunchKernelGGL(k_half_rows, dim3((uint32_t)((pieces + 255) / 256)), dim3(256), 0, stream, a.x, a.ldx, a.T, a.k, kp,
-                           (uint16_t*)ws);
+        const int kp = (int)half_padded(a.k), most = (1 << 30) / (kp / 8);  // (a launch's threads are counted in 32 bits)
+        for (int t = 0; t < a.T; t += most) {
+            const int rows = a.T - t < most ? a.T - t : most;
+            const uint64_t pieces = (uint64_t)rows * (uint64_t)(kp / 8);
+            hipLaunchKernelGGL(k_half_rows, dim3((uint32_t)((pieces + 255) / 256)), dim3(256), 0, stream, a.x + (uint64_t)t * a.ldx,
+                               a.ldx, rows, a.k, kp, (uint16_t*)ws + (uint64_t)t * (uint64_t)kp);
+        }
         a.x = (const uint16_t*)ws;
         a.ldx = (uint64_t)kp;
     }

@@ -13,9 +13,10 @@
 //
 // The row is read for its greatest value, for the bins, and for the list: the few values that a border or the token can
 // lie among.  A top-k needs no bins: up to TOP the k-th of the 256 groups' greatest values is a bound that only a few
-// values more than k reach, a longer one takes counts of F32 distances; with min-p alone the border is a value.  Only
-// equal values by the thousand make more of a bin than a list holds: then a border is found digit by digit of the
-// values' keys.
+// values more than k reach, a longer one takes counts of F32 distances; with min-p alone the border is a value.  In a flat
+// row the bins of border and token may hold more than a list: then they take one after the other (`only`).  More of a bin
+// than a list holds (a high temperature, equal values by the thousand), or a longer top-k: each border is found digit
+// by digit of the values' keys.
 // What bounds it is the arithmetic of a workgroup's passes (a CU takes 1024 threads' instruction in 16 cycles: 20
 // instructions a value are 0.08 us a 1024 values) and its steps between them; few long rows are therefore split over
 // workgroups, a launch a step.
@@ -1033,7 +1034,19 @@ template <int TY>
 static void sample_as(const SampleArgs& a, hipStream_t stream) {
     const int parts = sample_parts(a.xtype, a.rows, a.vocab);
     if (parts == 1) {
-        hipLaunchKernelGGL(k_sample<TY>, dim3(a.rows), dim3(ST), 0, stream, a);
+        constexpr int MOST = 1 << 20;  // (a launch's threads are counted in 32 bits)
+        for (int t = 0; t < a.rows; t += MOST) {
+            SampleArgs g = a;
+            g.rows = a.rows - t < MOST ? a.rows - t : MOST;
+            g.x = (const uint8_t*)a.x + (uint64_t)t * a.ldx * Reader<TY>::ES;
+            g.u = a.u + t;
+            if (a.temperature) g.temperature = a.temperature + t;
+            if (a.top_k) g.top_k = a.top_k + t;
+            if (a.top_p) g.top_p = a.top_p + t;
+            if (a.min_p) g.min_p = a.min_p + t;
+            g.token = a.token + t, g.logprob = a.logprob + t, g.kept = a.kept + t;
+            hipLaunchKernelGGL(k_sample<TY>, dim3(g.rows), dim3(ST), 0, stream, g);
+        }
         return;
     }
     const dim3 all((uint32_t)a.rows * (uint32_t)parts);

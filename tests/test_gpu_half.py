@@ -76,6 +76,9 @@ def near(got, want, err, what):
 SHAPES = [(1, 1, 1), (1, 64, 1), (7, 3, 2), (16, 64, 1), (33, 65, 3), (130, 640, 5), (64, 2048, 8), (257, 130, 9), (1000, 4096, 1),
           (96, 192, 16), (300, 1000, 17), (512, 1024, 31), (130, 8192, 33), (65, 63, 64), (1027, 320, 65), (256, 512, 128),
           (384, 257, 129), (520, 1344, 200), (1500, 704, 257), (72, 14336, 40), (2100, 448, 300), (4096, 192, 513)]
+# each tile, over whole K and over many parts of it
+SHAPES += [(12957, 81, 417), (6114, 6461, 129), (8306, 37, 132), (2754, 5090, 66), (8203, 36, 36), (76, 5898, 1370), (8776, 167, 33),
+           (101, 5689, 1406), (8324, 52, 9), (34, 5633, 738), (2982, 5916, 30), (33, 2878, 14), (4096, 256, 7), (4096, 193, 5)]
 
 
 @pytest.mark.parametrize("ty", [BF16, F16], ids=["bf16", "f16"])
