@@ -139,20 +139,25 @@ SYN_DEV void half_load(const void* p, int ty, uint64_t i, int in, float (&v)[N])
     }
 }
 
-// The same as they lie in memory, to be unpacked when they are used: N (4 or 8) values that are all there.
+// N (4 or 8) values that are all there as they lie in memory, at most 16 bytes, to be unpacked when they are used.
 template <int N>
-SYN_DEV void half_fetch(const void* p, int ty, uint64_t i, uint32_t (&raw)[N]) {
-    if (ty == T_F32)
-        __builtin_memcpy(raw, (const float*)p + i, 4 * N);
+struct HalfRaw {
+    uint32_t w[4];
+};
+template <int N>
+SYN_DEV void half_fetch(const void* p, int ty, uint64_t i, HalfRaw<N>& raw) {
+    if (N == 4 && ty == T_F32)
+        __builtin_memcpy(raw.w, (const float*)p + i, 16);
     else
-        __builtin_memcpy(raw, (const uint16_t*)p + i, 2 * N);
+        __builtin_memcpy(raw.w, (const uint16_t*)p + i, 2 * N);
 }
 template <int N>
-SYN_DEV void half_unpack(int ty, const uint32_t (&raw)[N], float (&v)[N]) {
+SYN_DEV void half_unpack(int ty, const HalfRaw<N>& raw, float (&v)[N]) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-        const uint32_t b = raw[j / 2] >> (16 * (j & 1)) & 0xFFFFu;
-        v[j] = ty == T_F32 ? u2f(raw[j]) : ty == T_F16 ? f16_to_f32(b) : u2f(b << 16);
+        const uint32_t b = raw.w[j / 2] >> (16 * (j & 1)) & 0xFFFFu;
+        v[j] = ty == T_F16 ? f16_to_f32(b) : u2f(b << 16);
+        if constexpr (N == 4) v[j] = ty == T_F32 ? u2f(raw.w[j]) : v[j];
     }
 }
 

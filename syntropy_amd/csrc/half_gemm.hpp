@@ -144,34 +144,34 @@ __global__ __launch_bounds__(64 * C::NW, C::MT* C::NT >= 16 ? 1 : 2) void k_half
         });
     };
 
-    // What the epilogue reads of one operand (the gate, else the residual) is fetched a unit of it ahead, the first
-    // unit before all else: a unit waits for memory otherwise, with nothing beside it.
+    // What the epilogue reads of gate and residual is fetched a unit of it ahead, the first unit before all else: a unit
+    // waits for memory otherwise, with nothing beside it.  (F32 operands of an output of 16 bits, twice as long, are not.)
     constexpr int IC = WK > 1 ? 1 : MT;                           // row tiles of an emission
     constexpr int OC = 32 * IC, PITCH = OC * 4 + 16;
     constexpr int PER = OT == OUT_16 ? 8 : 4, ROW = OC / PER;     // values of 16 bytes, pieces a token
     constexpr int TURNS = 32 * ROW / 64, GROUP = TURNS < 4 ? TURNS : 4, GROUPS = TURNS / GROUP;
     static_assert(64 % ROW == 0, "the same outputs each turn");
-    uint32_t ahead[2][GROUP][PER];
-    const void* const op = g.gate ? g.gate : g.res;
-    const int otype = g.gate ? g.gtype : g.rtype;
-    const uint64_t ldo = g.gate ? g.ldg : g.ldr;
+    HalfRaw<PER> gates[GROUP] = {}, sums[GROUP] = {};
+    const bool gates_ahead = g.gate && (OT == OUT_F32 || g.gtype != T_F32), res_ahead = g.res && (OT == OUT_F32 || g.rtype != T_F32);
     const int lo = lane % ROW * PER;                              // of the emission's outputs
-    auto fetch = [&](int i0, int j, int gi, uint32_t (&to)[GROUP][PER]) {
+    auto fetch = [&](int i0, int j, int gi) {
         if constexpr (OT != OUT_PART) {
+            if (!gates_ahead && !res_ahead) return;  // uniform
             const int tb = t0 + (wn * NT + j) * 32, nb = n0 + wm * 32 * MT + 32 * i0;
-            if (!op || nb + OC > g.n_out) return;  // uniform
 #pragma unroll
             for (int q = 0; q < GROUP; ++q) {
                 const int t = tb + (64 * (GROUP * gi + q) + lane) / ROW;
-                if (t < g.T) half_fetch<PER>(op, otype, (uint64_t)t * ldo + nb + lo, to[q]);
+                if (t >= g.T || nb + lo + PER > g.n_out) continue;
+                if (gates_ahead) half_fetch<PER>(g.gate, g.gtype, (uint64_t)t * g.ldg + nb + lo, gates[q]);
+                if (res_ahead) half_fetch<PER>(g.res, g.rtype, (uint64_t)t * g.ldr + nb + lo, sums[q]);
             }
         }
     };
     if constexpr (WK == 1) {
-        fetch(0, 0, 0, ahead[0]);
+        fetch(0, 0, 0);
     } else {
         static_assert(MT * NT % WK == 0 || MT * NT < WK, "as many tiles a part");
-        if (wk < MT * NT) fetch(wk / NT, wk % NT, 0, ahead[0]);
+        if (wk < MT * NT) fetch(wk / NT, wk % NT, 0);
     }
 
     if constexpr (C::WIDE) {
@@ -269,18 +269,43 @@ __global__ __launch_bounds__(64 * C::NW, C::MT* C::NT >= 16 ? 1 : 2) void k_half
             wave_lds_sync();
         }
     }
-    // The outputs of token tile j, row tiles i0 .. i0 + IC - 1; unit: how many units were before; (in, jn): the next ones.
-    auto emit = [&](auto jc, auto i0c, auto unitc, int in, int jn) {
-        constexpr int j = decltype(jc)::value, i0 = decltype(i0c)::value;
-        const int tb = t0 + (wn * NT + j) * 32, nb = n0 + wm * WR + 32 * i0;
+    // WK > 1: output tile q goes to the wavefront of part q % WK: the others' sums of it through LDS
+    auto area = [&](int part, int i, int j) {
+        return reinterpret_cast<f32x4*>(lds) + ((((part * C::WM + wm) * WN + wn) * MT + i) * NT + j) * 256 + lane;
+    };
+    if constexpr (WK > 1) {
+        static_for<MT * NT>([&](auto qc) {
+            constexpr int q = decltype(qc)::value, i = q / NT, j = q % NT;
+            if (q % WK == wk) return;  // uniform
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                area(wk, i, j)[64 * e] = f32x4{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
+        });
+        lds_barrier();
+    }
+    // The outputs of row tiles i0 .. i0 + IC - 1 of token tile j on their way out, the biases added.  WK > 1: the parts'
+    // sums are added in their order, from this wavefront's own on.
+    auto stage = [&](auto i0c, auto jc) {
+        constexpr int i0 = decltype(i0c)::value, j = decltype(jc)::value;
         static_for<IC>([&](auto ic) {
             constexpr int i = i0 + decltype(ic)::value;
+            f32x16 sum = acc[i][j];
+            if constexpr (WK > 1) {
+#pragma unroll
+                for (int q = 1; q < WK; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const f32x4 v = area((wk + q) % WK, i, j)[64 * e];
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) sum[4 * e + m] += v[m];
+                    }
+            }
 #pragma unroll
             for (int e4 = 0; e4 < 4; ++e4) {
                 const int o = i * 32 + 8 * e4 + 4 * h;  // of the wavefront's rows
                 float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * e4 + e];
+                for (int e = 0; e < 4; ++e) v[e] = sum[4 * e4 + e];
                 if constexpr (OT != OUT_PART) {
                     if (g.bias) {
                         const float4 bv = *reinterpret_cast<const float4*>(bias + o);
@@ -290,9 +315,26 @@ __global__ __launch_bounds__(64 * C::NW, C::MT* C::NT >= 16 ? 1 : 2) void k_half
                 *reinterpret_cast<float4*>(mine + c * PITCH + (o - 32 * i0) * 4) = float4{v[0], v[1], v[2], v[3]};
             }
         });
+    };
+    // A unit is what is on its way out at a time.  Only the registers it comes from are a unit's own code, what follows is in it
+    // once: a workgroup runs through it once or twice, and with a copy a unit and type the epilogue was 30 to 60 KB (with
+    // that, and the residual not fetched ahead beside a gate, 14336 x 4096 at 2048 rows 251 us in place of 234).
+    constexpr int UNITS = WK > 1 ? (MT * NT + WK - 1) / WK : NT;
+    auto tile_of = [&](int u) { return WK > 1 ? u * WK + wk : u; };
+#pragma unroll 1
+    for (int u = 0; u < UNITS; ++u) {
+        if (WK > 1 && tile_of(u) >= MT * NT) break;  // uniform
+        static_for<WK == 1 ? NT : MT * NT>([&](auto qc) {
+            constexpr int q = decltype(qc)::value;
+            if (q == tile_of(u)) stage(std::integral_constant<int, WK == 1 ? 0 : q / NT>{}, std::integral_constant<int, q % NT>{});
+        });
+        auto rows_of = [&](int u) { return WK > 1 ? tile_of(u) / NT : 0; };
+        auto tokens_of = [&](int u) { return tile_of(u) % NT; };
+        const int un = u + 1 < UNITS && (WK == 1 || tile_of(u + 1) < MT * NT) ? u + 1 : u;
+        const int i0 = rows_of(u), j = tokens_of(u), tb = t0 + (wn * NT + j) * 32, nb = n0 + wm * WR + 32 * i0;
         wave_lds_sync();
         if constexpr (OT != OUT_PART) {
-            // in place and in a loop, eight values at a time: each activation's code once
+            // in place, eight values at a time
             half_act_of(g.act, [&](auto act) {
                 constexpr int ACT = decltype(act)::value;
 #pragma unroll 1
@@ -308,125 +350,102 @@ __global__ __launch_bounds__(64 * C::NW, C::MT* C::NT >= 16 ? 1 : 2) void k_half
             });
         }
         const float* staged = reinterpret_cast<const float*>(mine);
-        if (nb + OC > g.n_out) {  // uniform: the last outputs, value by value
+        // Piece p of the unit: token p / ROW, outputs p % ROW * PER ..  (y may be gate or residual: what a lane writes
+        // it has read, and no other lane reads.)
+        const int n = nb + lo;
+        const bool whole = n + PER <= g.n_out;
 #pragma unroll 1
-            for (int p = lane; p < 32 * OC; p += 64) {
-                const int t = p / OC, n = nb + p % OC;
-                if (tb + t >= g.T || n >= g.n_out) continue;
-                float v = staged[t * (PITCH / 4) + n - nb];
-                if constexpr (OT == OUT_PART) {
-                    g.partial[((uint64_t)z * g.T + tb + t) * (uint64_t)g.n_out + n] = v;
+        for (int gi = 0; gi < GROUPS; ++gi) {
+            auto token = [&](int q) { return (64 * (GROUP * gi + q) + lane) / ROW; };
+            uint32_t out[GROUP][4];
+#pragma unroll
+            for (int q = 0; q < GROUP; ++q) {
+                const int t = token(q);
+                float v[PER];
+#pragma unroll
+                for (int e = 0; e < PER; e += 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(staged + t * (PITCH / 4) + lo + e);
+                    v[e] = f.x, v[e + 1] = f.y, v[e + 2] = f.z, v[e + 3] = f.w;
+                }
+                if constexpr (OT != OUT_PART) {
+                    float o[PER] = {};
+                    if (g.gate) {
+                        if (gates_ahead)
+                            half_unpack<PER>(g.gtype, gates[q], o);
+                        else if (tb + t < g.T && whole)
+                            half_load<PER>(g.gate, g.gtype, (uint64_t)(tb + t) * g.ldg + n, PER, o);
+#pragma unroll
+                        for (int e = 0; e < PER; ++e) v[e] = v[e] * o[e];
+                    }
+                    if (g.res) {
+                        if (res_ahead)
+                            half_unpack<PER>(g.rtype, sums[q], o);
+                        else if (tb + t < g.T && whole)
+                            half_load<PER>(g.res, g.rtype, (uint64_t)(tb + t) * g.ldr + n, PER, o);
+#pragma unroll
+                        for (int e = 0; e < PER; ++e) v[e] = v[e] + o[e];
+                    }
+                }
+                if constexpr (OT != OUT_16) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) out[q][e] = f2u(v[e]);
+                } else if (g.ytype == T_F16) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) out[q][e] = i8_half2<T_F16>(v[2 * e], v[2 * e + 1]);
                 } else {
-                    if (g.gate) v = v * half_at(g.gate, g.gtype, (uint64_t)(tb + t) * g.ldg + n);
-                    if (g.res) v = v + half_at(g.res, g.rtype, (uint64_t)(tb + t) * g.ldr + n);
-                    i8_store(g.y, g.ytype, (uint64_t)(tb + t) * g.ldy + n, v);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) out[q][e] = i8_half2<T_BF16>(v[2 * e], v[2 * e + 1]);
                 }
             }
-            // (tiles beside it may not be the last ones)
-            if constexpr (WK > 1) fetch(in, jn, 0, ahead[(decltype(unitc)::value + GROUPS) & 1]);
-        } else {
-            // Piece p of the tile: token p / ROW, outputs p % ROW * PER ..  A group's gate and residual are read before the
-            // first of its outputs is written (y may be either, and no other group's).
-            const int n = nb + lo;
-            static_for<GROUPS>([&](auto gc) {
-                constexpr int gi = decltype(gc)::value, now = (decltype(unitc)::value + gi) & 1;
-                if constexpr (gi + 1 < GROUPS)
-                    fetch(i0, j, gi + 1, ahead[1 - now]);
+            const bool on = gi + 1 < GROUPS;
+            fetch(on ? i0 : rows_of(un), on ? j : tokens_of(un), on ? gi + 1 : 0);
+#pragma unroll
+            for (int q = 0; q < GROUP; ++q) {
+                const int t = token(q);
+                if (tb + t >= g.T || !whole) continue;
+                if constexpr (OT == OUT_PART)
+                    __builtin_memcpy(g.partial + ((uint64_t)z * g.T + tb + t) * (uint64_t)g.n_out + n, out[q], 16);
+                else if constexpr (OT == OUT_F32)
+                    __builtin_memcpy((float*)g.y + (uint64_t)(tb + t) * g.ldy + n, out[q], 16);
                 else
-                    fetch(in, jn, 0, ahead[1 - now]);
-                float res[GROUP][PER];
-                auto token = [&](int q) { return (64 * (GROUP * gi + q) + lane) / ROW; };
-                if constexpr (OT != OUT_PART) {
-                    if (g.gate && g.res) {
+                    __builtin_memcpy((uint16_t*)g.y + (uint64_t)(tb + t) * g.ldy + n, out[q], 16);
+            }
+        }
+        // The outputs behind the last whole piece, value by value, their operands' loads before the first is waited for (all of
+        // a ragged tile's outputs in turn took 21 of 39 us of 12976 x 1024 at 256 rows with a residual).
+        const int left = g.n_out - nb, e0 = left / PER * PER, ragged = left - e0;
+        if (left < OC && ragged > 0) {  // uniform
+            constexpr int MOST = (32 * (PER - 1) + 63) / 64;
+            float gate[MOST], res[MOST];
+            auto place = [&](int m, int& t, int& n) {
+                const int p = 64 * m + lane;
+                t = p / ragged, n = e0 + p % ragged;
+                return t < 32 && tb + t < g.T;
+            };
+            if constexpr (OT != OUT_PART) {
 #pragma unroll
-                        for (int q = 0; q < GROUP; ++q)
-                            if (tb + token(q) < g.T)
-                                half_load<PER>(g.res, g.rtype, (uint64_t)(tb + token(q)) * g.ldr + n, PER, res[q]);
-                    }
+                for (int m = 0; m < MOST; ++m) {
+                    int t, n;
+                    if (!place(m, t, n)) continue;
+                    if (g.gate) gate[m] = half_at(g.gate, g.gtype, (uint64_t)(tb + t) * g.ldg + nb + n);
+                    if (g.res) res[m] = half_at(g.res, g.rtype, (uint64_t)(tb + t) * g.ldr + nb + n);
                 }
+            }
 #pragma unroll
-                for (int q = 0; q < GROUP; ++q) {
-                    const int t = token(q);
-                    if (tb + t >= g.T) continue;
-                    float v[PER];
-#pragma unroll
-                    for (int e = 0; e < PER; e += 4) {
-                        const float4 f = *reinterpret_cast<const float4*>(staged + t * (PITCH / 4) + lo + e);
-                        v[e] = f.x, v[e + 1] = f.y, v[e + 2] = f.z, v[e + 3] = f.w;
-                    }
-                    if constexpr (OT == OUT_PART) {
-                        __builtin_memcpy(g.partial + ((uint64_t)z * g.T + tb + t) * (uint64_t)g.n_out + n, v, 16);
-                    } else {
-                        if (op) {
-                            float o[PER];
-                            half_unpack<PER>(otype, ahead[now][q], o);
-                            if (g.gate) {
-#pragma unroll
-                                for (int e = 0; e < PER; ++e) v[e] = v[e] * o[e];
-                                if (g.res) {
-#pragma unroll
-                                    for (int e = 0; e < PER; ++e) v[e] = v[e] + res[q][e];
-                                }
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < PER; ++e) v[e] = v[e] + o[e];
-                            }
-                        }
-                        const uint64_t to = (uint64_t)(tb + t) * g.ldy + n;
-                        if constexpr (OT == OUT_F32) {
-                            __builtin_memcpy((float*)g.y + to, v, 16);
-                        } else {
-                            uint32_t w[4];
-                            if (g.ytype == T_F16) {
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) w[e] = i8_half2<T_F16>(v[2 * e], v[2 * e + 1]);
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) w[e] = i8_half2<T_BF16>(v[2 * e], v[2 * e + 1]);
-                            }
-                            __builtin_memcpy((uint16_t*)g.y + to, w, 16);
-                        }
-                    }
+            for (int m = 0; m < MOST; ++m) {
+                int t, n;
+                if (!place(m, t, n)) continue;
+                float v = staged[t * (PITCH / 4) + n];
+                if constexpr (OT == OUT_PART) {
+                    g.partial[((uint64_t)z * g.T + tb + t) * (uint64_t)g.n_out + nb + n] = v;
+                } else {
+                    if (g.gate) v = v * gate[m];
+                    if (g.res) v = v + res[m];
+                    i8_store(g.y, g.ytype, (uint64_t)(tb + t) * g.ldy + nb + n, v);
                 }
-            });
+            }
         }
         wave_lds_sync();
-        __builtin_amdgcn_sched_barrier(0);  // (the sums of one token tile at a time in vector registers)
-    };
-    if constexpr (WK == 1) {
-        static_for<NT>([&](auto jc) {
-            constexpr int j = decltype(jc)::value;
-            emit(jc, std::integral_constant<int, 0>{}, std::integral_constant<int, j * GROUPS>{}, 0, j + 1 < NT ? j + 1 : j);
-        });
-    } else {
-        // output tile u goes to the wavefront of part u % WK: the others' sums of it through LDS, added in the
-        // parts' order from its own on
-        auto area = [&](int part, int i, int j) {
-            return reinterpret_cast<f32x4*>(lds) + ((((part * C::WM + wm) * WN + wn) * MT + i) * NT + j) * 256 + lane;
-        };
-        static_for<MT * NT>([&](auto uc) {
-            constexpr int u = decltype(uc)::value, i = u / NT, j = u % NT;
-            if (u % WK == wk) return;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                area(wk, i, j)[64 * e] = f32x4{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
-        });
-        lds_barrier();
-        static_for<MT * NT>([&](auto uc) {
-            constexpr int u = decltype(uc)::value, i = u / NT, j = u % NT;
-            if (u % WK != wk) return;  // uniform
-#pragma unroll
-            for (int q = 1; q < WK; ++q)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const f32x4 v = area((wk + q) % WK, i, j)[64 * e];
-#pragma unroll
-                    for (int m = 0; m < 4; ++m) acc[i][j][4 * e + m] += v[m];
-                }
-            constexpr int next = u + WK < MT * NT ? u + WK : u;
-            emit(std::integral_constant<int, j>{}, std::integral_constant<int, i>{}, std::integral_constant<int, u / WK * GROUPS>{},
-                 next / NT, next % NT);
-        });
     }
 }
 
