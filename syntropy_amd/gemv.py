@@ -375,6 +375,8 @@ def block_norm(x: torch.Tensor, branch: torch.Tensor | None, g: torch.Tensor | N
     if g is None and x.dim() != 2:
         raise GemvError("Len", "x must be rows of values where no norm's weights say how many")
     device = x.get_device()
+    if device < 0:
+        raise GemvError("Len", "`x` must be on a device")
     if stream is None and device == _current_device():
         return _block_norm(x, branch, g, eps, rows, post, gate, scale, h, y, dtype, device, _current_stream(device))
     return _on_stream(x, stream, lambda handle: _block_norm(x, branch, g, eps, rows, post, gate, scale, h, y, dtype, device, handle))
