@@ -1,9 +1,8 @@
 """How the calls of the half-precision product, the norms between blocks and the sampling are launched, on the CPU
-(host/block_launches.cpp): limits of LDS, shapes of grids, every kernel by the device tests' cases, and the host code
-under sanitizers over the ends of every size and type."""
+(host/block_launches.cpp): limits of LDS, shapes of grids, every kernel by the device tests' cases, the ends of every
+size and type."""
 import itertools
 import os
-import shutil
 import subprocess
 
 import pytest
@@ -11,8 +10,6 @@ import pytest
 import host_launches as H
 from host_launches import BF16, F16, F32
 from syntropy_amd import _lib
-from syntropy_amd import build as B
-from test_host_sanitizers import CLANG, ENV, SAN
 
 NONE = 9
 TYPES = (F32, F16, BF16)
@@ -111,13 +108,3 @@ def at_their_ends(exe, env=None):
 
 def test_sizes_at_their_ends(exe):
     at_their_ends(exe)
-
-
-@pytest.mark.skipif(not (os.path.exists(B.HIPCC) and os.path.exists(CLANG)), reason="needs hipcc and ROCm's clang++ with its sanitizer runtimes")
-def test_sizes_at_their_ends_under_sanitizers(tmp_path_factory):
-    out = str(tmp_path_factory.mktemp("sanitized_block"))
-    try:
-        B.build_host_sanitized(out)
-        at_their_ends(program(out, out, SAN), dict(os.environ, **ENV))
-    finally:
-        shutil.rmtree(out, ignore_errors=True)
