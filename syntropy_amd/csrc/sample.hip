@@ -434,19 +434,28 @@ struct Sampler : Reader<TY> {
         }
         __syncthreads();
     }
-    // (one wavefront) The least values of the bins from a1, a0 - 1, b and b - 1 up, the wanted ones' edges: by 16 numbers at
-    // a time between one that is below and one that is not, 16 lanes an edge.
+    // (one wavefront) The least values of the bins from a1, a0 - 1, b and b - 1 up, the wanted ones' edges, 16 lanes an edge: by
+    // 16 numbers at a time between one that is below and one that is not, at first the eight on either side of where the
+    // edge lies in 64 bits, where it lies among them (it does but for the rounding of F32 distances).
     SYN_DEV void edges(Mode mode, Wanted& w) const {
         const int l = threadIdx.x & 63, group = l >> 4;
         const int at = group == 0 ? w.a1 : group == 1 ? (mode == BINS ? w.a0 - 1 : -1) : w.b < 0 ? -1 : group == 2 ? w.b : w.b - 1;
-        uint32_t lo = KEY_NONE, hi = sp_order((float)sc.m);
+        auto in = [&](uint32_t key) {
+            const float v = sp_value(key);
+            return mode == LIST_MIN_P ? sc.s(v) <= last : (mode == LIST_K ? bin32(v) : Scale::bin(sc.s(v))) <= at;
+        };
+        const uint32_t top = sp_order((float)sc.m);
+        const double s = mode == LIST_MIN_P ? last : (double)at + (mode == LIST_K ? 1.0 : 0.5);
+        const uint32_t near = sp_order((float)(sc.m - s / sc.c));
+        uint32_t lo = near > KEY_NONE + 8 ? near - 8 : KEY_NONE, hi = near + 8 < top ? near + 8 : top;
+        if (lo > KEY_NONE && (lo >= top || in(lo))) lo = KEY_NONE;
+        if (hi <= lo || !in(hi)) hi = top;
+        if (at < 0 && mode != LIST_MIN_P) lo = hi - 1;  // (none)
 #pragma unroll 1
-        for (int i = 0; i < 9; ++i) {
+        for (int i = 0; i < 9 && __builtin_amdgcn_ballot_w64(hi - lo > 1) != 0; ++i) {
             const uint32_t step = (hi - lo + 15) >> 4, up = lo + step * (uint32_t)((l & 15) + 1);
             const uint32_t t = up < hi && up > lo ? up : hi;
-            const float v = sp_value(t);
-            const bool in = mode == LIST_MIN_P ? sc.s(v) <= last : (mode == LIST_K ? bin32(v) : Scale::bin(sc.s(v))) <= at;
-            const uint32_t yes = (uint32_t)(__builtin_amdgcn_ballot_w64(in || t == hi) >> (16 * group)) & 0xFFFFu;
+            const uint32_t yes = (uint32_t)(__builtin_amdgcn_ballot_w64(in(t) || t == hi) >> (16 * group)) & 0xFFFFu;
             const int f = __builtin_ctz(yes);
             const uint32_t to = lo + step * (uint32_t)(f + 1);
             hi = to < hi && to > lo ? to : hi;
