@@ -265,9 +265,10 @@ int syn_token_logprobs(int32_t xtype, const void* x, uint64_t x_stride, uint32_t
 
 /* ---- Products over half-precision weights with an epilogue ---------------------------------------
  * y = act(x W^T + bias) gate + residual over W [n_out, k_in] and x [rows, k_in] of wtype (SYN_F16 or SYN_BF16):
- * products of the values as they are, sums in F32 (in an order that depends on n_out, k_in and rows alone), then the
- * epilogue in F32, rounded once, to y's type.  syn_gemv over F16 and BF16 weights is the product of F32 activations in the
- * reference's order; this one has no counterpart there.
+ * products of the values as they are, sums in F32, then the epilogue in F32, rounded once, to y's type.  The order of a
+ * sum depends on n_out, k_in and rows alone where w_stride and x_stride are below 2^22 values; rows farther apart than a
+ * tile's 32-bit offsets reach (2^31 bytes over its 32 to 256 rows) are summed as 3 to 8 rows are.  syn_gemv over F16 and
+ * BF16 weights is the product of F32 activations in the reference's order; this one has no counterpart there.
  *   act: SYN_ACT_*: none, relu, silu(v) = v / (1 + exp(-v)), gelu(v) = v Phi(v), and its tanh form
  *     v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2;
  *   bias F32 [n_out], gate and residual [rows, n_out] (F32, F16 or BF16): each may be NULL.

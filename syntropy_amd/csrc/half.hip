@@ -72,7 +72,7 @@ void launch_half_gemv(const HalfArgs& in, bool lines, uint8_t* ws, hipStream_t s
         a.x = (const uint16_t*)ws;
         a.ldx = (uint64_t)kp;
     }
-    // (rows may be so far apart that a tile's offsets pass 32 bits)
+    // (rows may be so far apart that a tile's offsets pass 32 bits: their sums have the few-token form's order)
     if (!half_gemm_reaches(p.tile, a)) {
         launch_half_few(a, stream);
         return;
