@@ -322,7 +322,8 @@ int syn_block_norm(int32_t xtype, const void* x, uint64_t x_stride, int32_t btyp
  * least above it, min_p below 0 as 0 and above 1 as 1; u outside [0, 1) as the nearest in it.  A row with a NaN or
  * +infinity among its logits, with no visible logit, or with a NaN setting, u, or a temperature that is none of the
  * above has the token -1, kept 0 and logprob NaN.
- * Sums are held to about 2^-62 vocab of a weight, in an order that does not matter: equal calls give equal tokens.
+ * Each sum is within 2^(11 - b) of its value, b = min(50, 62 - log2 vocab rounded up) (2^-34 at 128256 logits), and added up in
+ * an order that does not matter: equal calls give equal tokens.
  * Weights below 2^-64 of the greatest count as that at most.  Fewer than 2^24 rows of at most SYN_SAMPLE_MAX_VOCAB logits.
  * ws: 256-byte aligned, syn_sample_tokens_workspace_bytes (0: may be NULL).  No counterpart in the reference. */
 #define SYN_SAMPLE_MAX_VOCAB (1 << 24)

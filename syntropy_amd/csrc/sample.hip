@@ -6,10 +6,13 @@
 // T = 0 stands for top-k 1.
 //
 // A token and a count are whole numbers, and the borders between tokens are as near to one another as 1e-6 of W, so
-// sums are exact to about 2^-44 of a weight whatever their order: with t_i = (max x - x_i) log2(e) / T in 64 bits,
-// values are put in bins of 1/32 of t, and a bin's weights are added as whole numbers of 2^-bits of the weight in
+// sums have to be exact to far less than that, and the same whatever their order: with t_i = (max x - x_i) log2(e) / T in
+// 64 bits, values are put in bins of 1/32 of t, and a bin's weights are added as whole numbers of 2^-bits of the weight in
 // the bin's middle.  A bin is a run of the order; a prefix of the order is whole bins, whose sums are whole numbers
 // too, of 2^-bits of the greatest weight, and a part of one, whose values are put in order as a list.
+// A weight is off by 2^-48 of itself (the exponential's polynomial) and half of its whole number's 1, equal logits all the
+// same way; a bin's sum by half of 2^-bits of the greatest weight, which is 2^(10 - bits) over all bins and the most of it.
+// bits is min(50, 62 - log2 vocab rounded up), 45 at 128256 logits: together below 2^(11 - bits) of the row's sum.
 //
 // The row is read for its greatest value, for the bins, and for the list: the few values that a border or the token can
 // lie among.  A top-k needs no bins: up to TOP the k-th of the 256 groups' greatest values is a bound that only a few
@@ -357,8 +360,8 @@ struct Sampler : Reader<TY> {
             each([&](float v, int) { add_to_bin(v, beyond); });
         add_beyond(beyond);
     }
-    // (every thread) The counts and sums of the bins before each, in place.  (Whole numbers: a sum grows exactly where a bin
-    // holds something.)
+    // (every thread) The counts and sums of the bins before each, in place.  (A bin's sum to the nearest whole number: where
+    // it is below half of 1 nothing is added, and no sum that is looked for lies there.)
     SYN_DEV void prefix() {
         static_assert(SB == 2 * ST, "two bins a thread");
         const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, b = 2 * (int)threadIdx.x;
