@@ -151,7 +151,8 @@ SYN_DEV float i8_value(int sum, float sx, float sw) { return ((float)sum * sx) *
 // result, and a quotient that is one rounds once.  Below -111 the power is infinite and the quotient 0 (a value
 // below 2^-150).  An infinite or NaN g is met in the product with g.  (14336 x 4096 gated at 1024 tokens 138.7 us;
 // 137.2 with neither the rest of log2(e) nor the values below -88.)
-// i8_times_sigmoid(v, z, rest) is v / (1 + exp(-z - rest)), rest far below z; silu(g) with both g.
+// i8_times_sigmoid(v, z, rest) is v / (1 + exp(-z) 2^-rest), rest (what z was rounded by, times log2(e)) far below z;
+// silu(g) with both g.
 SYN_DEV float i8_times_sigmoid(float v, float z, float rest) {
     constexpr float LOG2E = 1.44269504088896340736f, LOG2E_REST = (float)(1.44269504088896340736 - (double)LOG2E);
     const bool far = z < -80.0f;
