@@ -53,7 +53,7 @@ struct HalfTile {
 enum HalfOut { OUT_PART, OUT_F32, OUT_16 };  // the sums of a part of K; F32; F16 or BF16
 
 template <class C, int WTY, int OT>
-__global__ __launch_bounds__(64 * C::NW, C::MT* C::NT >= 16 ? 1 : 2) void k_half_gemm(HalfArgs g, int tiles_w, int tiles_t) {
+__global__ __launch_bounds__(64 * C::NW, 2) void k_half_gemm(HalfArgs g, int tiles_w, int tiles_t) {
     constexpr int WN = C::WN, WK = C::WK, MT = C::MT, NT = C::NT, RING = C::RING, LINE = C::LINE;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int lane = threadIdx.x & 63;
