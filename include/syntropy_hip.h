@@ -273,7 +273,7 @@ int syn_token_logprobs(int32_t xtype, const void* x, uint64_t x_stride, uint32_t
  *     v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2;
  *   bias F32 [n_out], gate and residual [rows, n_out] (F32, F16 or BF16): each may be NULL.
  * W's rows are w_stride values apart, a multiple of 8, each on 16 bytes and followed by ZEROS up to a multiple of 128
- * values (w_stride is at least that, and the view w_bytes reaches the last row's).  Rows of x, gate, residual and y
+ * values (w_stride is at least that and at most 2^30, and the view w_bytes reaches the last row's).  Rows of x, gate, residual and y
  * are x_stride, ... values apart, at any value's address; x's are read as they lie where k_in is a multiple of 128,
  * x on 16 bytes and x_stride a multiple of 8 (x_aligned in the workspace's query: 1 for that, 0 for any), else through
  * a copy in the workspace.  residual or gate may be y itself (address, stride and type); y overlaps no operand

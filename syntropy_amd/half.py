@@ -21,13 +21,14 @@ from .gemv import GemvError, _current_device, _current_stream, _need, _on_stream
 MAX_K = 1 << 20
 ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 _PAIR = 128  # values of two 128-byte lines
+_MAX_STRIDE = 1 << 30
 
 
 @dataclass(frozen=True, eq=False)
 class Weights:
     """`matrix` F16 or BF16 [n_out, k_in] with an optional F32 `bias` [n_out], device tensors.  A matrix whose rows are
-    whole pairs of 128-byte lines (k_in a multiple of 128) on 16 bytes is kept as it is; any other is copied once, here,
-    into such rows with zeros behind the values."""
+    whole pairs of 128-byte lines (k_in a multiple of 128) on 16 bytes, at most 2^30 values apart, is kept as it is; any
+    other is copied once, here, into such rows with zeros behind the values."""
 
     matrix: torch.Tensor
     bias: torch.Tensor | None = None
@@ -41,7 +42,7 @@ class Weights:
             raise GemvError("RowLength", f"rows of {k_in} values (1 to {MAX_K})")
         if b is not None and (b.device != w.device or b.dtype != torch.float32 or not b.is_contiguous() or b.shape != (n_out,)):
             raise GemvError("Len", f"bias must be a contiguous F32 tensor of {n_out} values beside the matrix")
-        if k_in % _PAIR or w.stride(1) != 1 or w.stride(0) < k_in or w.stride(0) % 8 or w.data_ptr() % 16:
+        if k_in % _PAIR or w.stride(1) != 1 or not k_in <= w.stride(0) <= _MAX_STRIDE or w.stride(0) % 8 or w.data_ptr() % 16:
             rows = torch.zeros(n_out, -(-k_in // _PAIR) * _PAIR, dtype=w.dtype, device=w.device)[:, :k_in]
             w = rows.copy_(w)
         stride = w.stride(0)
