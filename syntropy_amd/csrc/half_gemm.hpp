@@ -144,8 +144,10 @@ __global__ __launch_bounds__(64 * C::NW, 2) void k_half_gemm(HalfArgs g, int til
         });
     };
 
-    // What the epilogue reads of gate and residual is fetched a unit of it ahead, the first unit before all else: a unit
-    // waits for memory otherwise, with nothing beside it.  (F32 operands of an output of 16 bits, twice as long, are not.)
+    // What the epilogue reads of gate and residual is fetched a group of pieces ahead, the first group before all else.  Within
+    // a unit a group is under way beside the one before.  A unit's first group is not: the wait for LDS at the end of the
+    // unit before is one for all memory, that unit's stores too.  (F32 operands of an output of 16 bits, twice as
+    // long, are not fetched ahead.)
     constexpr int IC = WK > 1 ? 1 : MT;                           // row tiles of an emission
     constexpr int OC = 32 * IC, PITCH = OC * 4 + 16;
     constexpr int PER = OT == OUT_16 ? 8 : 4, ROW = OC / PER;     // values of 16 bytes, pieces a token
