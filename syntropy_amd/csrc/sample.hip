@@ -120,6 +120,7 @@ struct Wanted {
     int n0, i0, end;
     uint32_t before, total;
     double sum0, sum1, under, all;
+    double to;  // of the other modes: about how far its last value lies
 };
 
 // A place in the order: how many values reach it, their sum, and the key of the last one.
@@ -422,6 +423,7 @@ struct Sampler : Reader<TY> {
             Wanted w{};
             w.b = w.cut = -1;
             w.lo = b > KEY_NONE ? sp_value(b) : sp_value(KEY_NONE + 1);
+            w.to = b > KEY_NONE ? sc.s(w.lo) : (double)(SB - 1);
             w.hi = w.lo2 = w.hi2 = __builtin_inff();
             if (threadIdx.x == 0) r.want = w;
         }
@@ -471,11 +473,13 @@ struct Sampler : Reader<TY> {
     SYN_DEV Wanted wanted(Mode mode) const {
         Wanted w{};
         w.b = w.cut = -1;
+        w.to = last;
         if (mode == LIST_MIN_P) return w;
         w.n = (uint32_t)LIST + 1;
         if (mode == LIST_K) {
             w.a1 = bin_of(AT_LEAST_N, k, 0.0);
             w.n = r.counts[w.a1 + 1];
+            w.to = (double)w.a1 + 1.0;
             return w;
         }
         if (k < r.counts[SB]) return w;  // (a top-k longer than a list: its border, then the others', in seldom())
@@ -727,9 +731,7 @@ struct Sampler : Reader<TY> {
                 const int a1 = r.want.a1, b = r.want.b;
                 order((int)n, (double)r.want.a0 - 0.5, b >= 0 ? (double)(b - a1 - 1) : 0.0, (double)a1 + (b >= 0 ? 1.5 : 0.5));
             } else {
-                const float lo = r.want.lo;  // (of a top-k: its bound, or where it bounds nothing the lowest value)
-                order((int)n, 0.0, 0.0, mode == LIST_MIN_P ? last : mode == LIST_K ? (double)r.want.a1 + 1.0
-                                        : lo > sp_value(KEY_NONE + 1) ? sc.s(lo) : (double)(SB - 1));
+                order((int)n, 0.0, 0.0, r.want.to);
             }
             const bool only = r.want.only;
             if (only) __syncthreads();
